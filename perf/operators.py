@@ -6,7 +6,7 @@ Three operators of a language model's training step stand around the sparse laye
          pieces of the vocabulary without keeping the logits, with the gradients of x and W
   norm   residual_norm: the norm after a block (optional), its gate and residual scale, the residual
          add and the norm before the next block in one pass, forward and backward
-  adamw  adamw_step: one AdamW step over a list of tensors (dense ones and the padded value arrays of
+  adamw  AdamWPlan: one AdamW step over a list of tensors (dense ones and the padded value arrays of
          sparse weights, whose padding slots are left alone), with moments in 32 or in 8 bits
 
 ``own`` false: the plain form, elementary torch operations in 32 bits (rounded once at the end);
@@ -330,8 +330,9 @@ def _adamw(s):
     if own:
         import sparsecore_b200 as sl
 
-        sl.adamw_step(s["params"], s["g"], s["ms"], s["vs"], step=s["step"], lr=LR, betas=BETAS, eps=EPS, weight_decay=DECAY,
-                      live=s["live"], scales=s["scales"], seed=s["seed"])
+        if "plan" not in s:  # what a program keeps from step to step: its tensors' table
+            s["plan"] = sl.AdamWPlan(s["params"], s["ms"], s["vs"], live=s["live"], scales=s["scales"])
+        s["plan"].step(s["g"], step=s["step"], lr=LR, betas=BETAS, eps=EPS, weight_decay=DECAY, seed=s["seed"])
     else:
         scales = s["scales"] or [None] * len(s["params"])
         [_adamw_one(p, g, m, v, live, sc, s["step"], s["seed"], i) for i, (p, g, m, v, live, sc) in
