@@ -366,6 +366,96 @@ SL_API int sl_unpack_live_batch(const sl_live_desc* descs, int64_t n_descs, int6
 SL_API int sl_exclusive_scan(const int32_t* counts, int64_t n, int32_t* out,
                       int64_t* total_dev, void* stream);
 
+/* ── The dense part of a training step ───────────────────────────────────
+ * No reference counterpart: the reference runs stock torch for its norms,
+ * loss and optimizer (sparselab/nn.py:183-184, examples/demo_15_mini_gpt.py).
+ * Element types of the calls below. */
+enum { SL_F32 = 0, SL_BF16 = 1, SL_F16 = 2 };
+
+/* One tensor of an AdamW step.  m and v are float[n] (state_bits 32) or
+ * e4m3 bytes [n] with one fp32 scale per SL_ADAMW_BLOCK elements in scale_m
+ * and scale_v, v then holding the second moment's square root (state_bits
+ * 8).  live: int32[n] column indices of a padded CSR (slots below 0 are left
+ * alone), or NULL.  number: the tensor's number in the caller's list, which
+ * its dither bits depend on. */
+enum { SL_ADAMW_BLOCK = 256 };
+typedef struct sl_adamw_item {
+    void* p;
+    const void* g;
+    void* m;
+    void* v;
+    float* scale_m;
+    float* scale_v;
+    const int32_t* live;
+    int64_t n;
+    int64_t number;
+} sl_adamw_item;
+/* AdamW with decoupled weight decay over `count` tensors (a HOST array) of
+ * one element type (p and g), in place; up to 384 tensors a launch.
+ * hyper_dev: NULL, or what sl_adamw_hyper wrote (lr ... seed are then not
+ * read). */
+SL_API int sl_adamw_multi(const sl_adamw_item* items, int64_t count, int dtype, int state_bits, double lr,
+                   double beta1, double beta2, double eps, double weight_decay, int64_t step,
+                   uint32_t seed, const void* hyper_dev, void* stream);
+/* The same step's numbers made on the device, for captured steps: adds 1 to
+ * *step_dev and writes sl_adamw_hyper_bytes() bytes to hyper_dev.  lr_dev: a
+ * learning rate on the device, or NULL to take `lr`. */
+SL_API int64_t sl_adamw_hyper_bytes(void);
+SL_API int sl_adamw_hyper(int64_t* step_dev, const float* lr_dev, double lr, double beta1, double beta2,
+                   double eps, double weight_decay, uint32_t seed, void* hyper_dev, void* stream);
+
+/* The norms around a block with its gate, residual scale and residual add:
+ *   u = N(y; post_weight, post_bias), or y where post_weight is NULL
+ *   out = residual + scale * gate * u;   h = N(out; weight, bias)
+ * rows x cols operands, contiguous.  y, h, dh, dy have type `dtype`;
+ * residual, out, dout, dresidual `residual_dtype`; the vectors and their
+ * gradients `weight_dtype`; gate and dgate `gate_dtype` (each `dtype` or
+ * SL_F32).  gate: [gate_groups, cols], each row shared by rows / gate_groups
+ * rows, or NULL.  scale_dev: a scale on the device in place of `scale`.
+ * stats: float[4 * rows], written by the forward call (NULL: not kept) and
+ * read by the backward one.  backward writes dresidual and every other
+ * gradient whose pointer is set, from dout and dh (NULL: zero); workspace:
+ * sl_norm_workspace_bytes() bytes. */
+enum { SL_NORM_LAYER = 0, SL_NORM_RMS = 1, SL_NORM_MAX_COLS = 16384 };
+typedef struct sl_norm_args {
+    const void* y;
+    const void* residual;
+    const void* weight;
+    const void* bias;
+    const void* gate;
+    const void* post_weight;
+    const void* post_bias;
+    void* out;
+    void* h;
+    float* stats;
+    const float* scale_dev;
+    const void* dout;
+    const void* dh;
+    void* dresidual;
+    void* dy;
+    void* dgate;
+    void* dweight;
+    void* dbias;
+    void* dpost_weight;
+    void* dpost_bias;
+    float* dscale;
+    void* workspace;
+    int64_t rows;
+    int64_t cols;
+    int64_t gate_groups;
+    float scale;
+    float eps;
+    float post_eps;
+    int kind;
+    int dtype;
+    int residual_dtype;
+    int weight_dtype;
+    int gate_dtype;
+} sl_norm_args;
+SL_API int64_t sl_norm_workspace_bytes(int64_t rows, int64_t cols, int64_t gate_groups);
+SL_API int sl_norm_forward(const sl_norm_args* args, void* stream);
+SL_API int sl_norm_backward(const sl_norm_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

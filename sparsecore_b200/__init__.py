@@ -7,6 +7,9 @@ A drop-in for the reference ``sparselab`` package's sparse-training path:
     SparseLinear       nn.Linear replacement backed by a PaddedCSR
     SparsityAlgorithm, DynamicSparsityAlgorithm, Static, SET, RigL
                        dynamic-sparsity routers (GPU prune / regrow)
+    residual_norm      the norms around a block with its gate, scale and residual add
+    FusedAdamW, AdamWPlan, adamw_step
+                       AdamW over all tensors in one launch, moments in 32 or 8 bits
 
 ``import sparsecore_b200 as sparselab`` gives the reference's names.  Every
 kernel runs in the in-tree CUDA library ``_lib/libsparsecore_b200.so``
@@ -18,6 +21,8 @@ from . import layout
 from .layout import PaddedCSR, transpose_with_perm
 from .ops import critical_path_stream, set_async_weight_grad, spmm
 from .nn import SparseLinear, sparse_mlp
+from .norm import residual_norm
+from .optim import AdamWPlan, FusedAdamW, LiveAdamW, adamw_step
 from .router import SparsityAlgorithm, Static, DynamicSparsityAlgorithm, SET, RigL, dense_grad
 from . import torch_ops  # registers torch.ops.sparselab.spmm_fwd / sddmm_dw
 
@@ -26,6 +31,11 @@ __all__ = [
     "spmm",
     "SparseLinear",
     "sparse_mlp",
+    "residual_norm",
+    "AdamWPlan",
+    "FusedAdamW",
+    "LiveAdamW",
+    "adamw_step",
     "SparsityAlgorithm",
     "DynamicSparsityAlgorithm",
     "Static",

@@ -39,6 +39,20 @@ class SlCsr(ctypes.Structure):
     ]
 
 
+class SlNormArgs(ctypes.Structure):
+    """Mirror of `sl_norm_args`."""
+
+    _fields_ = ([(n, P) for n in ("y", "residual", "weight", "bias", "gate", "post_weight", "post_bias", "out", "h",
+                                  "stats", "scale_dev", "dout", "dh", "dresidual", "dy", "dgate", "dweight", "dbias",
+                                  "dpost_weight", "dpost_bias", "dscale", "workspace")]
+                + [(n, I64) for n in ("rows", "cols", "gate_groups")] + [(n, F32) for n in ("scale", "eps", "post_eps")]
+                + [(n, I32) for n in ("kind", "dtype", "residual_dtype", "weight_dtype", "gate_dtype")])
+
+
+# Element types of the training step's dense operators (SL_F32 ...).
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+byref = ctypes.byref
+
 # name -> (restype, argtypes); every symbol the header declares.
 SIGNATURES: dict[str, tuple] = {
     "sl_last_error": (ctypes.c_char_p, []),
@@ -83,6 +97,12 @@ SIGNATURES: dict[str, tuple] = {
     "sl_unpack_live_batch": (I32, [P, I64, I64, P, P]),
     "sl_transpose_f32": (I32, [P, I64, I64, P, P]),
     "sl_transpose_bias_f32": (I32, [P, I64, I64, P, P, P]),
+    "sl_adamw_multi": (I32, [P, I64, I32, I32, F64, F64, F64, F64, F64, I64, ctypes.c_uint32, P, P]),
+    "sl_adamw_hyper_bytes": (I64, []),
+    "sl_adamw_hyper": (I32, [P, P, F64, F64, F64, F64, F64, ctypes.c_uint32, P, P]),
+    "sl_norm_workspace_bytes": (I64, [I64, I64, I64]),
+    "sl_norm_forward": (I32, [P, P]),
+    "sl_norm_backward": (I32, [P, P]),
     "sl_set_regrow_draws": (I32, [P, P, P, I64, P, P, I64, P, P, I64, P]),
 }
 
@@ -155,6 +175,7 @@ KERNELS_PER_CALL = {
     "sl_unpack_live_batch": 1, "sl_exclusive_scan": 1,
     "sl_set_regrow_draws": 0,  # host only
     "sl_probe_ffma": 1, "sl_probe_smem": 1,
+    "sl_adamw_multi": 1, "sl_adamw_hyper": 1, "sl_norm_forward": 1, "sl_norm_backward": 2,
 }
 launches = {"count": 0}
 
@@ -171,6 +192,34 @@ def call(name: str, *args) -> None:
     rc = fn(*args)
     launches["count"] += KERNELS_PER_CALL.get(name, 1)
     check(rc, name)
+
+
+def lib_on(device: torch.device) -> ctypes.CDLL:
+    """The library, for queries whose answer depends on `device` (its SM count)."""
+    if torch.cuda.current_device() == device.index:
+        return lib()
+    return _OnDevice(device)
+
+
+class _OnDevice:
+    def __init__(self, device):
+        self.device = device
+
+    def __getattr__(self, name):
+        def fn(*args):
+            with torch.cuda.device(self.device):
+                return getattr(lib(), name)(*args)
+        return fn
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` on `device`, whichever device is current, with that device's
+    current stream as the last argument."""
+    if torch.cuda.current_device() == device.index:
+        call(name, *args, stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream_ptr(device))
 
 
 def check(rc: int, fn: str = "") -> None:
