@@ -456,6 +456,40 @@ SL_API int64_t sl_norm_workspace_bytes(int64_t rows, int64_t cols, int64_t gate_
 SL_API int sl_norm_forward(const sl_norm_args* args, void* stream);
 SL_API int sl_norm_backward(const sl_norm_args* args, void* stream);
 
+/* Softmax cross entropy of the logits x . weight^T against target tokens,
+ * in pieces of the vocabulary: the logits are never stored.  x [tokens, dim]
+ * and weight [vocab, dim] contiguous of one type, targets int64[tokens].
+ * A token whose target is ignore_index counts for nothing (its row of x is
+ * not read into anything); one whose target is outside [0, vocab) has a NaN
+ * loss.  loss: one float (mean over the tokens that count, or sum);
+ * loss_rows: float[tokens], written where set (required with
+ * SL_XENT_NONE).  prep (kept from forward to backward) and scratch: sizes by
+ * sl_xent_sizes, 256-byte aligned.  backward: grad is one float (mean, sum)
+ * or float[tokens]; dx [tokens, dim] and dweight [vocab, dim] are written
+ * where set. */
+enum { SL_XENT_MEAN = 0, SL_XENT_SUM = 1, SL_XENT_NONE = 2 };
+typedef struct sl_xent_args {
+    const void* x;
+    const void* weight;
+    const int64_t* targets;
+    float* loss;
+    float* loss_rows;
+    void* prep;
+    void* scratch;
+    const float* grad;
+    void* dx;
+    void* dweight;
+    int64_t tokens;
+    int64_t dim;
+    int64_t vocab;
+    int64_t ignore_index;
+    int dtype;
+    int reduction;
+} sl_xent_args;
+SL_API int sl_xent_sizes(const sl_xent_args* args, int64_t* prep, int64_t* forward, int64_t* backward);
+SL_API int sl_xent_forward(const sl_xent_args* args, void* stream);
+SL_API int sl_xent_backward(const sl_xent_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,6 +7,8 @@ A drop-in for the reference ``sparselab`` package's sparse-training path:
     SparseLinear       nn.Linear replacement backed by a PaddedCSR
     SparsityAlgorithm, DynamicSparsityAlgorithm, Static, SET, RigL
                        dynamic-sparsity routers (GPU prune / regrow)
+    linear_cross_entropy
+                       the LM head's softmax cross entropy without the logits, with its gradients
     residual_norm      the norms around a block with its gate, scale and residual add
     FusedAdamW, AdamWPlan, adamw_step
                        AdamW over all tensors in one launch, moments in 32 or 8 bits
@@ -21,6 +23,7 @@ from . import layout
 from .layout import PaddedCSR, transpose_with_perm
 from .ops import critical_path_stream, set_async_weight_grad, spmm
 from .nn import SparseLinear, sparse_mlp
+from .loss import linear_cross_entropy
 from .norm import residual_norm
 from .optim import AdamWPlan, FusedAdamW, LiveAdamW, adamw_step
 from .router import SparsityAlgorithm, Static, DynamicSparsityAlgorithm, SET, RigL, dense_grad
@@ -31,6 +34,7 @@ __all__ = [
     "spmm",
     "SparseLinear",
     "sparse_mlp",
+    "linear_cross_entropy",
     "residual_norm",
     "AdamWPlan",
     "FusedAdamW",

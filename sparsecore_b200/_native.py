@@ -49,6 +49,13 @@ class SlNormArgs(ctypes.Structure):
                 + [(n, I32) for n in ("kind", "dtype", "residual_dtype", "weight_dtype", "gate_dtype")])
 
 
+class SlXentArgs(ctypes.Structure):
+    """Mirror of `sl_xent_args`."""
+
+    _fields_ = ([(n, P) for n in ("x", "weight", "targets", "loss", "loss_rows", "prep", "scratch", "grad", "dx", "dweight")]
+                + [(n, I64) for n in ("tokens", "dim", "vocab", "ignore_index")] + [("dtype", I32), ("reduction", I32)])
+
+
 # Element types of the training step's dense operators (SL_F32 ...).
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 byref = ctypes.byref
@@ -103,6 +110,9 @@ SIGNATURES: dict[str, tuple] = {
     "sl_norm_workspace_bytes": (I64, [I64, I64, I64]),
     "sl_norm_forward": (I32, [P, P]),
     "sl_norm_backward": (I32, [P, P]),
+    "sl_xent_sizes": (I32, [P, P, P, P]),
+    "sl_xent_forward": (I32, [P, P]),
+    "sl_xent_backward": (I32, [P, P]),
     "sl_set_regrow_draws": (I32, [P, P, P, I64, P, P, I64, P, P, I64, P]),
 }
 
@@ -176,6 +186,7 @@ KERNELS_PER_CALL = {
     "sl_set_regrow_draws": 0,  # host only
     "sl_probe_ffma": 1, "sl_probe_smem": 1,
     "sl_adamw_multi": 1, "sl_adamw_hyper": 1, "sl_norm_forward": 1, "sl_norm_backward": 2,
+    "sl_xent_sizes": 0, "sl_xent_forward": 4, "sl_xent_backward": 4,
 }
 launches = {"count": 0}
 

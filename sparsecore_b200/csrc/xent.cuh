@@ -1,0 +1,73 @@
+// What the parts of the linear cross entropy share: the layout of its
+// buffers and of its operands as 16-bit planes.
+#pragma once
+
+#include "typed.cuh"
+
+namespace slb {
+namespace xent {
+
+constexpr int kPart = 64;           // vocabulary columns of one partial (max, sum) of a row
+constexpr float kGradScale = 32768.f;  // softmax - onehot is held in fp16 times 2^15
+
+// First bytes of the `prep` buffer.
+struct Header {
+    unsigned max_x, max_w, max_g;  // bits of the largest finite |.|
+    int count;                     // tokens that count
+    unsigned done;                 // CTAs of the finish that have written their sums
+    float g;                       // what every gradient is multiplied by at the end
+};
+
+enum : int { kIgnored = -1, kInvalid = -2 };  // in place of a target
+
+// Power of two that brings values of up to `bits` (a float's bits) below
+// 2^15, where fp16 holds what is down to 2^-29 of it at full precision.
+__device__ __forceinline__ int plane_exponent(unsigned bits) {
+    const int e = static_cast<int>(bits >> 23);
+    if (e == 0) return 0;
+    const int k = 14 - (e - 127);
+    return k > 100 ? 100 : k < -100 ? -100 : k;
+}
+
+// One operand: planes of [rows, stride] 16-bit values whose sum is it.
+struct Operand {
+    const void* base;
+    int64_t rows, cols, stride;  // of a plane, in elements
+    int64_t plane;               // elements from one plane to the next
+};
+
+struct Problem {
+    Header* head;
+    const int* tgt;         // [T]
+    float* row_max;         // [T] the softmax's maximum of each row, and
+    float* row_inv;         // [T] one over its sum
+    float* zt;              // [T] logit of the target
+    float2* part;           // [parts][T]
+    const float* g_rows;    // [T] gradients of the single losses, or null
+    int64_t T, D, V;
+    bool f32;               // planes of fp16 pairs, scaled
+    bool bf16;
+};
+
+// C[m, n] = sum over k of A . B^T, and what becomes of it.
+int gemm_stats(const Problem& p, const Operand& x, const Operand& w, cudaStream_t s);
+// Columns [v0, v0 + cols) of the gradient of the logits, as planes in g.
+int gemm_grad(const Problem& p, const Operand& x, const Operand& w, int64_t v0, int64_t cols, const Operand& g,
+              cudaStream_t s);
+
+struct Output {
+    void* dst;        // [M, N] in the caller's type
+    int dtype;
+    float* acc;       // [M, N] sums of the pieces so far, or null
+    bool first, last; // piece
+    float* slabs;     // workspace of a split sum
+    int64_t slab_floats;
+    bool by_x;        // undo x's scale, not w's
+};
+// dx += G[T, cols] . W[cols, D]
+int gemm_dx(const Problem& p, const Operand& g, int64_t cols, const Operand& w, int64_t v0, const Output& o, cudaStream_t s);
+// dw[v0 ...] = G^T[cols, T] . X[T, D]
+int gemm_dw(const Problem& p, const Operand& g, int64_t cols, const Operand& x, const Output& o, cudaStream_t s);
+
+}  // namespace xent
+}  // namespace slb

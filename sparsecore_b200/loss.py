@@ -1,0 +1,134 @@
+"""The language-model head's loss: softmax cross entropy of ``x @ weight.T``
+over a vocabulary, in pieces of it, without keeping the logits, with the
+gradients of ``x`` and ``weight`` (``sl_xent_forward`` / ``sl_xent_backward``).
+
+``F.cross_entropy(head(x), targets)`` holds logits of [tokens, vocab] and
+their gradient in 32 bits; here a bounded piece of the gradient exists at a
+time.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _native as N
+
+__all__ = ["linear_cross_entropy"]
+
+_REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
+
+
+def _args(x, weight, targets, ignore_index, reduction):
+    a = N.SlXentArgs()
+    a.x, a.weight, a.targets = N.ptr(x), N.ptr(weight), N.ptr(targets)
+    a.tokens, a.dim, a.vocab = x.shape[0], x.shape[1], weight.shape[0]
+    a.ignore_index, a.dtype, a.reduction = ignore_index, N.DTYPES[x.dtype], reduction
+    return a
+
+
+def _sizes(a):
+    out = (ctypes.c_int64 * 3)()
+    at = ctypes.addressof(out)
+    N.call("sl_xent_sizes", N.byref(a), at, at + 8, at + 16)
+    return list(out)
+
+
+def _buffer(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def _forward(x, weight, targets, ignore_index, reduction):
+    x, weight, targets = x.contiguous(), weight.contiguous(), targets.contiguous()
+    a = _args(x, weight, targets, ignore_index, reduction)
+    if reduction == 2:
+        loss = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
+        a.loss_rows = N.ptr(loss)
+    else:  # no tokens at all: the mean of nothing is NaN, their sum zero
+        loss = torch.full((), 0.0 if reduction else float("nan"), device=x.device) if x.shape[0] == 0 else \
+            torch.empty((), dtype=torch.float32, device=x.device)
+        a.loss = N.ptr(loss)
+    prep = None
+    if x.shape[0]:
+        sizes = _sizes(a)
+        prep, scratch = _buffer(sizes[0], x.device), _buffer(sizes[1], x.device)
+        a.prep, a.scratch = N.ptr(prep), N.ptr(scratch)
+        N.call_on(x.device, "sl_xent_forward", N.byref(a))
+    return loss, (x, weight, targets, prep)
+
+
+class _LinearCrossEntropyFunction(torch.autograd.Function):
+    """Inputs ``(x, weight, targets, ignore_index, reduction)``, x [tokens, dim];
+    returns the loss.  The operands' 16-bit planes, each row's maximum and its
+    sum are kept for the backward pass; the logits are made again there."""
+
+    @staticmethod
+    def forward(ctx, x, weight, targets, ignore_index, reduction):
+        loss, saved = _forward(x, weight, targets, ignore_index, reduction)
+        ctx.save_for_backward(*saved)
+        ctx.opts = (ignore_index, reduction)
+        return loss
+
+    @staticmethod
+    def backward(ctx, grad):
+        x, weight, targets, prep = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = torch.empty_like(x) if need[0] else None
+        dw = torch.empty_like(weight) if need[1] else None
+        if prep is None:
+            return dx, None if dw is None else dw.zero_(), None, None, None
+        a = _args(x, weight, targets, *ctx.opts)
+        grad = grad.to(torch.float32).contiguous()
+        scratch = _buffer(_sizes(a)[2], x.device)
+        a.prep, a.scratch, a.grad = N.ptr(prep), N.ptr(scratch), N.ptr(grad)
+        a.dx, a.dweight = N.ptr(dx), N.ptr(dw)
+        N.call_on(x.device, "sl_xent_backward", N.byref(a))
+        return dx, dw, None, None, None
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100,
+                         reduction: str = "mean") -> torch.Tensor:
+    """``F.cross_entropy(x @ weight.T, targets)`` in 32 bits, differentiable in
+    ``x`` and ``weight``.
+
+    ``x``: [..., dim], ``weight``: [vocab, dim], of one type (float32, bfloat16
+    or float16); ``targets``: int64 of x's leading shape.  Tokens whose target is
+    ``ignore_index`` count for nothing, whatever their row of x holds.  A target
+    outside [0, vocab) gives that token (and so the sum and the mean) a NaN loss
+    and NaN gradients.  ``reduction``: "mean" over the tokens that count (NaN
+    where none does, with gradients of zero), "sum", or "none" (a loss for each
+    token, 0 for ignored ones).  The loss is float32.
+
+    Raises TypeError (not tensors), RuntimeError (not on one CUDA device) and
+    ValueError (shapes, types, reduction).
+    """
+    for t, name in ((x, "x"), (weight, "weight"), (targets, "targets")):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"linear_cross_entropy: {name} must be a torch.Tensor, got {type(t).__name__}")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"linear_cross_entropy: reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    if x.device.type != "cuda":
+        raise RuntimeError(f"linear_cross_entropy: x must be on a CUDA device (got device={x.device}). "
+                           f"sparsecore_b200 has no CPU path.")
+    for t, name in ((weight, "weight"), (targets, "targets")):
+        if t.device != x.device:
+            raise RuntimeError(f"linear_cross_entropy: {name} is on {t.device} but x is on {x.device}")
+    if x.dtype not in N.DTYPES:
+        raise ValueError(f"linear_cross_entropy: x must be float32, bfloat16 or float16, got {x.dtype}")
+    if weight.dtype != x.dtype:
+        raise ValueError(f"linear_cross_entropy: weight must be {x.dtype} like x, got {weight.dtype}")
+    if targets.dtype != torch.int64:
+        raise ValueError(f"linear_cross_entropy: targets must be torch.int64, got {targets.dtype}")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"linear_cross_entropy: x must be [..., dim] and weight [vocab, dim], got {tuple(x.shape)} "
+                         f"and {tuple(weight.shape)}")
+    if targets.shape != x.shape[:-1]:
+        raise ValueError(f"linear_cross_entropy: targets must have shape {tuple(x.shape[:-1])}, got {tuple(targets.shape)}")
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"linear_cross_entropy: weight must not be empty, got {tuple(weight.shape)}")
+    args = (x.reshape(-1, x.shape[-1]), weight, targets.reshape(-1), int(ignore_index), _REDUCTIONS[reduction])
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        loss = _LinearCrossEntropyFunction.apply(*args)
+    else:
+        loss, _ = _forward(*args)
+    return loss.view(targets.shape) if reduction == "none" else loss
