@@ -152,8 +152,8 @@ live_batch_kernel(const sl_live_desc* __restrict__ descs, int64_t n, float* __re
     }
 }
 
-bool make_tmap_2d(CUtensorMap* map, const float* base, int64_t rows, int64_t cols, int box_rows,
-                  int box_cols, bool swizzle128) {
+// The driver's encoder, looked up once (no libcuda link); null if missing.
+static PFN_cuTensorMapEncodeTiled_v12000 tmap_encode() {
     static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
     static std::once_flag once;
     std::call_once(once, [] {
@@ -164,6 +164,12 @@ bool make_tmap_2d(CUtensorMap* map, const float* base, int64_t rows, int64_t col
             q == cudaDriverEntryPointSuccess)
             encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
     });
+    return encode;
+}
+
+bool make_tmap_2d(CUtensorMap* map, const float* base, int64_t rows, int64_t cols, int box_rows,
+                  int box_cols, bool swizzle128) {
+    const auto encode = tmap_encode();
     if (encode == nullptr || !aligned16(base) || (cols * 4) % 16 != 0) return false;
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * sizeof(float)};
@@ -174,6 +180,19 @@ bool make_tmap_2d(CUtensorMap* map, const float* base, int64_t rows, int64_t col
                   swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool make_tmap_16bit(CUtensorMap* map, const void* base, bool bf16, int64_t cols, int64_t rows, int64_t planes,
+                     int64_t stride, int64_t plane, int box_rows) {
+    const auto encode = tmap_encode();
+    if (encode == nullptr || !aligned16(base) || stride % 8 != 0 || plane % 8 != 0) return false;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(planes)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(stride) * 2, static_cast<cuuint64_t>(plane) * 2};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
+                  dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 unsigned* device_status_word() {

@@ -20,6 +20,11 @@ namespace slb {
 bool make_tmap_2d(CUtensorMap* map, const float* base, int64_t rows, int64_t cols,
                   int box_rows, int box_cols, bool swizzle128 = false);
 
+// [planes, rows, cols] of 16-bit values, rows `stride` and planes `plane`
+// elements apart -> tensor map with 128-byte swizzled boxes of box_rows x 64.
+bool make_tmap_16bit(CUtensorMap* map, const void* base, bool bf16, int64_t cols, int64_t rows, int64_t planes,
+                     int64_t stride, int64_t plane, int box_rows);
+
 // Per-device status word owned by the library (bit 0 = a bounded wait timed
 // out); allocated on first use on the current device.
 unsigned* device_status_word();

@@ -6,7 +6,7 @@
 //   G_tv = exp(z_tv - m_t) / s_t - [v = target_t]       (times the loss's gradient)
 //   dx = G . W            dW = G^T . x
 //
-// Forward: a matrix product whose epilogue leaves, of every 64 columns of
+// Forward: a matrix product whose epilogue leaves, of every 128 columns of
 // a row, their maximum and the sum of exponentials below it; a second small
 // kernel joins them.  Backward: pieces of the vocabulary, each with its
 // logits made again, turned into G in the epilogue, and multiplied twice.
@@ -61,7 +61,7 @@ Layout layout(int64_t T, int64_t D, int64_t V, int dtype, bool copy_w) {
     l.gp = up(std::min(l.piece, V), 64);
     l.g = take(planes * T * l.gp * 2);
     l.acc = take(V > l.piece ? 4 * T * D : 0);
-    l.slab_floats = int64_t(16) << 20;
+    l.slab_floats = kSlabFloats;
     l.slabs = take(4 * l.slab_floats);
     l.bwd = o;
     return l;

@@ -7,7 +7,10 @@
 namespace slb {
 namespace xent {
 
-constexpr int kPart = 64;           // vocabulary columns of one partial (max, sum) of a row
+constexpr int kPart = 128;          // vocabulary columns of one partial (max, sum) of a row
+// Sums of 256 x 256 that a split product may leave to be joined: one for each
+// pair of a B200's 148 SMs.
+constexpr int64_t kSlabFloats = 74 * 65536;
 constexpr float kGradScale = 32768.f;  // softmax - onehot is held in fp16 times 2^15
 
 // First bytes of the `prep` buffer.

@@ -1,163 +1,486 @@
-// The matrix products of the linear cross entropy and their epilogues:
-// plain tiles of 64 x 64 on the 32-bit units.
+// The matrix products of the linear cross entropy and their epilogues, on
+// the tensor cores.
+//
+// A pair of CTAs (one on each of two SMs) multiplies tiles of 256 x 256 along
+// the whole sum, one after another (the grid is as large as the GPU).  In
+// each CTA one thread keeps TMA loads of 64-column slices of the operands
+// going round a ring of shared-memory stages, one thread of the first CTA
+// issues the MMAs, and eight warps take finished sums out of tensor memory,
+// which holds two tiles: one is multiplied while the other is read.
+//
+// 32-bit operands come as two fp16 planes, a stage holding both, and are
+// multiplied as lo.hi, hi.lo and hi.hi.  The matrix units cut rather than
+// round when they add to a sum, so for these a sum in tensor memory is at
+// most kChunk stages long; the epilogue's warps add the chunks in registers,
+// rounding to nearest.
 #include <algorithm>
 
+#include "umma.cuh"
 #include "xent.cuh"
 
 namespace slb {
 namespace xent {
 namespace {
 
-constexpr int kT = 64, kK = 16, kThreads = 256;
+constexpr int kTile = 256;
+constexpr int kSlice = 64;                       // of the sum, in a stage: 128 bytes a row
+constexpr int kBox = 128 * kSlice * 2;           // bytes of one operand's plane in a stage
+constexpr int kRing = 12;                        // boxes in shared memory: 6 stages, or 3 of two planes
+constexpr int kChunk = 2;                        // stages added up in tensor memory for 32-bit operands
+constexpr int kEpilogueWarps = 8;
+constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // a warpgroup of loads and MMAs, two of results
+// Registers a thread: of 168 x 384 at launch, 40 x 128 stay with the first
+// warpgroup and 232 x 256 hold the results (128 sums a thread).
+constexpr int kRegsLow = 40, kRegsHigh = 232;
+static_assert(kRegsLow * 128 + kRegsHigh * 256 <= 168 * kThreads, "registers of the launch");
+constexpr size_t kSmem = kRing * kBox + 1024 + 256;
 
-// Element (i, k) of an operand lies at i * si + k * sk of each plane.
-struct View {
-    const void* base;
-    int64_t n, si, sk, plane;
-};
+enum Mode : int { kStats, kGrad, kOut };
 
 struct Args {
     Problem p;
-    View a, b;
     int64_t M, N, K;
-    int mode;  // 0: partial maxima and sums, 1: gradient planes, 2: output
+    int tiles_m, tiles_n, splits, per_split;  // per_split: stages
+    bool a_mn, b_mn;
     int64_t v0;
     void* g;
     int64_t g_stride, g_plane;
     Output o;
+    int64_t slab_stride;
+    unsigned* status;
 };
 
-template <typename T>
-__device__ __forceinline__ float get(const View& v, int64_t i, int64_t k, bool two) {
-    if (i >= v.n) return 0.f;
-    const T* q = static_cast<const T*>(v.base) + i * v.si + k * v.sk;
-    return two ? to_f(q[0]) + to_f(q[v.plane]) : to_f(q[0]);
+struct Shared {
+    uint64_t full[kRing / 2], empty[kRing / 2], tmem_full[2], tmem_empty[2];
+    uint32_t tmem;
+};
+
+// Tiles in groups of 8 rows of tiles, down the columns of a group: what runs
+// at one time shares few operand rows.
+__device__ __forceinline__ void locate(const Args& a, int id, int& m, int& n, int& split) {
+    const int per = a.tiles_m * a.tiles_n;
+    split = id / per;
+    id -= split * per;
+    const int group = id / (8 * a.tiles_n), first = group * 8, rows = min(8, a.tiles_m - first);
+    id -= group * 8 * a.tiles_n;
+    m = first + id % rows;
+    n = id / rows;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-gemm_kernel(Args a) {
-    __shared__ float As[kK][kT + 1], Bs[kK][kT + 1], C[kT][kT + 1];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t m0 = static_cast<int64_t>(blockIdx.x) * kT, n0 = static_cast<int64_t>(blockIdx.y) * kT;
-    const bool two = a.p.f32;
-    float acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < a.K; k0 += kK) {
-        for (int i = threadIdx.x; i < kT * kK; i += kThreads) {
-            const int r = i / kK, k = i % kK;
-            const bool in = k0 + k < a.K;
-            As[k][r] = in ? get<T>(a.a, m0 + r, k0 + k, two) : 0.f;
-            Bs[k][r] = in ? get<T>(a.b, n0 + r, k0 + k, two) : 0.f;
-        }
-        __syncthreads();
+__device__ __forceinline__ float exp2_fast(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+__device__ __forceinline__ void store32(void* dst, const uint32_t (&v)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack2(__half a, __half b) {
+    return static_cast<uint32_t>(__half_as_ushort(a)) | static_cast<uint32_t>(__half_as_ushort(b)) << 16;
+}
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16 a, __nv_bfloat16 b) {
+    return static_cast<uint32_t>(__bfloat16_as_ushort(a)) | static_cast<uint32_t>(__bfloat16_as_ushort(b)) << 16;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// What brings a sum of 32-bit operands' planes back to the logit.
+__device__ __forceinline__ float logit_scale(const Problem& p) {
+    return exp2f(static_cast<float>(min(127, -plane_exponent(p.head->max_x) - plane_exponent(p.head->max_w))));
+}
+
+// Maximum and sum of exponentials of this thread's row t over 128 columns
+// from n0; z holds the logits over `u`.
+__device__ __forceinline__ void epilogue_stats(const Args& a, float (&z)[128], int64_t t, int64_t n0, float u) {
+    const int n = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(128), a.N - n0)));
+    if (t >= a.M || n == 0) return;
+    const int tg = a.p.tgt[t];
+    if (tg >= n0 && tg < n0 + n) {
+        const int at = static_cast<int>(tg - n0);
+        float q = 0.f;
 #pragma unroll
-        for (int k = 0; k < kK; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(As[k][ty * 4 + i], Bs[k][tx * 4 + j], acc[i][j]);
-        __syncthreads();
+        for (int j = 0; j < 128; ++j) q = j == at ? z[j] : q;
+        a.p.zt[t] = q * u;
     }
-    float ux = 1.f, uw = 1.f;
-    if (two) {
-        ux = exp2f(-static_cast<float>(plane_exponent(a.p.head->max_x)));
-        uw = exp2f(-static_cast<float>(plane_exponent(a.p.head->max_w)));
+    float m = -INFINITY, s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (n < 128) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j) z[j] = j < n ? z[j] : -INFINITY;  // exp gives 0
     }
-    if (a.mode == 2) {
-        const float gs = a.p.bf16 ? 1.f : 1.f / kGradScale, u = a.o.by_x ? ux : uw, g = a.p.head->g;
-        for (int i = 0; i < 4; ++i)
-            for (int j = 0; j < 4; ++j) {
-                const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-                if (m >= a.M || n >= a.N) continue;
-                float v = acc[i][j];
-                if (a.o.acc) {
-                    if (!a.o.first) v += a.o.acc[m * a.N + n];
-                    a.o.acc[m * a.N + n] = v;
-                }
-                if (!a.o.last) continue;
-                v = v * gs * u * g;
-                if (a.o.dtype == SL_F32) static_cast<float*>(a.o.dst)[m * a.N + n] = v;
-                else if (a.o.dtype == SL_BF16) static_cast<__nv_bfloat16*>(a.o.dst)[m * a.N + n] = __float2bfloat16_rn(v);
-                else static_cast<__half*>(a.o.dst)[m * a.N + n] = __float2half_rn(v);
+#pragma unroll
+    for (int j = 0; j < 128; ++j) m = fmaxf(m, z[j]);
+    m *= u;
+#pragma unroll
+    for (int j = 0; j < 128; ++j) s[j & 3] += exp2_fast((z[j] * u - m) * kLog2e);
+    a.p.part[n0 / kPart * a.M + t] = make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
+}
+
+// G = exp(z - m) / s - [target], as planes.
+template <int PL>
+__device__ __forceinline__ void epilogue_grad(const Args& a, float (&z)[128], int64_t t, int64_t n0, float u) {
+    const int64_t room = min(static_cast<int64_t>(128), a.g_stride - n0);
+    if (t >= a.M || room <= 0) return;
+    const int tg = a.p.tgt[t];
+    const int at = tg >= 0 && tg - a.v0 - n0 >= 0 && tg - a.v0 - n0 < 128 ? static_cast<int>(tg - a.v0 - n0) : -1;
+    float one = a.p.bf16 ? 1.f : kGradScale;
+    if (a.p.g_rows) one = a.p.head->g > 0.f ? one * (a.p.g_rows[t] / a.p.head->g) : 0.f;
+    const float m = a.p.row_max[t], c = a.p.row_inv[t] * one;
+    const bool on = tg != kIgnored;
+    char* dst = static_cast<char*>(a.g) + 2 * (t * a.g_stride + n0);
+#pragma unroll
+    for (int j = 0; j < 128; j += 16) {
+        if (j >= room) break;
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int k = 0; k < 16; k += 2) {
+            float v[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                v[q] = exp2_fast((z[j + k + q] * u - m) * kLog2e) * c - (j + k + q == at ? one : 0.f);
+                if (!on) v[q] = 0.f;
             }
-        return;
-    }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) C[ty * 4 + i][tx * 4 + j] = acc[i][j] * ux * uw;
-    __syncthreads();
-    if (a.mode == 0) {
-        // one partial for each row of the tile
-        if (threadIdx.x < kT && m0 + threadIdx.x < a.M) {
-            const int64_t t = m0 + threadIdx.x;
-            const int n = static_cast<int>(min(static_cast<int64_t>(kT), a.N - n0));
-            float m = -INFINITY, s = 0.f;
-            for (int j = 0; j < n; ++j) m = fmaxf(m, C[threadIdx.x][j]);
-            for (int j = 0; j < n; ++j) s += expf(C[threadIdx.x][j] - m);
-            a.p.part[blockIdx.y * a.M + t] = make_float2(m, s);
-            const int64_t at = a.p.tgt[t] - n0;
-            if (a.p.tgt[t] >= 0 && at >= 0 && at < n) a.p.zt[t] = C[threadIdx.x][at];
+            if (PL == 1 && a.p.bf16) {
+                hi[k / 2] = pack2(__float2bfloat16_rn(v[0]), __float2bfloat16_rn(v[1]));
+            } else {
+                const __half h0 = __float2half_rn(v[0]), h1 = __float2half_rn(v[1]);
+                hi[k / 2] = pack2(h0, h1);
+                if (PL == 2)
+                    lo[k / 2] = pack2(__float2half_rn(v[0] - __half2float(h0)), __float2half_rn(v[1] - __half2float(h1)));
+            }
         }
-        return;
-    }
-    for (int i = threadIdx.x; i < kT * kT; i += kThreads) {
-        const int r = i / kT, c = i % kT;
-        const int64_t t = m0 + r, n = n0 + c;
-        if (t >= a.M || n >= a.g_stride) continue;
-        const int tg = a.p.tgt[t];
-        float v = 0.f;
-        if (n < a.N && tg != kIgnored) {
-            v = expf(C[r][c] - a.p.row_max[t]) * a.p.row_inv[t] - (a.v0 + n == tg ? 1.f : 0.f);
-            if (a.p.g_rows) v = a.p.head->g > 0.f ? v * (a.p.g_rows[t] / a.p.head->g) : 0.f;
-        }
-        if (a.p.bf16) {
-            static_cast<__nv_bfloat16*>(a.g)[t * a.g_stride + n] = __float2bfloat16_rn(v);
-        } else {
-            v *= kGradScale;
-            const __half hi = __float2half_rn(v);
-            static_cast<__half*>(a.g)[t * a.g_stride + n] = hi;
-            if (two) static_cast<__half*>(a.g)[a.g_plane + t * a.g_stride + n] = __float2half_rn(v - __half2float(hi));
-        }
+        store32(dst + 2 * j, hi);
+        if (PL == 2) store32(dst + 2 * (a.g_plane + j), lo);
     }
 }
 
-int launch(const Args& a, int64_t cols, cudaStream_t s) {
-    const dim3 grid(static_cast<unsigned>((a.M + kT - 1) / kT), static_cast<unsigned>((cols + kT - 1) / kT));
-    if (a.p.bf16) gemm_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(a);
-    else gemm_kernel<__half><<<grid, kThreads, 0, s>>>(a);
+// What is multiplied into a finished sum.
+__device__ __forceinline__ float out_scale(const Problem& p, bool by_x, bool f32) {
+    const float g = (p.bf16 ? 1.f : 1.f / kGradScale) * p.head->g;
+    return f32 ? g * exp2f(-static_cast<float>(plane_exponent(by_x ? p.head->max_x : p.head->max_w))) : g;
+}
+
+__device__ __forceinline__ void store_out(const Output& o, int64_t i, float v) {
+    if (o.dtype == SL_F32) static_cast<float*>(o.dst)[i] = v;
+    else if (o.dtype == SL_BF16) static_cast<__nv_bfloat16*>(o.dst)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(o.dst)[i] = __float2half_rn(v);
+}
+
+__device__ __forceinline__ void epilogue_out(const Args& a, float (&z)[128], int64_t m, int64_t n0, int split, float scale) {
+    if (m >= a.M) return;
+    if (a.splits > 1) {
+        float* dst = a.o.slabs + split * a.slab_stride + m * (static_cast<int64_t>(a.tiles_n) * kTile) + n0;
+#pragma unroll
+        for (int j = 0; j < 128; j += 8) {
+            uint32_t v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = __float_as_uint(z[j + k]);
+            store32(dst + j, v);
+        }
+        return;
+    }
+    const int n = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(128), a.N - n0)));
+    const int64_t row = m * a.N + n0;
+    if (a.o.acc) {
+        float* q = a.o.acc + row;
+#pragma unroll
+        for (int j = 0; j < 128; ++j)
+            if (j < n) {
+                if (!a.o.first) z[j] += q[j];
+                if (!a.o.last) q[j] = z[j];
+            }
+        if (!a.o.last) return;
+    }
+    const int64_t bytes = a.o.dtype == SL_F32 ? 4 : 2;
+    char* dst = static_cast<char*>(a.o.dst) + row * bytes;
+    if (n == 128 && (reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
+#pragma unroll
+        for (int j = 0; j < 128; j += 16) {
+            uint32_t v[8];
+            if (a.o.dtype == SL_F32) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = __float_as_uint(z[j + 8 * h + k] * scale);
+                    store32(dst + 4 * (j + 8 * h), v);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float p = z[j + 2 * k] * scale, q = z[j + 2 * k + 1] * scale;
+                    v[k] = a.o.dtype == SL_BF16 ? pack2(__float2bfloat16_rn(p), __float2bfloat16_rn(q))
+                                                : pack2(__float2half_rn(p), __float2half_rn(q));
+                }
+                store32(dst + 2 * j, v);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 128; ++j)
+        if (j < n) store_out(a.o, row + j, z[j] * scale);
+}
+
+template <int PL, int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Args a) {
+    constexpr int kStages = kRing / (2 * PL);
+    constexpr int kStageBytes = 2 * PL * kBox;
+    extern __shared__ char raw[];
+    char* ring = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    Shared& sh = *reinterpret_cast<Shared*>(ring + kRing * kBox);
+    const int warp = threadIdx.x >> 5, lane = lane_id();
+    const uint32_t rank = cluster_rank();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&sh.full[s], 1);
+            mbar_init(&sh.empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&sh.tmem_full[b], 1);
+            mbar_init(&sh.tmem_empty[b], 2 * kEpilogueWarps);
+        }
+        fence_barrier_init();
+    }
+    if (warp == 1) tmem_alloc_pair(&sh.tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    const int tiles = a.tiles_m * a.tiles_n * a.splits, pairs = gridDim.x / 2, pair = blockIdx.x / 2;
+    const int all = static_cast<int>((a.K + kSlice - 1) / kSlice);
+    const int chunk = PL == 2 ? kChunk : all;
+
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
+    if (warp == 0 && lane == 0) {  // loads
+        uint32_t stage = 0, phase = 0;
+        bool ok = true;
+        for (int id = pair; id < tiles && ok; id += pairs) {
+            int tm, tn, split;
+            locate(a, id, tm, tn, split);
+            const int row_a = tm * kTile + static_cast<int>(rank) * 128, row_b = tn * kTile + static_cast<int>(rank) * 128;
+            const int k1 = min(all, (split + 1) * a.per_split);
+            for (int k = split * a.per_split; k < k1; ++k) {
+                if (!mbar_wait(&sh.empty[stage], phase ^ 1, a.status)) { ok = false; break; }
+                if (rank == 0) mbar_expect_tx(&sh.full[stage], 2 * kStageBytes);
+                const uint32_t bar = leader_addr(&sh.full[stage]);
+                char* dst = ring + stage * kStageBytes;
+                const int x = k * kSlice;
+#pragma unroll
+                for (int pl = 0; pl < PL; ++pl, dst += 2 * kBox) {
+                    if (a.a_mn) {
+                        tma_load_3d_pair(dst, &map_a, row_a, x, pl, bar);
+                        tma_load_3d_pair(dst + kBox / 2, &map_a, row_a + 64, x, pl, bar);
+                    } else {
+                        tma_load_3d_pair(dst, &map_a, x, row_a, pl, bar);
+                    }
+                    if (a.b_mn) {
+                        tma_load_3d_pair(dst + kBox, &map_b, row_b, x, pl, bar);
+                        tma_load_3d_pair(dst + kBox + kBox / 2, &map_b, row_b + 64, x, pl, bar);
+                    } else {
+                        tma_load_3d_pair(dst + kBox, &map_b, x, row_b, pl, bar);
+                    }
+                }
+                if (++stage == kStages) stage = 0, phase ^= 1;
+            }
+        }
+        // The last stages are free again before the CTA ends: every commit of
+        // the other CTA's thread has then arrived here.
+        for (int s = 0; s < kStages && ok; ++s) {
+            ok = mbar_wait(&sh.empty[stage], phase ^ 1, a.status);
+            if (++stage == kStages) stage = 0, phase ^= 1;
+        }
+        if (!ok)  // given up: let the copies in flight land before the CTA may end
+            for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+    } else if (warp == 1 && lane == 0 && rank == 0) {  // MMAs of both CTAs
+        const uint32_t idesc = umma_idesc(a.p.bf16, a.a_mn, a.b_mn, kTile);
+        const uint32_t step_a = (a.a_mn ? 16 * 128 : 32) >> 4, step_b = (a.b_mn ? 16 * 128 : 32) >> 4;
+        uint32_t stage = 0, phase = 0, done = 0;
+        bool ok = true;
+        for (int id = pair; id < tiles && ok; id += pairs) {
+            int tm, tn, split;
+            locate(a, id, tm, tn, split);
+            const int k1 = min(all, (split + 1) * a.per_split);
+            for (int k0 = split * a.per_split; k0 < k1 && ok; k0 += chunk, ++done) {
+                const uint32_t buf = done & 1;
+                if (!mbar_wait_cluster(&sh.tmem_empty[buf], ((done >> 1) & 1) ^ 1, a.status)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t d = tmem + buf * kTile;
+                uint32_t add = 0;
+                const int end = min(k1, k0 + chunk);
+                for (int k = k0; k < end; ++k) {
+                    if (!mbar_wait_cluster(&sh.full[stage], phase, a.status)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t base = smem_addr(ring + stage * kStageBytes);
+                    uint64_t da[PL], db[PL];
+#pragma unroll
+                    for (int pl = 0; pl < PL; ++pl) {
+                        da[pl] = umma_desc(base + pl * 2 * kBox, a.a_mn);
+                        db[pl] = umma_desc(base + pl * 2 * kBox + kBox, a.b_mn);
+                    }
+                    // the small products first, while the sum is small
+#pragma unroll
+                    for (int pr = PL == 2 ? 0 : 2; pr < 3; ++pr) {
+                        const uint64_t qa = da[pr == 0 ? PL - 1 : 0], qb = db[pr == 1 ? PL - 1 : 0];
+#pragma unroll
+                        for (int i = 0; i < kSlice / 16; ++i) {
+                            umma_pair(d, qa + i * step_a, qb + i * step_b, idesc, add);
+                            add = 1;
+                        }
+                    }
+                    umma_commit_pair(&sh.empty[stage]);
+                    if (++stage == kStages) stage = 0, phase ^= 1;
+                }
+                umma_commit_pair(&sh.tmem_full[buf]);
+            }
+        }
+    }
+    } else {  // results
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+        const float u = MODE == kOut ? out_scale(a.p, a.o.by_x, PL == 2) : PL == 2 ? logit_scale(a.p) : 1.f;
+        uint32_t done = 0;
+        bool ok = true;
+        for (int id = pair; id < tiles && ok; id += pairs) {
+            int tm, tn, split;
+            locate(a, id, tm, tn, split);
+            const int k1 = min(all, (split + 1) * a.per_split);
+            float z[128] = {};
+            for (int k0 = split * a.per_split; k0 < k1; k0 += chunk, ++done) {
+                const uint32_t buf = done & 1;
+                if (!__all_sync(0xffffffffu, mbar_wait(&sh.tmem_full[buf], (done >> 1) & 1, a.status))) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t at = tmem + lanes + buf * kTile + half * 128;
+#pragma unroll
+                for (int j = 0; j < 128; j += 32) {
+                    uint32_t r[32];
+                    tmem_load32(at + j, r);
+                    tmem_load_wait();
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) z[j + k] = PL == 1 ? __uint_as_float(r[k]) : z[j + k] + __uint_as_float(r[k]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(leader_addr(&sh.tmem_empty[buf]));
+            }
+            if (!ok) break;
+            const int64_t t = static_cast<int64_t>(tm) * kTile + rank * 128 + quarter * 32 + lane;
+            const int64_t n0 = static_cast<int64_t>(tn) * kTile + half * 128;
+            if (MODE == kStats) epilogue_stats(a, z, t, n0, u);
+            else if (MODE == kGrad) epilogue_grad<PL>(a, z, t, n0, u);
+            else epilogue_out(a, z, t, n0, split, u);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // no CTA leaves while the other may still signal it
+    tc_fence_after();
+    if (warp == 1) tmem_free_pair(tmem, 512);
+}
+
+// Sum of a split product's slabs, in their order.
+__global__ void __launch_bounds__(256)
+join_kernel(Problem p, Output o, int64_t M, int64_t N, int64_t stride, int64_t slab, int splits, bool f32) {
+    const float scale = out_scale(p, o.by_x, f32);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+    for (int64_t i = blockIdx.x * static_cast<int64_t>(256) + threadIdx.x; i < M * N; i += step) {
+        const int64_t m = i / N;
+        const float* q = o.slabs + m * stride + (i - m * N);
+        float v = 0.f;
+        for (int s = 0; s < splits; ++s) v += q[s * slab];
+        if (o.acc) {
+            if (!o.first) v += o.acc[i];
+            if (!o.last) o.acc[i] = v;
+        }
+        if (o.last) store_out(o, i, v * scale);
+    }
+}
+
+template <int PL, int MODE>
+int launch(const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, cudaStream_t s) {
+    if (int rc = cuda_status(cudaFuncSetAttribute(gemm_kernel<PL, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                  static_cast<int>(kSmem)), "sl_xent"))
+        return rc;
+    const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits;
+    const int64_t pairs = std::min<int64_t>(tiles, std::max(1, num_sms() / 2));
+    gemm_kernel<PL, MODE><<<static_cast<unsigned>(2 * pairs), kThreads, kSmem, s>>>(ma, mb, a);
     SL_RETURN_IF_LAUNCH_FAILED("sl_xent");
     return SL_OK;
 }
 
-View rows(const Operand& o, int64_t from, int64_t n) {
-    return {static_cast<const char*>(o.base) + 2 * from * o.stride, n, o.stride, 1, o.plane};
+template <int MODE>
+int run(Args& a, const Operand& A, const Operand& B, cudaStream_t s) {
+    CUtensorMap ma, mb;
+    const int planes = a.p.f32 ? 2 : 1;
+    if (!make_tmap_16bit(&ma, A.base, a.p.bf16, A.cols, A.rows, planes, A.stride, planes == 2 ? A.plane : A.stride * A.rows, a.a_mn ? 64 : 128) ||
+        !make_tmap_16bit(&mb, B.base, a.p.bf16, B.cols, B.rows, planes, B.stride, planes == 2 ? B.plane : B.stride * B.rows, a.b_mn ? 64 : 128))
+        return fail(SL_ERR_CUDA, "sl_xent: tensor map could not be made");
+    a.status = device_status_word();
+    if (a.status == nullptr) return fail(SL_ERR_CUDA, "sl_xent: no device status word");
+    a.tiles_m = static_cast<int>((a.M + kTile - 1) / kTile);
+    a.tiles_n = static_cast<int>((a.N + kTile - 1) / kTile);
+    const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n, pairs = std::max(1, num_sms() / 2);
+    SL_REQUIRE(tiles * 2 <= INT_MAX, "sl_xent", "too many tiles");
+    const int all = static_cast<int>((a.K + kSlice - 1) / kSlice);
+    a.splits = 1;
+    a.per_split = all;
+    if (MODE == kOut) {
+        // Few tiles and a long sum: the sum is split so that all pairs of SMs
+        // have a part, of eight stages at least.
+        a.slab_stride = a.M * a.tiles_n * kTile;
+        const int64_t want = std::min({pairs / tiles, static_cast<int64_t>(all / 8), a.o.slab_floats / a.slab_stride});
+        if (want > 1) {
+            a.per_split = static_cast<int>((all + want - 1) / want);
+            a.splits = (all + a.per_split - 1) / a.per_split;
+        }
+    }
+    if (int rc = a.p.f32 ? launch<2, MODE>(ma, mb, a, s) : launch<1, MODE>(ma, mb, a, s)) return rc;
+    if (a.splits > 1) {
+        const int64_t blocks = std::min<int64_t>((a.M * a.N + 255) / 256, num_sms() * 8);
+        join_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(a.p, a.o, a.M, a.N, static_cast<int64_t>(a.tiles_n) * kTile, a.slab_stride, a.splits, a.p.f32);
+        SL_RETURN_IF_LAUNCH_FAILED("sl_xent");
+    }
+    return SL_OK;
 }
-View columns(const Operand& o, int64_t n) { return {o.base, n, 1, o.stride, o.plane}; }
+
+Operand rows_from(Operand o, int64_t from, int64_t n) {
+    o.base = static_cast<const char*>(o.base) + 2 * from * o.stride;
+    o.rows = n;
+    return o;
+}
 
 }  // namespace
 
 int gemm_stats(const Problem& p, const Operand& x, const Operand& w, cudaStream_t s) {
-    Args a{p, rows(x, 0, p.T), rows(w, 0, p.V), p.T, p.V, p.D, 0};
-    return launch(a, p.V, s);
+    Args a{};
+    a.p = p; a.M = p.T; a.N = p.V; a.K = p.D;
+    return run<kStats>(a, x, w, s);
 }
 
-int gemm_grad(const Problem& p, const Operand& x, const Operand& w, int64_t v0, int64_t cols, const Operand& g,
-              cudaStream_t s) {
-    Args a{p, rows(x, 0, p.T), rows(w, v0, cols), p.T, cols, p.D, 1, v0, const_cast<void*>(g.base), g.stride, g.plane};
-    return launch(a, g.stride, s);
+int gemm_grad(const Problem& p, const Operand& x, const Operand& w, int64_t v0, int64_t cols, const Operand& g, cudaStream_t s) {
+    Args a{};
+    a.p = p; a.M = p.T; a.N = cols; a.K = p.D;
+    a.v0 = v0; a.g = const_cast<void*>(g.base); a.g_stride = g.stride; a.g_plane = g.plane;
+    return run<kGrad>(a, x, rows_from(w, v0, cols), s);
 }
 
 int gemm_dx(const Problem& p, const Operand& g, int64_t cols, const Operand& w, int64_t v0, const Output& o, cudaStream_t s) {
-    View b = columns(w, p.D);
-    b.base = static_cast<const char*>(b.base) + 2 * v0 * w.stride;
-    Args a{p, rows(g, 0, p.T), b, p.T, p.D, cols, 2};
-    a.o = o;
-    return launch(a, p.D, s);
+    Args a{};
+    a.p = p; a.M = p.T; a.N = p.D; a.K = cols; a.b_mn = true; a.o = o;
+    return run<kOut>(a, g, rows_from(w, v0, cols), s);
 }
 
 int gemm_dw(const Problem& p, const Operand& g, int64_t cols, const Operand& x, const Output& o, cudaStream_t s) {
-    Args a{p, columns(g, cols), columns(x, p.D), cols, p.D, p.T, 2};
-    a.o = o;
-    return launch(a, p.D, s);
+    Args a{};
+    a.p = p; a.M = cols; a.N = p.D; a.K = p.T; a.a_mn = a.b_mn = true; a.o = o;
+    return run<kOut>(a, g, x, s);
 }
 
 }  // namespace xent
