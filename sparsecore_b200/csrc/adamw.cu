@@ -39,6 +39,7 @@ struct Item {
     int64_t n;
     int64_t first;  // number of its first tile
     uint32_t number;
+    bool plain;     // no padding, all addresses on 16 bytes (8-bit moments: on 8)
 };
 
 // The table travels in the launch's parameters: no copy to the device, and a
@@ -63,167 +64,240 @@ __host__ __device__ __forceinline__ uint32_t mix32(uint32_t v) {
 
 // kPer elements from `i`; whole packs where `vec`, else up to `left` of them.
 template <typename T>
-__device__ __forceinline__ void load(const T* src, int64_t i, int left, bool vec, T (&out)[kPer]) {
+__device__ __forceinline__ void load(const T* src, int64_t i, int left, bool vec, float (&out)[kPer]) {
     if (vec) {
-        const Pack<T, kPer> q = *reinterpret_cast<const Pack<T, kPer>*>(src + i);
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) out[k] = q.v[k];
+        load_f<T, kPer>(src + i, out);
     } else {
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) out[k] = k < left ? src[i + k] : T{};
+        for (int k = 0; k < kPer; ++k) out[k] = k < left ? to_f(src[i + k]) : 0.f;
     }
 }
 template <typename T>
-__device__ __forceinline__ void store(T* dst, int64_t i, int left, bool vec, const T (&in)[kPer]) {
+__device__ __forceinline__ void store(T* dst, int64_t i, int left, bool vec, const float (&in)[kPer]) {
     if (vec) {
-        Pack<T, kPer> q;
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) q.v[k] = in[k];
-        *reinterpret_cast<Pack<T, kPer>*>(dst + i) = q;
+        store_f<T, kPer>(dst + i, in);
     } else {
 #pragma unroll
         for (int k = 0; k < kPer; ++k)
-            if (k < left) dst[i + k] = in[k];
+            if (k < left) dst[i + k] = from_f<T>(in[k]);
     }
 }
 
-__device__ __forceinline__ float warp_max(float v) {
+// Square root to 2^-22 of it; of a subnormal number 0.
+__device__ __forceinline__ float sqrt_fast(float v) {
+    float r;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// Eight e4m3 values times their scale.
+__device__ __forceinline__ void from_e4m3(uint2 c, float scale, float (&out)[kPer]) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t w = (k < 2 ? c.x : c.y) >> (16 * (k & 1));
+        const __half2 h(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xFFFFu), __NV_E4M3));
+        const float2 f = __half22float2(h);
+        out[2 * k] = f.x * scale;
+        out[2 * k + 1] = f.y * scale;
+    }
 }
 
-__device__ __forceinline__ float e4m3_to_f(uint8_t c) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+// v (already over its scale, up to 448) rounded up or down to an e4m3 value
+// by 16 dither bits.  Adding the bits below the three kept mantissa bits and
+// cutting there rounds away from zero with the probability of the part cut
+// off; values below the smallest normal 2^-6 are moved out into the binade
+// above it, whose spacing 2^-9 is theirs, and back.
+__device__ __forceinline__ float dithered(float v, uint32_t bits16) {
+    const float by = fabsf(v) < 0.015625f ? copysignf(0.015625f, v) : 0.f;
+    return __uint_as_float((__float_as_uint(v + by) + (bits16 << 4)) & 0xFFF00000u) - by;
 }
 
-// |a| (already times 448 / top) to e4m3 by 16 dither bits.  Adding the bits
-// below the three kept mantissa bits and cutting there rounds up with the
-// probability of the part cut off; values below the smallest normal 2^-6
-// are moved up into the binade above it, whose spacing 2^-9 is theirs.
-__device__ __forceinline__ uint32_t to_e4m3(float a, uint32_t bits16) {
-    a = fminf(a, 448.f);
-    const bool small = a < 0.015625f;
-    const uint32_t raw = __float_as_uint(small ? a + 0.015625f : a) + (bits16 << 4);
-    return (raw >> 20) - (120u << 3) - (small ? 8u : 0u);
+__device__ __forceinline__ uint2 to_e4m3(const float (&q)[kPer]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        w[k] = __nv_cvt_float2_to_fp8x2(make_float2(q[2 * k], q[2 * k + 1]), __NV_SATFINITE, __NV_E4M3);
+    return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+}
+
+// Eight bytes of the 8-bit moments; those from `left` on are not touched.
+__device__ __forceinline__ uint2 load8(const uint8_t* src, int left, bool vec) {
+    if (vec) return *reinterpret_cast<const uint2*>(src);
+    uint32_t w[2] = {0, 0};
+    for (int k = 0; k < left; ++k) w[k >> 2] |= static_cast<uint32_t>(src[k]) << (8 * (k & 3));
+    return make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ void store8(uint8_t* dst, int left, bool vec, uint2 v) {
+    if (vec) {
+        *reinterpret_cast<uint2*>(dst) = v;
+    } else {
+        for (int k = 0; k < left; ++k) dst[k] = static_cast<uint8_t>((k < 4 ? v.x : v.y) >> (8 * (k & 3)));
+    }
+}
+
+// max that keeps a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float rcp_fast(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// Which of a thread's elements take the step: those of a padded array whose
+// column is not below 0, and never those behind the tensor's end.
+__device__ __forceinline__ uint32_t taking_part(const int32_t* live, int64_t i, int left) {
+    uint32_t on = (1u << left) - 1;
+    if (live == nullptr) return on;
+    if (left == kPer && aligned16(live + i)) {
+        const int4 a = reinterpret_cast<const int4*>(live + i)[0], b = reinterpret_cast<const int4*>(live + i)[1];
+        const int32_t c[kPer] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) on &= ~((static_cast<uint32_t>(c[k]) >> 31) << k);
+    } else {
+        for (int k = 0; k < left; ++k) on &= ~((static_cast<uint32_t>(live[i + k]) >> 31) << k);
+    }
+    return on;
+}
+
+// Eight elements of a tensor with 32-bit moments.
+template <typename T, bool PLAIN>
+__device__ __forceinline__ void step32(const Item& d, const Hyper& h, int64_t i, int left) {
+    T* P = static_cast<T*>(d.p);
+    const T* G = static_cast<const T*>(d.g);
+    float* M = static_cast<float*>(d.m);
+    float* V = static_cast<float*>(d.v);
+    const bool whole = left == kPer;
+    const bool pv = PLAIN || (whole && aligned16(P)), gv = PLAIN || (whole && aligned16(G)),
+               mv = PLAIN || (whole && aligned16(M)), vv = PLAIN || (whole && aligned16(V));
+    float p[kPer], g[kPer], m[kPer], v[kPer];
+    load(P, i, left, pv, p);
+    load(G, i, left, gv, g);
+    load(M, i, left, mv, m);
+    load(V, i, left, vv, v);
+    const uint32_t on = PLAIN ? 0xFFu : taking_part(d.live, i, left);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const float gf = g[k];
+        const float m1 = fmaf(gf - m[k], h.one_b1, m[k]);
+        const float v1 = fmaf(v[k], h.b2, gf * gf * h.one_b2);
+        if (PLAIN || (on >> k & 1)) {
+            p[k] = fmaf(-h.step_size, m1 / fmaf(sqrtf(v1), h.inv_root, h.eps), p[k] * h.decay);
+            m[k] = m1;
+            v[k] = v1;
+        }
+    }
+    store(P, i, left, pv, p);
+    store(M, i, left, mv, m);
+    store(V, i, left, vv, v);
+}
+
+// Eight elements of a block with 8-bit moments; a warp has the whole block.
+// The kernel is bound by its instructions as much as by its bytes (10 of a
+// 16-bit weight), so square root and quotient are the approximate ones (2^-22
+// of p's update), and padding, ends and odd addresses are kept out of the
+// ordinary path.
+template <typename T, bool PLAIN>
+__device__ __forceinline__ void step8(const Item& d, const Hyper& h, int64_t i, int64_t block, int left) {
+    T* P = static_cast<T*>(d.p);
+    const T* G = static_cast<const T*>(d.g);
+    uint8_t* M = static_cast<uint8_t*>(d.m) + i;
+    uint8_t* U = static_cast<uint8_t*>(d.v) + i;
+    const bool whole = left == kPer;
+    const bool pv = PLAIN || (whole && aligned16(P)), gv = PLAIN || (whole && aligned16(G)),
+               mv = PLAIN || (whole && (reinterpret_cast<uintptr_t>(M) & 7) == 0),
+               uv = PLAIN || (whole && (reinterpret_cast<uintptr_t>(U) & 7) == 0);
+    float p[kPer], g[kPer], m[kPer], u[kPer];
+    load(P, i, left, pv, p);
+    load(G, i, left, gv, g);
+    const uint2 cm = load8(M, left, mv), cu = load8(U, left, uv);
+    const uint32_t on = PLAIN ? 0xFFu : taking_part(d.live, i, left);
+    from_e4m3(cm, d.sm[block], m);
+    from_e4m3(cu, d.su[block], u);
+    float tm = 0.f, tu = 0.f;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const float gf = g[k];
+        const float m1 = fmaf(gf - m[k], h.one_b1, m[k]);
+        const float root = sqrt_fast(fmaf(u[k] * u[k], h.b2, gf * gf * h.one_b2));
+        if (PLAIN || (on >> k & 1)) {
+            p[k] = fmaf(-h.step_size, m1 * rcp_fast(fmaf(root, h.inv_root, h.eps)), p[k] * h.decay);
+            m[k] = m1;
+            u[k] = root;
+        }
+        tm = max_nan(tm, fabsf(m[k]));
+        tu = max_nan(tu, u[k]);
+    }
+    store(P, i, left, pv, p);
+    // the largest magnitudes' bits: what is not finite is above all that is
+    uint32_t bm = __reduce_max_sync(0xffffffffu, __float_as_uint(tm)), bu = __reduce_max_sync(0xffffffffu, __float_as_uint(tu));
+    uint32_t bad = 0;  // elements that are not finite: held as NaN, and no part of the scales
+    if (bm >= 0x7F800000u || bu >= 0x7F800000u) {
+        bm = bu = 0;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const uint32_t a = __float_as_uint(m[k]) & 0x7FFFFFFFu, b = __float_as_uint(u[k]) & 0x7FFFFFFFu;
+            if (a >= 0x7F800000u) bad |= 1u << k, m[k] = 0.f; else bm = max(bm, a);
+            if (b >= 0x7F800000u) bad |= 256u << k, u[k] = 0.f; else bu = max(bu, b);
+        }
+        bm = __reduce_max_sync(0xffffffffu, bm);
+        bu = __reduce_max_sync(0xffffffffu, bu);
+    }
+    const float fm = fmaxf(__uint_as_float(bm), 0x1p-100f), fu = fmaxf(__uint_as_float(bu), 0x1p-100f);
+    const float im = 448.f / fm, iu = 448.f / fu;
+    const uint32_t key = mix32(h.key + 0x85EBCA77u * d.number), first = static_cast<uint32_t>(i) * 0x9E3779B1u + key;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const uint32_t bits = mix32(first + k * 0x9E3779B1u);
+        const float floor = u[k] > 0.f ? 0.001953125f : 0.f;  // 2^-9, the smallest e4m3 value
+        m[k] = dithered(m[k] * im, bits & 0xFFFFu);
+        u[k] = fmaxf(dithered(u[k] * iu, bits >> 16), floor);
+    }
+    if (bad) {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            if (bad >> k & 1) m[k] = __int_as_float(0x7fffffff);
+            if (bad >> (8 + k) & 1) u[k] = __int_as_float(0x7fffffff);
+        }
+    }
+    store8(M, left, mv, to_e4m3(m));
+    store8(U, left, uv, to_e4m3(u));
+    if (lane_id() == 0) {
+        d.sm[block] = fm * (1.f / 448.f);
+        d.su[block] = fu * (1.f / 448.f);
+    }
 }
 
 template <typename T, bool EIGHT, int MAX>
 __global__ void __launch_bounds__(kThreads)
 adamw_multi_kernel(const __grid_constant__ Table<MAX> t, Hyper h, const Hyper* dev) {
     if (dev) h = *dev;
-    const int lane = lane_id(), warp = threadIdx.x >> 5;
+    int at = 0;
+    int64_t end = 0;
     for (int64_t tile = blockIdx.x; tile < t.tiles; tile += gridDim.x) {
-        int lo = 0, hi = t.count;
-        while (hi - lo > 1) {  // last tensor whose first tile is not behind
-            const int mid = (lo + hi) >> 1;
-            if (t.item[mid].first <= tile) lo = mid; else hi = mid;
+        if (tile >= end) {  // the last tensor whose first tile is not behind this one
+            int hi = t.count;
+            while (hi - at > 1) {
+                const int mid = (at + hi) >> 1;
+                if (t.item[mid].first <= tile) at = mid; else hi = mid;
+            }
+            end = at + 1 < t.count ? t.item[at + 1].first : t.tiles;
         }
-        const Item& d = t.item[lo];
+        const Item& d = t.item[at];
         const int64_t i = (tile - d.first) * kTile + threadIdx.x * kPer;
+        const bool full = (tile - d.first + 1) * kTile <= d.n;  // for the whole CTA
         const int64_t rest = d.n - i;
         const int left = rest >= kPer ? kPer : rest > 0 ? static_cast<int>(rest) : 0;
-        if (!EIGHT && left == 0) continue;
-        T* P = static_cast<T*>(d.p);
-        const T* G = static_cast<const T*>(d.g);
-        const bool whole = left == kPer;
-        const bool pv = whole && aligned16(P), gv = whole && aligned16(G);
-        T p[kPer], g[kPer];
-        float m[kPer], u[kPer];  // u: the second moment
-        bool on[kPer];
-        load(P, i, left, pv, p);
-        load(G, i, left, gv, g);
-        if (d.live) {
-            int32_t c[kPer];
-            if (whole && aligned16(d.live)) {
-                const int4 a = reinterpret_cast<const int4*>(d.live + i)[0], b = reinterpret_cast<const int4*>(d.live + i)[1];
-                c[0] = a.x; c[1] = a.y; c[2] = a.z; c[3] = a.w; c[4] = b.x; c[5] = b.y; c[6] = b.z; c[7] = b.w;
-            } else {
-#pragma unroll
-                for (int k = 0; k < kPer; ++k) c[k] = k < left ? d.live[i + k] : -1;
-            }
-#pragma unroll
-            for (int k = 0; k < kPer; ++k) on[k] = c[k] >= 0;
+        if constexpr (EIGHT) {
+            const int64_t block = (tile - d.first) * (kTile / kBlock) + (threadIdx.x >> 5);
+            if (full && d.plain) step8<T, true>(d, h, i, block, kPer);
+            else if (block * kBlock < d.n) step8<T, false>(d, h, i, block, left);
         } else {
-#pragma unroll
-            for (int k = 0; k < kPer; ++k) on[k] = k < left;
-        }
-        const int64_t block = (tile - d.first) * (kTile / kBlock) + warp;
-        const bool block_on = block * kBlock < d.n;  // the same in all lanes of the warp
-        bool mv = whole, uv = whole;
-        if (EIGHT) {
-            if (!block_on) continue;
-            const uint8_t* M = static_cast<const uint8_t*>(d.m);
-            const uint8_t* U = static_cast<const uint8_t*>(d.v);
-            mv = whole && (reinterpret_cast<uintptr_t>(M) & 7) == 0;
-            uv = whole && (reinterpret_cast<uintptr_t>(U) & 7) == 0;
-            uint8_t cm[kPer], cu[kPer];
-            load(M, i, left, mv, cm);
-            load(U, i, left, uv, cu);
-            const float sm = d.sm[block], su = d.su[block];
-#pragma unroll
-            for (int k = 0; k < kPer; ++k) {
-                m[k] = e4m3_to_f(cm[k]) * sm;
-                const float r = e4m3_to_f(cu[k]) * su;
-                u[k] = r * r;
-            }
-        } else {
-            const float* M = static_cast<const float*>(d.m);
-            const float* U = static_cast<const float*>(d.v);
-            mv = whole && aligned16(M);
-            uv = whole && aligned16(U);
-            load(M, i, left, mv, m);
-            load(U, i, left, uv, u);
-        }
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            const float gf = to_f(g[k]);
-            const float m1 = fmaf(gf - m[k], h.one_b1, m[k]);
-            const float v1 = fmaf(u[k], h.b2, gf * gf * h.one_b2);
-            const float root = sqrtf(v1);
-            if (on[k]) {
-                p[k] = from_f<T>(fmaf(-h.step_size, m1 / fmaf(root, h.inv_root, h.eps), to_f(p[k]) * h.decay));
-                m[k] = m1;
-                u[k] = EIGHT ? root : v1;
-            } else if (EIGHT) {
-                u[k] = sqrtf(u[k]);
-            }
-        }
-        store(P, i, left, pv, p);
-        if (!EIGHT) {
-            store(static_cast<float*>(d.m), i, left, mv, m);
-            store(static_cast<float*>(d.v), i, left, uv, u);
-            continue;
-        }
-        // The largest finite values of the block set the new scales; one that
-        // is not finite stays a NaN of its own and spoils no other element.
-        float tm = 0.f, tu = 0.f;
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            if (k >= left) m[k] = u[k] = 0.f;
-            if (fabsf(m[k]) <= 3.4028234e38f) tm = fmaxf(tm, fabsf(m[k]));
-            if (u[k] <= 3.4028234e38f) tu = fmaxf(tu, u[k]);
-        }
-        tm = fmaxf(warp_max(tm), 0x1p-100f);
-        tu = fmaxf(warp_max(tu), 0x1p-100f);
-        const float im = 448.f / tm, iu = 448.f / tu;
-        const uint32_t key = mix32(h.key + 0x85EBCA77u * d.number);
-        uint8_t cm[kPer], cu[kPer];
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            const uint32_t bits = mix32(static_cast<uint32_t>(i + k) * 0x9E3779B1u + key);
-            const float am = fabsf(m[k]);
-            uint32_t c = to_e4m3(am * im, bits & 0xFFFFu) | (m[k] < 0.f ? 0x80u : 0u);
-            cm[k] = static_cast<uint8_t>(am <= 3.4028234e38f ? c : 0x7Fu);
-            c = to_e4m3(u[k] * iu, bits >> 16);
-            if (c == 0 && u[k] > 0.f) c = 1;
-            cu[k] = static_cast<uint8_t>(u[k] <= 3.4028234e38f ? c : 0x7Fu);
-        }
-        store(static_cast<uint8_t*>(d.m), i, left, mv, cm);
-        store(static_cast<uint8_t*>(d.v), i, left, uv, cu);
-        if (lane == 0) {
-            d.sm[block] = tm * (1.f / 448.f);
-            d.su[block] = tu * (1.f / 448.f);
+            if (full && d.plain) step32<T, true>(d, h, i, kPer);
+            else if (left) step32<T, false>(d, h, i, left);
         }
     }
 }
@@ -268,7 +342,9 @@ int launch(const sl_adamw_item* items, int64_t count, const Hyper& h, const Hype
         for (; at < count && t.count < MAX; ++at) {
             const sl_adamw_item& a = items[at];
             if (a.n == 0) continue;
-            t.item[t.count++] = {a.p, a.g, a.m, a.v, a.scale_m, a.scale_v, a.live, a.n, t.tiles, static_cast<uint32_t>(a.number)};
+            const int64_t state = EIGHT ? 8 : 16;
+            const bool plain = !a.live && !off_by(a.p, 16) && !off_by(a.g, 16) && !off_by(a.m, state) && !off_by(a.v, state);
+            t.item[t.count++] = {a.p, a.g, a.m, a.v, a.scale_m, a.scale_v, a.live, a.n, t.tiles, static_cast<uint32_t>(a.number), plain};
             t.tiles += (a.n + kTile - 1) / kTile;
         }
         if (t.count == 0) continue;

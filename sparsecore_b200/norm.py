@@ -23,8 +23,6 @@ MAX_COLS = 16384
 
 
 def _vector(t, name, D, y):
-    if t is None:
-        return None
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"residual_norm: {name} must be a torch.Tensor, got {type(t).__name__}")
     if t.device != y.device:
@@ -33,63 +31,74 @@ def _vector(t, name, D, y):
         raise ValueError(f"residual_norm: {name} must have shape ({D},), got {tuple(t.shape)}")
     if t.dtype not in (y.dtype, torch.float32):
         raise ValueError(f"residual_norm: {name} must be {y.dtype} or torch.float32, got {t.dtype}")
-    return t
 
 
-def _forward(y, residual, weight, bias, gate, scale_t, pw, pb, kind, eps, post_eps, scale, keep_stats):
-    T, D = y.shape
-    y, residual = y.contiguous(), residual.contiguous()
-    weight, bias, gate, pw, pb = (t if t is None else t.contiguous() for t in (weight, bias, gate, pw, pb))
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _solid(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _sizes(dtype, rdtype, weight, gate, scale_t, T, D, opts):
+    """The plain numbers of sl_norm_args."""
+    kind, eps, post_eps, scale = opts
+    kinds = N.DTYPES
+    dt = kinds[dtype]
+    return (T, D, 1 if gate is None else gate.numel() // D, scale, eps, post_eps, kind, dt, kinds[rdtype],
+            kinds[weight.dtype], dt if gate is None else kinds[gate.dtype])
+
+
+def _forward(y, residual, weight, bias, gate, scale_t, pw, pb, opts, keep_stats):
+    D = y.shape[-1]
+    T = y.numel() // D
+    y, residual, weight, bias, gate, pw, pb = (_solid(t) for t in (y, residual, weight, bias, gate, pw, pb))
     out, h = torch.empty_like(residual), torch.empty_like(y)
-    stats = torch.empty(4, T, dtype=torch.float32, device=y.device) if keep_stats else None
-    a = _args(y.dtype, residual.dtype, weight, gate, T, D, kind, eps, post_eps, scale, scale_t)
-    a.y, a.residual, a.weight, a.bias = N.ptr(y), N.ptr(residual), N.ptr(weight), N.ptr(bias)
-    a.gate, a.post_weight, a.post_bias = N.ptr(gate), N.ptr(pw), N.ptr(pb)
-    a.out, a.h, a.stats = N.ptr(out), N.ptr(h), N.ptr(stats)
+    stats = torch.empty(4 * T, dtype=torch.float32, device=y.device) if keep_stats else None
+    a = N.SlNormArgs(y.data_ptr(), residual.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(gate), _ptr(pw), _ptr(pb),
+                     out.data_ptr(), h.data_ptr(), _ptr(stats), _ptr(scale_t), None, None, None, None, None, None, None,
+                     None, None, None, None, *_sizes(y.dtype, residual.dtype, weight, gate, scale_t, T, D, opts))
     N.call_on(y.device, "sl_norm_forward", N.byref(a))
     return out, h, (y, weight, bias, gate, pw, pb, stats)
 
 
 class _ResidualNormFunction(torch.autograd.Function):
     """Inputs ``(y, residual, weight, bias, gate, scale_t, post_weight,
-    post_bias, kind, eps, post_eps, scale)``; y and residual [rows, D], gate
-    [groups, D], the vectors of one type.  Returns ``(out, h)``."""
+    post_bias, (kind, eps, post_eps, scale))``, the vectors of one type.
+    Returns ``(out, h)``."""
 
     @staticmethod
-    def forward(ctx, y, residual, weight, bias, gate, scale_t, pw, pb, kind, eps, post_eps, scale):
-        out, h, (y, weight, bias, gate, pw, pb, stats) = _forward(y, residual, weight, bias, gate, scale_t, pw, pb, kind,
-                                                                  eps, post_eps, scale, True)
+    def forward(ctx, y, residual, weight, bias, gate, scale_t, pw, pb, opts):
+        out, h, (y, weight, bias, gate, pw, pb, stats) = _forward(y, residual, weight, bias, gate, scale_t, pw, pb, opts, True)
         need = ctx.needs_input_grad
         keep_y = pw is not None or need[4] or need[5]
         ctx.save_for_backward(y if keep_y else None, out, weight, bias, gate, scale_t, pw, pb, stats)
-        ctx.opts = (y.dtype, kind, eps, post_eps, scale)
+        ctx.opts = (y.dtype, opts)
         ctx.set_materialize_grads(False)
         return out, h
 
     @staticmethod
     def backward(ctx, dout, dh):
         y, out, weight, bias, gate, scale_t, pw, pb, stats = ctx.saved_tensors
-        dtype, kind, eps, post_eps, scale = ctx.opts
+        dtype, opts = ctx.opts
         need = ctx.needs_input_grad
-        T, D = out.shape
+        D = out.shape[-1]
+        T = out.numel() // D
         dev = out.device
-        dout, dh = (None if t is None else t.contiguous() for t in (dout, dh))
+        dout, dh = _solid(dout), _solid(dh)
         dr = torch.empty_like(out)
         # Without a norm, a gate or a scale after the block both gradients are the same numbers.
-        same = pw is None and gate is None and scale_t is None and scale == 1.0 and dtype == out.dtype
+        same = pw is None and gate is None and scale_t is None and opts[3] == 1.0 and dtype == out.dtype
         like = lambda t, i: torch.empty_like(t) if t is not None and need[i] else None  # noqa: E731
-        dy = torch.empty(T, D, dtype=dtype, device=dev) if need[0] and not same else None
-        dw, db, dpw, dpb, dgate = like(weight, 2), like(bias, 3), like(pw, 6), like(pb, 7), like(gate, 4)
-        ds = like(scale_t, 5)
+        dy = torch.empty(out.shape, dtype=dtype, device=dev) if need[0] and not same else None
+        dw, db, dpw, dpb, dgate, ds = (like(t, i) for t, i in ((weight, 2), (bias, 3), (pw, 6), (pb, 7), (gate, 4), (scale_t, 5)))
         if T:
-            a = _args(dtype, out.dtype, weight, gate, T, D, kind, eps, post_eps, scale, scale_t)
-            groups = gate.shape[0] if gate is not None else 1
-            ws = torch.empty(int(N.lib_on(dev).sl_norm_workspace_bytes(T, D, groups)), dtype=torch.uint8, device=dev)
-            a.y, a.out, a.weight, a.bias = N.ptr(y), N.ptr(out), N.ptr(weight), N.ptr(bias)
-            a.gate, a.post_weight, a.post_bias, a.stats = N.ptr(gate), N.ptr(pw), N.ptr(pb), N.ptr(stats)
-            a.dout, a.dh, a.dresidual, a.dy = N.ptr(dout), N.ptr(dh), N.ptr(dr), N.ptr(dy)
-            a.dgate, a.dweight, a.dbias = N.ptr(dgate), N.ptr(dw), N.ptr(db)
-            a.dpost_weight, a.dpost_bias, a.dscale, a.workspace = N.ptr(dpw), N.ptr(dpb), N.ptr(ds), N.ptr(ws)
+            sizes = _sizes(dtype, out.dtype, weight, gate, scale_t, T, D, opts)
+            ws = torch.empty(int(N.lib_on(dev).sl_norm_workspace_bytes(T, D, sizes[2])), dtype=torch.uint8, device=dev)
+            a = N.SlNormArgs(_ptr(y), None, weight.data_ptr(), _ptr(bias), _ptr(gate), _ptr(pw), _ptr(pb), out.data_ptr(),
+                             None, stats.data_ptr(), _ptr(scale_t), _ptr(dout), _ptr(dh), dr.data_ptr(), _ptr(dy),
+                             _ptr(dgate), _ptr(dw), _ptr(db), _ptr(dpw), _ptr(dpb), _ptr(ds), ws.data_ptr(), *sizes)
             N.call_on(dev, "sl_norm_backward", N.byref(a))
         else:
             for t in (dw, db, dpw, dpb, dgate, ds):
@@ -97,17 +106,7 @@ class _ResidualNormFunction(torch.autograd.Function):
                     t.zero_()
         if same and need[0]:
             dy = dr
-        return dy, dr if need[1] else None, dw, db, dgate, ds, dpw, dpb, None, None, None, None
-
-
-def _args(dtype, rdtype, weight, gate, T, D, kind, eps, post_eps, scale, scale_t):
-    a = N.SlNormArgs()
-    a.rows, a.cols, a.gate_groups = T, D, gate.shape[0] if gate is not None else 1
-    a.scale, a.eps, a.post_eps, a.kind = scale, eps, post_eps, kind
-    a.dtype, a.residual_dtype, a.weight_dtype = N.DTYPES[dtype], N.DTYPES[rdtype], N.DTYPES[weight.dtype]
-    a.gate_dtype = N.DTYPES[gate.dtype] if gate is not None else a.dtype
-    a.scale_dev = N.ptr(scale_t)
-    return a
+        return dy, dr if need[1] else None, dw, db, dgate, ds, dpw, dpb, None
 
 
 def residual_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -150,17 +149,17 @@ def residual_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
     D = y.shape[-1]
     if not 1 <= D <= MAX_COLS:
         raise ValueError(f"residual_norm: the last dimension must be 1 to {MAX_COLS}, got {D}")
-    vectors = {"weight": weight, "bias": bias, "post_weight": post_weight, "post_bias": post_bias}
-    for name, t in vectors.items():
-        _vector(t, name, D, y)
-    if len({t.dtype for t in vectors.values() if t is not None}) > 1:
-        raise ValueError("residual_norm: weight, bias, post_weight and post_bias must have one type")
+    _vector(weight, "weight", D, y)
+    for t, name in ((bias, "bias"), (post_weight, "post_weight"), (post_bias, "post_bias")):
+        if t is not None:
+            _vector(t, name, D, y)
+            if t.dtype != weight.dtype:
+                raise ValueError("residual_norm: weight, bias, post_weight and post_bias must have one type")
     if post_bias is not None and post_weight is None:
         raise ValueError("residual_norm: post_bias needs post_weight")
     eps, post_eps = float(eps), float(eps if post_eps is None else post_eps)
     if not eps >= 0.0 or not post_eps >= 0.0:
         raise ValueError(f"residual_norm: eps must not be negative, got {eps}, {post_eps}")
-    rows = y.numel() // D
     if gate is not None:
         if not isinstance(gate, torch.Tensor):
             raise TypeError(f"residual_norm: gate must be a torch.Tensor, got {type(gate).__name__}")
@@ -177,7 +176,6 @@ def residual_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
         if not (groups == 1 or whole or runs):
             raise ValueError(f"residual_norm: gate of shape {shape} is not [D], y's shape {tuple(y.shape)}, or "
                              f"[y.shape[0], 1, ..., D]")
-        gate = gate.reshape(groups, D)
     scale_t = None
     if isinstance(scale, torch.Tensor):
         if scale.device != y.device:
@@ -185,10 +183,9 @@ def residual_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
         if scale.numel() != 1 or scale.dtype != torch.float32:
             raise ValueError("residual_norm: a tensor scale must be one float32 element")
         scale, scale_t = 1.0, scale
-    args = (y.reshape(rows, D), residual.reshape(rows, D), weight, bias, gate, scale_t, post_weight, post_bias,
-            _KINDS[kind], eps, post_eps, float(scale))
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in args):
-        out, h = _ResidualNormFunction.apply(*args)
-    else:
-        out, h, _ = _forward(*args, False)
-    return out.reshape(y.shape), h.reshape(y.shape)
+    opts = (_KINDS[kind], eps, post_eps, float(scale))
+    if torch.is_grad_enabled() and (y.requires_grad or residual.requires_grad or weight.requires_grad
+                                    or any(t is not None and t.requires_grad
+                                           for t in (bias, gate, scale_t, post_weight, post_bias))):
+        return _ResidualNormFunction.apply(y, residual, weight, bias, gate, scale_t, post_weight, post_bias, opts)
+    return _forward(y, residual, weight, bias, gate, scale_t, post_weight, post_bias, opts, False)[:2]
