@@ -413,9 +413,9 @@ SL_API int sl_adamw_hyper(int64_t* step_dev, const float* lr_dev, double lr, dou
  * SL_F32).  gate: [gate_groups, cols], each row shared by rows / gate_groups
  * rows, or NULL.  scale_dev: a scale on the device in place of `scale`.
  * stats: float[4 * rows], written by the forward call (NULL: not kept) and
- * read by the backward one.  backward writes dresidual and every other
- * gradient whose pointer is set, from dout and dh (NULL: zero); workspace:
- * sl_norm_workspace_bytes() bytes. */
+ * read by the backward one.  backward reads y and out besides and writes
+ * dresidual, and every other gradient whose pointer is set, from dout and
+ * dh; workspace: sl_norm_workspace_bytes() bytes. */
 enum { SL_NORM_LAYER = 0, SL_NORM_RMS = 1, SL_NORM_MAX_COLS = 16384 };
 typedef struct sl_norm_args {
     const void* y;

@@ -17,8 +17,7 @@ int check(const sl_norm_args* n, const char* fn, bool back) {
     if (n->rows == 0) return SL_OK;
     SL_REQUIRE(n->weight && n->out, fn, "NULL operand");
     SL_REQUIRE(back || (n->y && n->residual && n->h), fn, "NULL operand");
-    SL_REQUIRE(!back || (n->stats && n->dresidual && n->workspace), fn, "NULL operand");
-    SL_REQUIRE(!back || n->y || !(n->post_weight || n->dgate || n->dscale), fn, "the block's output is needed");
+    SL_REQUIRE(!back || (n->y && n->stats && n->dout && n->dh && n->dresidual && n->workspace), fn, "NULL operand");
     SL_REQUIRE(!n->dgate || n->gate, fn, "a gradient of a gate that is not there");
     const int64_t e = dtype_bytes(n->dtype), er = dtype_bytes(n->residual_dtype), ew = dtype_bytes(n->weight_dtype),
                   eg = dtype_bytes(n->gate ? n->gate_dtype : SL_F32);

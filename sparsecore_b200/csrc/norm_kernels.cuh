@@ -66,12 +66,6 @@ struct Row {
         for (int j = 0; j < NV; ++j)
             if (col + j * step < cols) v[j] = *reinterpret_cast<const Pack<T, VE>*>(src + col + j * step);
     }
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int k = 0; k < VE; ++k) v[j].v[k] = from_f<T>(0.f);
-    }
     __device__ __forceinline__ void get(int j, float (&o)[VE]) const { unpack(v[j], o); }
 };
 
@@ -190,7 +184,7 @@ norm_fwd_kernel(Args<TY, TR> a) {
         if (POST) {
             load_v<TY, VE>(a.pw, a.vec_f32, c, q);
 #pragma unroll
-            for (int k = 0; k < VE; ++k) y[k] = (a.layer ? (y[k] - st.w) * st.z : y[k] * st.z) * q[k];
+            for (int k = 0; k < VE; ++k) y[k] = (y[k] - st.w) * st.z * q[k];
             if (a.pb) {
                 load_v<TY, VE>(a.pb, a.vec_f32, c, q);
 #pragma unroll
@@ -219,7 +213,7 @@ norm_fwd_kernel(Args<TY, TR> a) {
         float w[VE], o[VE];
         load_v<TY, VE>(a.w, a.vec_f32, c, w);
 #pragma unroll
-        for (int k = 0; k < VE; ++k) o[k] = (a.layer ? (r[j][k] - st.y) * st.x : r[j][k] * st.x) * w[k];
+        for (int k = 0; k < VE; ++k) o[k] = (r[j][k] - st.y) * st.x * w[k];
         if (a.b) {
             load_v<TY, VE>(a.b, a.vec_f32, c, w);
 #pragma unroll
@@ -266,8 +260,8 @@ norm_bwd_kernel(Args<TY, TR> a) {
         Row<TR, VE, NV> xr, dr;
         Row<TY, VE, NV> nr;
         xr.load(a.out + row, col, step, cols);
-        if (a.dh) nr.load(a.dh + row, col, step, cols); else nr.clear();
-        if (a.dout) dr.load(a.dout + row, col, step, cols); else dr.clear();
+        nr.load(a.dh + row, col, step, cols);
+        dr.load(a.dout + row, col, step, cols);
         const float4 st = a.stats[t];
         float c1 = 0.f, c2 = 0.f;
 #pragma unroll
@@ -457,9 +451,9 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
                     for (int q = 0; q < size; ++q) copy16(to + (R::first(op) + j * size + q) * lap, static_cast<const char*>(src) + 16 * q);
                 };
                 put(kX, a.out + i, R::kR);
-                if (a.dh) put(kDn, a.dh + i, R::kT);
-                if (a.dout) put(kD, a.dout + i, R::kR);
-                if (a.y) put(kY, a.y + i, R::kT);
+                put(kDn, a.dh + i, R::kT);
+                put(kD, a.dout + i, R::kR);
+                put(kY, a.y + i, R::kT);
                 if (ring_gate) put(kG, static_cast<const TY*>(a.gate) + i, R::kT);
             }
         }
@@ -468,10 +462,7 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
     // Vector j of an operand of row t.
     auto get = [&](auto type, int op, const auto* base, int64_t t, const char* from, int j, float (&o)[VE]) {
         using T = decltype(type);
-        if (base == nullptr) {
-#pragma unroll
-            for (int k = 0; k < VE; ++k) o[k] = 0.f;
-        } else if constexpr (RING) {
+        if constexpr (RING) {
             constexpr int size = VE * sizeof(T) / 16;
             Pack<T, VE> p;
 #pragma unroll

@@ -71,9 +71,8 @@ class _ResidualNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, residual, weight, bias, gate, scale_t, pw, pb, opts):
         out, h, (y, weight, bias, gate, pw, pb, stats) = _forward(y, residual, weight, bias, gate, scale_t, pw, pb, opts, True)
-        need = ctx.needs_input_grad
-        keep_y = pw is not None or need[4] or need[5]
-        ctx.save_for_backward(y if keep_y else None, out, weight, bias, gate, scale_t, pw, pb, stats)
+        plain = pw is None and gate is None and scale_t is None
+        ctx.save_for_backward(None if plain else y, out, weight, bias, gate, scale_t, pw, pb, stats)
         ctx.opts = (y.dtype, opts)
         ctx.set_materialize_grads(False)
         return out, h
@@ -86,7 +85,8 @@ class _ResidualNormFunction(torch.autograd.Function):
         D = out.shape[-1]
         T = out.numel() // D
         dev = out.device
-        dout, dh = _solid(dout), _solid(dh)
+        dout = torch.zeros_like(out) if dout is None else _solid(dout)  # an output that nothing used
+        dh = torch.zeros(out.shape, dtype=dtype, device=dev) if dh is None else _solid(dh)
         dr = torch.empty_like(out)
         # Without a norm, a gate or a scale after the block both gradients are the same numbers.
         same = pw is None and gate is None and scale_t is None and opts[3] == 1.0 and dtype == out.dtype
@@ -96,8 +96,8 @@ class _ResidualNormFunction(torch.autograd.Function):
         if T:
             sizes = _sizes(dtype, out.dtype, weight, gate, scale_t, T, D, opts)
             ws = torch.empty(int(N.lib_on(dev).sl_norm_workspace_bytes(T, D, sizes[2])), dtype=torch.uint8, device=dev)
-            a = N.SlNormArgs(_ptr(y), None, weight.data_ptr(), _ptr(bias), _ptr(gate), _ptr(pw), _ptr(pb), out.data_ptr(),
-                             None, stats.data_ptr(), _ptr(scale_t), _ptr(dout), _ptr(dh), dr.data_ptr(), _ptr(dy),
+            a = N.SlNormArgs((out if y is None else y).data_ptr(), None, weight.data_ptr(), _ptr(bias), _ptr(gate), _ptr(pw), _ptr(pb), out.data_ptr(),
+                             None, stats.data_ptr(), _ptr(scale_t), dout.data_ptr(), dh.data_ptr(), dr.data_ptr(), _ptr(dy),
                              _ptr(dgate), _ptr(dw), _ptr(db), _ptr(dpw), _ptr(dpb), _ptr(ds), ws.data_ptr(), *sizes)
             N.call_on(dev, "sl_norm_backward", N.byref(a))
         else:
