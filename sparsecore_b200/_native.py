@@ -186,7 +186,7 @@ KERNELS_PER_CALL = {
     "sl_set_regrow_draws": 0,  # host only
     "sl_probe_ffma": 1, "sl_probe_smem": 1,
     "sl_adamw_multi": 1, "sl_adamw_hyper": 1, "sl_norm_forward": 1, "sl_norm_backward": 2,
-    "sl_xent_sizes": 0, "sl_xent_forward": 4, "sl_xent_backward": 4,
+    "sl_xent_sizes": 0, "sl_xent_forward": 3, "sl_xent_backward": 3,
 }
 launches = {"count": 0}
 

@@ -25,13 +25,14 @@ namespace xent {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMaxBlocks = 1024;  // of an operand's pass
 
 struct Layout {
     int64_t dp;                              // columns of a plane's row
     int64_t tgt, row_max, row_inv, x, w, prep;  // offsets in `prep`, and its size
-    int64_t zt, part, fwd;                   // in the forward call's scratch
+    int64_t zt, part, sums, counts, maxima, fwd;  // in the forward call's scratch
     int64_t piece, gp;                       // vocabulary columns of a piece, of a G row
-    int64_t g, acc, slabs, slab_floats, bwd; // in the backward call's
+    int64_t g, acc, slabs, bwd;              // in the backward call's
 };
 
 int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
@@ -51,7 +52,9 @@ Layout layout(int64_t T, int64_t D, int64_t V, int dtype, bool copy_w) {
     o = 0;
     l.zt = take(4 * T);
     l.part = take((V + kPart - 1) / kPart * T * 8);
-    take(8 * ((T + 7) / 8));  // the finish's sums
+    l.sums = take(8 * ((T + 31) / 32));
+    l.counts = take(4 * ((T + 31) / 32));
+    l.maxima = take(4 * kMaxBlocks * 2);
     l.fwd = o;
     o = 0;
     // A piece's G: 256 MB at most, a multiple of the tile's 256 columns.
@@ -61,153 +64,207 @@ Layout layout(int64_t T, int64_t D, int64_t V, int dtype, bool copy_w) {
     l.gp = up(std::min(l.piece, V), 64);
     l.g = take(planes * T * l.gp * 2);
     l.acc = take(V > l.piece ? 4 * T * D : 0);
-    l.slab_floats = kSlabFloats;
-    l.slabs = take(4 * l.slab_floats);
+    const bool two = dtype == SL_F32;
+    const int64_t rest = V - (V - 1) / l.piece * l.piece;  // of the last piece
+    int64_t floats = 0;
+    for (const int64_t cols : {std::min(l.piece, V), rest})
+        floats = std::max({floats, split_sum(T, D, cols, two).floats, split_sum(cols, D, T, two).floats});
+    l.slabs = take(4 * floats);
     l.bwd = o;
     return l;
 }
 
 // ── operands ──
 
-// Largest finite magnitude of a 32-bit operand; the order of a maximum does
-// not change it.
-__global__ void __launch_bounds__(kThreads)
-absmax_kernel(const float* __restrict__ a, int64_t rows, int64_t cols, const int64_t* __restrict__ targets,
-              int64_t ignore, unsigned* out) {
-    float m = 0.f;
-    const int64_t n = rows * cols, step = static_cast<int64_t>(gridDim.x) * kThreads;
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < n; i += step) {
-        if (targets && targets[i / cols] == ignore) continue;
-        const float v = fabsf(a[i]);
-        if (v <= 3.4028234e38f) m = fmaxf(m, v);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane_id() == 0 && m > 0.f) atomicMax(out, __float_as_uint(m));
+// Sizes of the two operands' passes: rows of x, then rows of w.
+struct Source {
+    const void *x, *w;
+    const int64_t* targets;
+    int64_t T, V, D, ignore;
+};
+
+__device__ __forceinline__ unsigned block_max(unsigned v, unsigned* s) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if (lane_id() == 0) s[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = lane_id() < kThreads / 32 ? s[lane_id()] : 0u;
+    __syncthreads();
+    return __reduce_max_sync(0xffffffffu, v);
 }
 
-// Rows of an operand as planes, padded with zeros to `dp` columns; rows of
-// tokens that do not count become zeros, whatever they hold.
+__device__ __forceinline__ unsigned finite_bits(float v) {
+    const unsigned b = __float_as_uint(v) & 0x7FFFFFFFu;
+    return b < 0x7F800000u ? b : 0u;
+}
+
+// Largest finite magnitudes of 32-bit operands, a warp a row: CTAs below
+// `x_blocks` take x (rows of tokens that do not count are left out), the
+// others w; one value a CTA, joined by planes_kernel.
+__global__ void __launch_bounds__(kThreads)
+absmax_kernel(Source q, int x_blocks, unsigned* part, int vec) {
+    __shared__ unsigned s[kThreads / 32];
+    const bool is_w = blockIdx.x >= x_blocks;
+    const int64_t rows = is_w ? q.V : q.T, first = is_w ? blockIdx.x - x_blocks : blockIdx.x;
+    const int64_t step = (is_w ? gridDim.x - x_blocks : x_blocks) * static_cast<int64_t>(kThreads / 32);
+    const float* src = static_cast<const float*>(is_w ? q.w : q.x);
+    unsigned m = 0;
+    for (int64_t r = first * (kThreads / 32) + (threadIdx.x >> 5); r < rows; r += step) {
+        if (!is_w && q.targets[r] == q.ignore) continue;
+        const float* row = src + r * q.D;
+        if (vec) {
+#pragma unroll 4
+            for (int64_t c = lane_id() * 4; c < q.D; c += 128) {
+                const float4 v = *reinterpret_cast<const float4*>(row + c);
+                m = max(max(m, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
+            }
+        } else {
+            for (int64_t c = lane_id(); c < q.D; c += 32) m = max(m, finite_bits(row[c]));
+        }
+    }
+    m = block_max(m, s);
+    if (threadIdx.x == 0) part[blockIdx.x] = m;
+}
+
+// Rows of the operands as planes, padded with zeros to `dp` columns, a warp a
+// row; rows of tokens that do not count become zeros, whatever they hold.
+// Also the targets as 32-bit numbers.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-planes_kernel(const T* __restrict__ src, int64_t rows, int64_t cols, int64_t dp, const unsigned* max_bits,
-              const int* __restrict__ tgt, void* dst) {
-    const int64_t n = rows * dp, step = static_cast<int64_t>(gridDim.x) * kThreads;
-    const float scale = sizeof(T) == 4 ? exp2f(static_cast<float>(plane_exponent(*max_bits))) : 1.f;
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < n; i += step) {
-        const int64_t r = i / dp, c = i - r * dp;
-        const bool on = c < cols && !(tgt && tgt[r] == kIgnored);
-        if constexpr (sizeof(T) == 4) {
-            const float v = on ? src[r * cols + c] * scale : 0.f;
-            const __half hi = __float2half_rn(v);
-            static_cast<__half*>(dst)[i] = hi;
-            static_cast<__half*>(dst)[n + i] = __float2half_rn(v - __half2float(hi));
-        } else {
-            static_cast<T*>(dst)[i] = on ? src[r * cols + c] : from_f<T>(0.f);
+planes_kernel(Source q, int64_t dp, const unsigned* part, int x_blocks, int w_blocks, Header* head, int* __restrict__ tgt,
+              float* __restrict__ zt, void* xp, void* wp, int vec) {
+    __shared__ unsigned s[kThreads / 32];
+    float scale_x = 1.f, scale_w = 1.f;
+    if (sizeof(T) == 4) {
+        unsigned mx = 0, mw = 0;
+        for (int k = threadIdx.x; k < x_blocks; k += kThreads) mx = max(mx, part[k]);
+        for (int k = threadIdx.x; k < w_blocks; k += kThreads) mw = max(mw, part[x_blocks + k]);
+        mx = block_max(mx, s);
+        mw = block_max(mw, s);
+        scale_x = exp2f(static_cast<float>(plane_exponent(mx)));
+        scale_w = exp2f(static_cast<float>(plane_exponent(mw)));
+        if (blockIdx.x == 0 && threadIdx.x == 0) head->max_x = mx, head->max_w = mw;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) head->done = 0;
+    const int64_t rows = q.T + (wp ? q.V : 0), step = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
+    for (int64_t r = blockIdx.x * static_cast<int64_t>(kThreads / 32) + (threadIdx.x >> 5); r < rows; r += step) {
+        const bool is_w = r >= q.T;
+        const int64_t row = is_w ? r - q.T : r;
+        bool on = true;
+        if (!is_w) {
+            const int64_t v = q.targets[row];
+            on = v != q.ignore;
+            if (lane_id() == 0) {
+                const bool bad = on && (v < 0 || v >= q.V);
+                tgt[row] = !on ? kIgnored : bad ? kInvalid : static_cast<int>(v);
+                zt[row] = bad ? __int_as_float(0x7fffffff) : 0.f;  // no such token: its loss is NaN
+            }
+        }
+        const T* src = static_cast<const T*>(is_w ? q.w : q.x) + row * q.D;
+        const float scale = is_w ? scale_w : scale_x;
+        const int64_t plane = (is_w ? q.V : q.T) * dp;
+        uint16_t* dst = static_cast<uint16_t*>(is_w ? wp : xp) + row * dp;
+        for (int64_t c = lane_id() * 8; c < dp; c += 256) {
+            float v[8] = {};
+            if (on) {
+                if (vec && c < q.D) {
+                    load_f<T, 8>(src + c, v);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = c + k < q.D ? to_f(src[c + k]) : 0.f;
+                }
+            }
+            if constexpr (sizeof(T) == 4) {
+                float lo[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    v[k] *= scale;
+                    lo[k] = v[k] - __half2float(__float2half_rn(v[k]));
+                }
+                store_f<__half, 8>(reinterpret_cast<__half*>(dst) + c, v);
+                store_f<__half, 8>(reinterpret_cast<__half*>(dst) + plane + c, lo);
+            } else {
+                store_f<T, 8>(reinterpret_cast<T*>(dst) + c, v);
+            }
         }
     }
 }
 
-__global__ void __launch_bounds__(kThreads)
-targets_kernel(const int64_t* __restrict__ targets, int64_t T, int64_t V, int64_t ignore, int* __restrict__ tgt,
-               float* __restrict__ zt, Header* head) {
-    const int64_t t = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x;
-    bool on = false;
-    if (t < T) {
-        const int64_t v = targets[t];
-        on = v != ignore;
-        const bool bad = on && (v < 0 || v >= V);
-        tgt[t] = !on ? kIgnored : bad ? kInvalid : static_cast<int>(v);
-        zt[t] = bad ? __int_as_float(0x7fffffff) : 0.f;  // no such token: its loss is NaN
+// Largest finite magnitude of the single losses' gradients.
+__global__ void __launch_bounds__(1024)
+grad_max_kernel(const float* __restrict__ g, const int* __restrict__ tgt, int64_t T, Header* head) {
+    __shared__ unsigned s[32];
+    unsigned m = 0;
+    for (int64_t t = threadIdx.x; t < T; t += 1024)
+        if (tgt[t] != kIgnored) m = max(m, finite_bits(g[t]));
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane_id() == 0) s[threadIdx.x >> 5] = m;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        m = __reduce_max_sync(0xffffffffu, s[threadIdx.x]);
+        if (threadIdx.x == 0) head->max_g = m;
     }
-    const int c = __popc(__ballot_sync(0xffffffffu, on));
-    if (lane_id() == 0 && c) atomicAdd(&head->count, c);
 }
 
 // ── joining the partial sums ──
 
-__global__ void __launch_bounds__(kThreads)
-finish_kernel(Problem p, int64_t parts, float* __restrict__ rows, float* loss, double* sums, int mean) {
-    __shared__ double s[kThreads / 32];
+// (max, sum of exponentials below it) of two sets of logits.  An empty set is
+// (-inf, 0); equal infinities give a NaN, as they do in the definition.
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+    const float m = fmaxf(a.x, b.x);
+    return make_float2(m, (a.y == 0.f ? 0.f : a.y * expf(a.x - m)) + (b.y == 0.f ? 0.f : b.y * expf(b.x - m)));
+}
+
+// 32 rows a CTA, blockDim.y threads a row.
+__global__ void __launch_bounds__(1024)
+finish_kernel(Problem p, int parts, float* __restrict__ rows, float* loss, double* sums, int* counts) {
+    __shared__ float2 s[32][33];
+    __shared__ double total[32];
     __shared__ bool last;
-    const int warp = threadIdx.x >> 5, lane = lane_id();
-    const int64_t t = blockIdx.x * static_cast<int64_t>(kThreads / 32) + warp;
-    double mine = 0.0;
-    if (t < p.T) {
-        float m = -INFINITY, sum = 0.f;
-        for (int64_t k = lane; k < parts; k += 32) {
-            const float2 q = p.part[k * p.T + t];
-            const float n = fmaxf(m, q.x);
-            // an empty side has m = -inf; equal infinities stay a NaN, as they are in the definition
-            sum = (sum == 0.f ? 0.f : sum * expf(m - n)) + (q.y == 0.f ? 0.f : q.y * expf(q.x - n));
-            m = n;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float qm = __shfl_xor_sync(0xffffffffu, m, o), qs = __shfl_xor_sync(0xffffffffu, sum, o);
-            const float n = fmaxf(m, qm);
-            sum = (sum == 0.f ? 0.f : sum * expf(m - n)) + (qs == 0.f ? 0.f : qs * expf(qm - n));
-            m = n;
-        }
-        const int tg = p.tgt[t];
-        const float l = tg == kIgnored ? 0.f : m + logf(sum) - p.zt[t];
-        if (lane == 0) {
-            p.row_max[t] = m;
-            p.row_inv[t] = tg == kInvalid ? __int_as_float(0x7fffffff) : 1.f / sum;
-            if (rows) rows[t] = l;
-            mine = l;
-        }
-    }
-    if (!loss) return;
-    if (lane == 0) s[warp] = mine;
+    const int64_t t = blockIdx.x * static_cast<int64_t>(32) + threadIdx.x;
+    float2 q = make_float2(-INFINITY, 0.f);
+    if (t < p.T)
+        for (int k = threadIdx.y; k < parts; k += blockDim.y) q = join(q, p.part[k * p.T + t]);
+    s[threadIdx.y][threadIdx.x] = q;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        double a = 0.0;
-        for (int k = 0; k < kThreads / 32; ++k) a += s[k];
-        sums[blockIdx.x] = a;
-        __threadfence();
-        last = atomicAdd(&p.head->done, 1u) == gridDim.x - 1;
+    if (threadIdx.y == 0) {
+        for (int k = 1; k < blockDim.y; ++k) q = join(q, s[k][threadIdx.x]);
+        const int tg = t < p.T ? p.tgt[t] : kIgnored;
+        const float l = tg == kIgnored ? 0.f : q.x + logf(q.y) - p.zt[t];
+        if (t < p.T) {
+            p.row_max[t] = q.x;
+            p.row_inv[t] = tg == kInvalid ? __int_as_float(0x7fffffff) : 1.f / q.y;
+            if (rows) rows[t] = l;
+        }
+        double a = l;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+        const int n = __popc(__ballot_sync(0xffffffffu, tg != kIgnored));
+        if (threadIdx.x == 0) {
+            sums[blockIdx.x] = a;
+            counts[blockIdx.x] = n;
+            __threadfence();
+            last = atomicAdd(&p.head->done, 1u) == gridDim.x - 1;
+        }
     }
     __syncthreads();
     if (!last) return;
     __threadfence();
     // The CTA that comes last adds all sums in their order, whoever it is.
+    const int tid = threadIdx.y * 32 + threadIdx.x, threads = blockDim.y * 32;
     double a = 0.0;
-    for (int64_t k = threadIdx.x; k < gridDim.x; k += kThreads) a += __ldcg(sums + k);
+    int n = 0;
+    for (int64_t k = tid; k < gridDim.x; k += threads) a += __ldcg(sums + k), n += __ldcg(counts + k);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    n = __reduce_add_sync(0xffffffffu, n);
+    __shared__ int found[32];
+    if (threadIdx.x == 0) total[threadIdx.y] = a, found[threadIdx.y] = n;
     __syncthreads();
-    if (lane == 0) s[warp] = a;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        a = 0.0;
-        for (int k = 0; k < kThreads / 32; ++k) a += s[k];
-        *loss = static_cast<float>(mean ? a / p.head->count : a);
-        p.head->done = 0;
-    }
-}
-
-__global__ void grad_scale_kernel(Header* head, const float* grad, int mean) {
-    float g = grad ? *grad : __uint_as_float(head->max_g);
-    if (mean) g = head->count ? g / static_cast<float>(head->count) : 0.f;
-    head->g = g;
-}
-
-unsigned blocks_for(int64_t n) {
-    return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((n + kThreads - 1) / kThreads, num_sms() * 16)));
-}
-
-template <typename T>
-void to_planes(const void* src, int64_t rows, int64_t cols, int64_t dp, const unsigned* bits, const int* tgt, void* dst,
-               cudaStream_t s) {
-    planes_kernel<T><<<blocks_for(rows * dp), kThreads, 0, s>>>(static_cast<const T*>(src), rows, cols, dp, bits, tgt, dst);
-}
-
-void to_planes(int dtype, const void* src, int64_t rows, int64_t cols, int64_t dp, const unsigned* bits, const int* tgt,
-               void* dst, cudaStream_t s) {
-    if (dtype == SL_F32) to_planes<float>(src, rows, cols, dp, bits, tgt, dst, s);
-    else if (dtype == SL_BF16) to_planes<__nv_bfloat16>(src, rows, cols, dp, bits, tgt, dst, s);
-    else to_planes<__half>(src, rows, cols, dp, bits, tgt, dst, s);
+    if (tid) return;
+    a = 0.0, n = 0;
+    for (int k = 0; k < blockDim.y; ++k) a += total[k], n += found[k];
+    p.head->count = n;
+    if (loss) *loss = static_cast<float>(p.mean ? a / n : a);
 }
 
 // 16-bit weights are read where they lie when their rows start on 16 bytes.
@@ -248,31 +305,47 @@ Setup setup(const sl_xent_args& a) {
     s.p.T = a.tokens; s.p.D = a.dim; s.p.V = a.vocab;
     s.p.f32 = a.dtype == SL_F32;
     s.p.bf16 = a.dtype == SL_BF16;
+    s.p.mean = a.reduction == SL_XENT_MEAN;
     s.x = {s.prep + s.l.x, a.tokens, a.dim, s.l.dp, a.tokens * s.l.dp};
     s.w = copy ? Operand{s.prep + s.l.w, a.vocab, a.dim, s.l.dp, a.vocab * s.l.dp}
                : Operand{a.weight, a.vocab, a.dim, a.dim, 0};
     return s;
 }
 
+int blocks_for(int64_t rows) {
+    const int64_t most = std::min<int64_t>(kMaxBlocks, static_cast<int64_t>(num_sms()) * 6);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((rows + kThreads / 32 - 1) / (kThreads / 32), most)));
+}
+
 int forward(const sl_xent_args& a, cudaStream_t st) {
     Setup s = setup(a);
     const int64_t T = a.tokens, V = a.vocab;
-    if (int rc = cuda_status(cudaMemsetAsync(s.prep, 0, 256, st), "sl_xent_forward")) return rc;
     s.p.zt = reinterpret_cast<float*>(s.scratch + s.l.zt);
     s.p.part = reinterpret_cast<float2*>(s.scratch + s.l.part);
     int* tgt = reinterpret_cast<int*>(s.prep + s.l.tgt);
-    targets_kernel<<<static_cast<unsigned>((T + kThreads - 1) / kThreads), kThreads, 0, st>>>(a.targets, T, V, a.ignore_index, tgt, s.p.zt, s.p.head);
+    unsigned* maxima = reinterpret_cast<unsigned*>(s.scratch + s.l.maxima);
+    const bool copy = copies_w(a);
+    const Source src{a.x, a.weight, a.targets, T, V, a.dim, a.ignore_index};
+    const int vec = a.dim % 8 == 0 && !off_by(a.x, 16) && !off_by(a.weight, 16);
+    const int bx = blocks_for(T), bw = blocks_for(V);
+    void *xp = s.prep + s.l.x, *wp = copy ? s.prep + s.l.w : nullptr;
+    const int blocks = blocks_for(T + (copy ? V : 0));
     if (s.p.f32) {
-        absmax_kernel<<<blocks_for(T * a.dim), kThreads, 0, st>>>(static_cast<const float*>(a.x), T, a.dim, a.targets, a.ignore_index, &s.p.head->max_x);
-        absmax_kernel<<<blocks_for(V * a.dim), kThreads, 0, st>>>(static_cast<const float*>(a.weight), V, a.dim, nullptr, 0, &s.p.head->max_w);
+        absmax_kernel<<<bx + bw, kThreads, 0, st>>>(src, bx, maxima, vec);
+        planes_kernel<float><<<blocks, kThreads, 0, st>>>(src, s.l.dp, maxima, bx, bw, s.p.head, tgt, s.p.zt, xp, wp, vec);
+    } else if (s.p.bf16) {
+        planes_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(src, s.l.dp, nullptr, 0, 0, s.p.head, tgt, s.p.zt, xp, wp, vec);
+    } else {
+        planes_kernel<__half><<<blocks, kThreads, 0, st>>>(src, s.l.dp, nullptr, 0, 0, s.p.head, tgt, s.p.zt, xp, wp, vec);
     }
-    to_planes(a.dtype, a.x, T, a.dim, s.l.dp, &s.p.head->max_x, tgt, s.prep + s.l.x, st);
-    if (copies_w(a)) to_planes(a.dtype, a.weight, V, a.dim, s.l.dp, &s.p.head->max_w, nullptr, s.prep + s.l.w, st);
     SL_RETURN_IF_LAUNCH_FAILED("sl_xent_forward");
     if (int rc = gemm_stats(s.p, s.x, s.w, st)) return rc;
-    const int64_t parts = (V + kPart - 1) / kPart, blocks = (T + 7) / 8;
-    double* sums = reinterpret_cast<double*>(s.scratch + s.l.fwd - up(8 * blocks, 256));
-    finish_kernel<<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(s.p, parts, a.loss_rows, a.loss, sums, a.reduction == SL_XENT_MEAN);
+    const int parts = static_cast<int>((V + kPart - 1) / kPart);
+    int groups = 1;
+    while (groups < parts && groups < 32) groups *= 2;
+    finish_kernel<<<static_cast<unsigned>((T + 31) / 32), dim3(32, groups), 0, st>>>(
+        s.p, parts, a.loss_rows, a.loss, reinterpret_cast<double*>(s.scratch + s.l.sums),
+        reinterpret_cast<int*>(s.scratch + s.l.counts));
     SL_RETURN_IF_LAUNCH_FAILED("sl_xent_forward");
     return SL_OK;
 }
@@ -281,12 +354,12 @@ int backward(const sl_xent_args& a, cudaStream_t st) {
     Setup s = setup(a);
     const int64_t T = a.tokens, V = a.vocab;
     if (a.reduction == SL_XENT_NONE) {
-        if (int rc = cuda_status(cudaMemsetAsync(&s.p.head->max_g, 0, 4, st), "sl_xent_backward")) return rc;
-        absmax_kernel<<<blocks_for(T), kThreads, 0, st>>>(a.grad, T, 1, a.targets, a.ignore_index, &s.p.head->max_g);
         s.p.g_rows = a.grad;
+        grad_max_kernel<<<1, 1024, 0, st>>>(a.grad, s.p.tgt, T, s.p.head);
+        SL_RETURN_IF_LAUNCH_FAILED("sl_xent_backward");
+    } else {
+        s.p.grad = a.grad;
     }
-    grad_scale_kernel<<<1, 1, 0, st>>>(s.p.head, a.reduction == SL_XENT_NONE ? nullptr : a.grad, a.reduction == SL_XENT_MEAN);
-    SL_RETURN_IF_LAUNCH_FAILED("sl_xent_backward");
     float* slabs = reinterpret_cast<float*>(s.scratch + s.l.slabs);
     for (int64_t v0 = 0; v0 < V; v0 += s.l.piece) {
         const int64_t cols = std::min(s.l.piece, V - v0);
@@ -294,12 +367,12 @@ int backward(const sl_xent_args& a, cudaStream_t st) {
         if (int rc = gemm_grad(s.p, s.x, s.w, v0, cols, g, st)) return rc;
         if (a.dx) {
             const Output o{a.dx, a.dtype, V > s.l.piece ? reinterpret_cast<float*>(s.scratch + s.l.acc) : nullptr, v0 == 0,
-                           v0 + cols == V, slabs, s.l.slab_floats, false};
+                           v0 + cols == V, slabs, false};
             if (int rc = gemm_dx(s.p, g, cols, s.w, v0, o, st)) return rc;
         }
         if (a.dweight) {
             const Output o{static_cast<char*>(a.dweight) + v0 * a.dim * dtype_bytes(a.dtype), a.dtype, nullptr, true, true,
-                           slabs, s.l.slab_floats, true};
+                           slabs, true};
             if (int rc = gemm_dw(s.p, g, cols, s.x, o, st)) return rc;
         }
     }

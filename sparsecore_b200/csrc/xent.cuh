@@ -8,9 +8,7 @@ namespace slb {
 namespace xent {
 
 constexpr int kPart = 128;          // vocabulary columns of one partial (max, sum) of a row
-// Sums of 256 x 256 that a split product may leave to be joined: one for each
-// pair of a B200's 148 SMs.
-constexpr int64_t kSlabFloats = 74 * 65536;
+constexpr int64_t kMostSlabFloats = int64_t(16) << 20;  // sums that a split product may leave to be joined
 constexpr float kGradScale = 32768.f;  // softmax - onehot is held in fp16 times 2^15
 
 // First bytes of the `prep` buffer.
@@ -18,7 +16,6 @@ struct Header {
     unsigned max_x, max_w, max_g;  // bits of the largest finite |.|
     int count;                     // tokens that count
     unsigned done;                 // CTAs of the finish that have written their sums
-    float g;                       // what every gradient is multiplied by at the end
 };
 
 enum : int { kIgnored = -1, kInvalid = -2 };  // in place of a target
@@ -46,11 +43,21 @@ struct Problem {
     float* row_inv;         // [T] one over its sum
     float* zt;              // [T] logit of the target
     float2* part;           // [parts][T]
-    const float* g_rows;    // [T] gradients of the single losses, or null
+    const float* grad;      // the loss's gradient, or
+    const float* g_rows;    // [T] gradients of the single losses
+    bool mean;
     int64_t T, D, V;
     bool f32;               // planes of fp16 pairs, scaled
     bool bf16;
 };
+
+// How a product [M, N] with a sum of K is split over the sum, and the floats
+// that its parts leave to be joined (0: not split).
+struct SplitSum {
+    int splits, per_split;  // slices of 64 of the sum
+    int64_t floats;
+};
+SplitSum split_sum(int64_t M, int64_t N, int64_t K, bool two_planes);
 
 // C[m, n] = sum over k of A . B^T, and what becomes of it.
 int gemm_stats(const Problem& p, const Operand& x, const Operand& w, cudaStream_t s);
@@ -64,7 +71,6 @@ struct Output {
     float* acc;       // [M, N] sums of the pieces so far, or null
     bool first, last; // piece
     float* slabs;     // workspace of a split sum
-    int64_t slab_floats;
     bool by_x;        // undo x's scale, not w's
 };
 // dx += G[T, cols] . W[cols, D]

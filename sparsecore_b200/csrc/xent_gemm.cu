@@ -127,7 +127,10 @@ __device__ __forceinline__ void epilogue_grad(const Args& a, float (&z)[128], in
     const int tg = a.p.tgt[t];
     const int at = tg >= 0 && tg - a.v0 - n0 >= 0 && tg - a.v0 - n0 < 128 ? static_cast<int>(tg - a.v0 - n0) : -1;
     float one = a.p.bf16 ? 1.f : kGradScale;
-    if (a.p.g_rows) one = a.p.head->g > 0.f ? one * (a.p.g_rows[t] / a.p.head->g) : 0.f;
+    if (a.p.g_rows) {  // single losses' gradients, over the largest
+        const float top = __uint_as_float(a.p.head->max_g);
+        one = top > 0.f ? one * (a.p.g_rows[t] / top) : 0.f;
+    }
     const float m = a.p.row_max[t], c = a.p.row_inv[t] * one;
     const bool on = tg != kIgnored;
     char* dst = static_cast<char*>(a.g) + 2 * (t * a.g_stride + n0);
@@ -159,7 +162,9 @@ __device__ __forceinline__ void epilogue_grad(const Args& a, float (&z)[128], in
 
 // What is multiplied into a finished sum.
 __device__ __forceinline__ float out_scale(const Problem& p, bool by_x, bool f32) {
-    const float g = (p.bf16 ? 1.f : 1.f / kGradScale) * p.head->g;
+    float g = p.g_rows ? __uint_as_float(p.head->max_g) : *p.grad;
+    if (p.mean) g = p.head->count ? g / static_cast<float>(p.head->count) : 0.f;
+    if (!p.bf16) g *= 1.f / kGradScale;
     return f32 ? g * exp2f(-static_cast<float>(plane_exponent(by_x ? p.head->max_x : p.head->max_w))) : g;
 }
 
@@ -404,10 +409,17 @@ join_kernel(Problem p, Output o, int64_t M, int64_t N, int64_t stride, int64_t s
 }
 
 template <int PL, int MODE>
-int launch(const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, cudaStream_t s) {
+int launch(const Operand& A, const Operand& B, const Args& a, cudaStream_t s) {
+    // The first runtime call of this thread, maybe (a backward pass has its
+    // own): it makes the context current that the encoder needs.
     if (int rc = cuda_status(cudaFuncSetAttribute(gemm_kernel<PL, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                   static_cast<int>(kSmem)), "sl_xent"))
         return rc;
+    CUtensorMap ma, mb;
+    auto map = [&](CUtensorMap* m, const Operand& o, bool mn) {
+        return make_tmap_16bit(m, o.base, a.p.bf16, o.cols, o.rows, PL, o.stride, PL == 2 ? o.plane : o.stride * o.rows, mn ? 64 : 128);
+    };
+    if (!map(&ma, A, a.a_mn) || !map(&mb, B, a.b_mn)) return fail(SL_ERR_CUDA, "sl_xent: tensor map could not be made");
     const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits;
     const int64_t pairs = std::min<int64_t>(tiles, std::max(1, num_sms() / 2));
     gemm_kernel<PL, MODE><<<static_cast<unsigned>(2 * pairs), kThreads, kSmem, s>>>(ma, mb, a);
@@ -417,31 +429,22 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, cudaStre
 
 template <int MODE>
 int run(Args& a, const Operand& A, const Operand& B, cudaStream_t s) {
-    CUtensorMap ma, mb;
-    const int planes = a.p.f32 ? 2 : 1;
-    if (!make_tmap_16bit(&ma, A.base, a.p.bf16, A.cols, A.rows, planes, A.stride, planes == 2 ? A.plane : A.stride * A.rows, a.a_mn ? 64 : 128) ||
-        !make_tmap_16bit(&mb, B.base, a.p.bf16, B.cols, B.rows, planes, B.stride, planes == 2 ? B.plane : B.stride * B.rows, a.b_mn ? 64 : 128))
-        return fail(SL_ERR_CUDA, "sl_xent: tensor map could not be made");
     a.status = device_status_word();
     if (a.status == nullptr) return fail(SL_ERR_CUDA, "sl_xent: no device status word");
     a.tiles_m = static_cast<int>((a.M + kTile - 1) / kTile);
     a.tiles_n = static_cast<int>((a.N + kTile - 1) / kTile);
-    const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n, pairs = std::max(1, num_sms() / 2);
+    const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
     SL_REQUIRE(tiles * 2 <= INT_MAX, "sl_xent", "too many tiles");
     const int all = static_cast<int>((a.K + kSlice - 1) / kSlice);
     a.splits = 1;
     a.per_split = all;
     if (MODE == kOut) {
-        // Few tiles and a long sum: the sum is split so that all pairs of SMs
-        // have a part, of eight stages at least.
+        const SplitSum sp = split_sum(a.M, a.N, a.K, a.p.f32);
+        a.splits = sp.splits;
+        a.per_split = sp.per_split;
         a.slab_stride = a.M * a.tiles_n * kTile;
-        const int64_t want = std::min({pairs / tiles, static_cast<int64_t>(all / 8), a.o.slab_floats / a.slab_stride});
-        if (want > 1) {
-            a.per_split = static_cast<int>((all + want - 1) / want);
-            a.splits = (all + a.per_split - 1) / a.per_split;
-        }
     }
-    if (int rc = a.p.f32 ? launch<2, MODE>(ma, mb, a, s) : launch<1, MODE>(ma, mb, a, s)) return rc;
+    if (int rc = a.p.f32 ? launch<2, MODE>(A, B, a, s) : launch<1, MODE>(A, B, a, s)) return rc;
     if (a.splits > 1) {
         const int64_t blocks = std::min<int64_t>((a.M * a.N + 255) / 256, num_sms() * 8);
         join_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(a.p, a.o, a.M, a.N, static_cast<int64_t>(a.tiles_n) * kTile, a.slab_stride, a.splits, a.p.f32);
@@ -457,6 +460,30 @@ Operand rows_from(Operand o, int64_t from, int64_t n) {
 }
 
 }  // namespace
+
+// The tiles go over the 74 pairs of SMs in waves; splitting the sum fills the
+// last wave (and the first, where there are few tiles) for the price of
+// writing, reading and joining the parts.  In clocks: a slice of 64 takes
+// 512 (1536 for three products), a tile's end about 3000, a join's launch
+// 5000 and memory 3000 bytes a clock.  4096 x 768 from 12544 columns in 32
+// bits (48 tiles): 3 parts, 250 -> 190 us.
+SplitSum split_sum(int64_t M, int64_t N, int64_t K, bool two_planes) {
+    constexpr int64_t kPairs = 74;
+    const int64_t tiles_n = (N + kTile - 1) / kTile, tiles = (M + kTile - 1) / kTile * tiles_n, all = (K + kSlice - 1) / kSlice;
+    const int64_t slice = two_planes ? 1536 : 512, slab = M * tiles_n * kTile;
+    SplitSum best{1, static_cast<int>(all), 0};
+    int64_t least = INT64_MAX;
+    for (int64_t s = 1; s <= 64 && 4 * (s - 1) < all && (s == 1 || s * slab <= kMostSlabFloats); ++s) {
+        const int64_t per = (all + s - 1) / s, parts = (all + per - 1) / per;
+        const int64_t cost = (tiles * parts + kPairs - 1) / kPairs * (per * slice + 3000) +
+                             (parts > 1 ? 5000 + M * N * 4 * (parts + 1) / 3000 : 0);
+        if (cost < least) {
+            least = cost;
+            best = {static_cast<int>(parts), static_cast<int>(per), parts > 1 ? parts * slab : 0};
+        }
+    }
+    return best;
+}
 
 int gemm_stats(const Problem& p, const Operand& x, const Operand& w, cudaStream_t s) {
     Args a{};
