@@ -464,7 +464,8 @@ SL_API int sl_norm_backward(const sl_norm_args* args, void* stream);
  * loss.  loss: one float (mean over the tokens that count, or sum);
  * loss_rows: float[tokens], written where set (required with
  * SL_XENT_NONE).  prep (kept from forward to backward) and scratch: sizes by
- * sl_xent_sizes, 256-byte aligned.  backward: grad is one float (mean, sum)
+ * sl_xent_sizes, 256-byte aligned.  train: a backward call will follow (with
+ * the same arguments otherwise).  backward: grad is one float (mean, sum)
  * or float[tokens]; dx [tokens, dim] and dweight [vocab, dim] are written
  * where set. */
 enum { SL_XENT_MEAN = 0, SL_XENT_SUM = 1, SL_XENT_NONE = 2 };
@@ -485,6 +486,7 @@ typedef struct sl_xent_args {
     int64_t ignore_index;
     int dtype;
     int reduction;
+    int train;
 } sl_xent_args;
 SL_API int sl_xent_sizes(const sl_xent_args* args, int64_t* prep, int64_t* forward, int64_t* backward);
 SL_API int sl_xent_forward(const sl_xent_args* args, void* stream);

@@ -53,7 +53,7 @@ class SlXentArgs(ctypes.Structure):
     """Mirror of `sl_xent_args`."""
 
     _fields_ = ([(n, P) for n in ("x", "weight", "targets", "loss", "loss_rows", "prep", "scratch", "grad", "dx", "dweight")]
-                + [(n, I64) for n in ("tokens", "dim", "vocab", "ignore_index")] + [("dtype", I32), ("reduction", I32)])
+                + [(n, I64) for n in ("tokens", "dim", "vocab", "ignore_index")] + [("dtype", I32), ("reduction", I32), ("train", I32)])
 
 
 # Element types of the training step's dense operators (SL_F32 ...).
@@ -191,18 +191,19 @@ KERNELS_PER_CALL = {
 launches = {"count": 0}
 
 
-_fns: dict = {}
+_fns: dict = {}  # name -> (the library it is of, its entry point, its kernels)
 
 
 def call(name: str, *args) -> None:
     """Invoke a status-returning entry point; raise on error; count launches."""
-    lb = lib()
-    fn = _fns.get((id(lb), name))
-    if fn is None:
-        fn = _fns[(id(lb), name)] = getattr(lb, name)
-    rc = fn(*args)
-    launches["count"] += KERNELS_PER_CALL.get(name, 1)
-    check(rc, name)
+    lb = _lib or lib()
+    got = _fns.get(name)
+    if got is None or got[0] is not lb:
+        got = _fns[name] = (lb, getattr(lb, name), KERNELS_PER_CALL.get(name, 1))
+    rc = got[1](*args)
+    launches["count"] += got[2]
+    if rc:
+        check(rc, name)
 
 
 def lib_on(device: torch.device) -> ctypes.CDLL:

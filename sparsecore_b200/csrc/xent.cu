@@ -29,7 +29,7 @@ constexpr int kMaxBlocks = 1024;  // of an operand's pass
 
 struct Layout {
     int64_t dp;                              // columns of a plane's row
-    int64_t tgt, row_max, row_inv, x, w, prep;  // offsets in `prep`, and its size
+    int64_t row_max, row_inv, x, w, prep;    // offsets in `prep`, and its size
     int64_t zt, part, sums, counts, maxima, fwd;  // in the forward call's scratch
     int64_t piece, gp;                       // vocabulary columns of a piece, of a G row
     int64_t g, acc, slabs, bwd;              // in the backward call's
@@ -37,16 +37,15 @@ struct Layout {
 
 int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
-Layout layout(int64_t T, int64_t D, int64_t V, int dtype, bool copy_w) {
+Layout layout(int64_t T, int64_t D, int64_t V, int dtype, bool copy_x, bool copy_w) {
     Layout l{};
     const int64_t planes = dtype == SL_F32 ? 2 : 1;
     l.dp = up(D, 64);
     int64_t o = 256;
     auto take = [&](int64_t bytes) { const int64_t at = o; o += up(bytes, 256); return at; };
-    l.tgt = take(4 * T);
     l.row_max = take(4 * T);
     l.row_inv = take(4 * T);
-    l.x = take(planes * T * l.dp * 2);
+    l.x = take(copy_x ? planes * T * l.dp * 2 : 0);
     l.w = take(copy_w ? planes * V * l.dp * 2 : 0);
     l.prep = o;
     o = 0;
@@ -127,11 +126,10 @@ absmax_kernel(Source q, int x_blocks, unsigned* part, int vec) {
 
 // Rows of the operands as planes, padded with zeros to `dp` columns, a warp a
 // row; rows of tokens that do not count become zeros, whatever they hold.
-// Also the targets as 32-bit numbers.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-planes_kernel(Source q, int64_t dp, const unsigned* part, int x_blocks, int w_blocks, Header* head, int* __restrict__ tgt,
-              float* __restrict__ zt, void* xp, void* wp, int vec) {
+planes_kernel(Source q, int64_t dp, const unsigned* part, int x_blocks, int w_blocks, Header* head, void* xp,
+              void* wp, int vec) {
     __shared__ unsigned s[kThreads / 32];
     float scale_x = 1.f, scale_w = 1.f;
     if (sizeof(T) == 4) {
@@ -144,21 +142,11 @@ planes_kernel(Source q, int64_t dp, const unsigned* part, int x_blocks, int w_bl
         scale_w = exp2f(static_cast<float>(plane_exponent(mw)));
         if (blockIdx.x == 0 && threadIdx.x == 0) head->max_x = mx, head->max_w = mw;
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) head->done = 0;
     const int64_t rows = q.T + (wp ? q.V : 0), step = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
     for (int64_t r = blockIdx.x * static_cast<int64_t>(kThreads / 32) + (threadIdx.x >> 5); r < rows; r += step) {
         const bool is_w = r >= q.T;
         const int64_t row = is_w ? r - q.T : r;
-        bool on = true;
-        if (!is_w) {
-            const int64_t v = q.targets[row];
-            on = v != q.ignore;
-            if (lane_id() == 0) {
-                const bool bad = on && (v < 0 || v >= q.V);
-                tgt[row] = !on ? kIgnored : bad ? kInvalid : static_cast<int>(v);
-                zt[row] = bad ? __int_as_float(0x7fffffff) : 0.f;  // no such token: its loss is NaN
-            }
-        }
+        const bool on = is_w || q.targets[row] != q.ignore;
         const T* src = static_cast<const T*>(is_w ? q.w : q.x) + row * q.D;
         const float scale = is_w ? scale_w : scale_x;
         const int64_t plane = (is_w ? q.V : q.T) * dp;
@@ -191,17 +179,17 @@ planes_kernel(Source q, int64_t dp, const unsigned* part, int x_blocks, int w_bl
 
 // Largest finite magnitude of the single losses' gradients.
 __global__ void __launch_bounds__(1024)
-grad_max_kernel(const float* __restrict__ g, const int* __restrict__ tgt, int64_t T, Header* head) {
+grad_max_kernel(Problem p) {
     __shared__ unsigned s[32];
     unsigned m = 0;
-    for (int64_t t = threadIdx.x; t < T; t += 1024)
-        if (tgt[t] != kIgnored) m = max(m, finite_bits(g[t]));
+    for (int64_t t = threadIdx.x; t < p.T; t += 1024)
+        if (p.targets[t] != p.ignore) m = max(m, finite_bits(p.g_rows[t]));
     m = __reduce_max_sync(0xffffffffu, m);
     if (lane_id() == 0) s[threadIdx.x >> 5] = m;
     __syncthreads();
     if (threadIdx.x < 32) {
         m = __reduce_max_sync(0xffffffffu, s[threadIdx.x]);
-        if (threadIdx.x == 0) head->max_g = m;
+        if (threadIdx.x == 0) p.head->max_g = m;
     }
 }
 
@@ -228,11 +216,12 @@ finish_kernel(Problem p, int parts, float* __restrict__ rows, float* loss, doubl
     __syncthreads();
     if (threadIdx.y == 0) {
         for (int k = 1; k < blockDim.y; ++k) q = join(q, s[k][threadIdx.x]);
-        const int tg = t < p.T ? p.tgt[t] : kIgnored;
-        const float l = tg == kIgnored ? 0.f : q.x + logf(q.y) - p.zt[t];
+        const int tg = t < p.T ? target_of(p, t) : kIgnored;
+        const float nan = __int_as_float(0x7fffffff);  // of a target that does not exist
+        const float l = tg == kIgnored ? 0.f : tg == kInvalid ? nan : q.x + logf(q.y) - p.zt[t];
         if (t < p.T) {
             p.row_max[t] = q.x;
-            p.row_inv[t] = tg == kInvalid ? __int_as_float(0x7fffffff) : 1.f / q.y;
+            p.row_inv[t] = tg == kInvalid ? nan : 1.f / q.y;
             if (rows) rows[t] = l;
         }
         double a = l;
@@ -269,6 +258,9 @@ finish_kernel(Problem p, int parts, float* __restrict__ rows, float* loss, doubl
 
 // 16-bit weights are read where they lie when their rows start on 16 bytes.
 bool copies_w(const sl_xent_args& a) { return a.dtype == SL_F32 || a.dim % 8 != 0 || off_by(a.weight, 16); }
+// x too, where no gradient is asked for: rows that do not count then need
+// not be zeros, since a row of logits depends on its own row of x alone.
+bool copies_x(const sl_xent_args& a) { return a.train || a.dtype == SL_F32 || a.dim % 8 != 0 || off_by(a.x, 16); }
 
 int check(const sl_xent_args* a, const char* fn) {
     SL_REQUIRE(a != nullptr, fn, "NULL arguments");
@@ -294,19 +286,21 @@ struct Setup {
 Setup setup(const sl_xent_args& a) {
     Setup s;
     const bool copy = copies_w(a);
-    s.l = layout(a.tokens, a.dim, a.vocab, a.dtype, copy);
+    s.l = layout(a.tokens, a.dim, a.vocab, a.dtype, copies_x(a), copy);
     s.prep = static_cast<char*>(a.prep);
     s.scratch = static_cast<char*>(a.scratch);
     s.p = Problem{};
     s.p.head = reinterpret_cast<Header*>(s.prep);
-    s.p.tgt = reinterpret_cast<int*>(s.prep + s.l.tgt);
+    s.p.targets = a.targets;
+    s.p.ignore = a.ignore_index;
     s.p.row_max = reinterpret_cast<float*>(s.prep + s.l.row_max);
     s.p.row_inv = reinterpret_cast<float*>(s.prep + s.l.row_inv);
     s.p.T = a.tokens; s.p.D = a.dim; s.p.V = a.vocab;
     s.p.f32 = a.dtype == SL_F32;
     s.p.bf16 = a.dtype == SL_BF16;
     s.p.mean = a.reduction == SL_XENT_MEAN;
-    s.x = {s.prep + s.l.x, a.tokens, a.dim, s.l.dp, a.tokens * s.l.dp};
+    s.x = copies_x(a) ? Operand{s.prep + s.l.x, a.tokens, a.dim, s.l.dp, a.tokens * s.l.dp}
+                      : Operand{a.x, a.tokens, a.dim, a.dim, 0};
     s.w = copy ? Operand{s.prep + s.l.w, a.vocab, a.dim, s.l.dp, a.vocab * s.l.dp}
                : Operand{a.weight, a.vocab, a.dim, a.dim, 0};
     return s;
@@ -322,21 +316,19 @@ int forward(const sl_xent_args& a, cudaStream_t st) {
     const int64_t T = a.tokens, V = a.vocab;
     s.p.zt = reinterpret_cast<float*>(s.scratch + s.l.zt);
     s.p.part = reinterpret_cast<float2*>(s.scratch + s.l.part);
-    int* tgt = reinterpret_cast<int*>(s.prep + s.l.tgt);
     unsigned* maxima = reinterpret_cast<unsigned*>(s.scratch + s.l.maxima);
-    const bool copy = copies_w(a);
-    const Source src{a.x, a.weight, a.targets, T, V, a.dim, a.ignore_index};
+    const bool cx = copies_x(a), cw = copies_w(a);
+    const Source src{a.x, a.weight, a.targets, cx ? T : 0, V, a.dim, a.ignore_index};
     const int vec = a.dim % 8 == 0 && !off_by(a.x, 16) && !off_by(a.weight, 16);
     const int bx = blocks_for(T), bw = blocks_for(V);
-    void *xp = s.prep + s.l.x, *wp = copy ? s.prep + s.l.w : nullptr;
-    const int blocks = blocks_for(T + (copy ? V : 0));
+    void *xp = s.prep + s.l.x, *wp = cw ? s.prep + s.l.w : nullptr;
+    const int blocks = blocks_for(src.T + (cw ? V : 0));
     if (s.p.f32) {
         absmax_kernel<<<bx + bw, kThreads, 0, st>>>(src, bx, maxima, vec);
-        planes_kernel<float><<<blocks, kThreads, 0, st>>>(src, s.l.dp, maxima, bx, bw, s.p.head, tgt, s.p.zt, xp, wp, vec);
-    } else if (s.p.bf16) {
-        planes_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(src, s.l.dp, nullptr, 0, 0, s.p.head, tgt, s.p.zt, xp, wp, vec);
-    } else {
-        planes_kernel<__half><<<blocks, kThreads, 0, st>>>(src, s.l.dp, nullptr, 0, 0, s.p.head, tgt, s.p.zt, xp, wp, vec);
+        planes_kernel<float><<<blocks, kThreads, 0, st>>>(src, s.l.dp, maxima, bx, bw, s.p.head, xp, wp, vec);
+    } else if (cx || cw) {
+        if (s.p.bf16) planes_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(src, s.l.dp, nullptr, 0, 0, s.p.head, xp, wp, vec);
+        else planes_kernel<__half><<<blocks, kThreads, 0, st>>>(src, s.l.dp, nullptr, 0, 0, s.p.head, xp, wp, vec);
     }
     SL_RETURN_IF_LAUNCH_FAILED("sl_xent_forward");
     if (int rc = gemm_stats(s.p, s.x, s.w, st)) return rc;
@@ -355,7 +347,7 @@ int backward(const sl_xent_args& a, cudaStream_t st) {
     const int64_t T = a.tokens, V = a.vocab;
     if (a.reduction == SL_XENT_NONE) {
         s.p.g_rows = a.grad;
-        grad_max_kernel<<<1, 1024, 0, st>>>(a.grad, s.p.tgt, T, s.p.head);
+        grad_max_kernel<<<1, 1024, 0, st>>>(s.p);
         SL_RETURN_IF_LAUNCH_FAILED("sl_xent_backward");
     } else {
         s.p.grad = a.grad;
@@ -389,7 +381,7 @@ extern "C" int sl_xent_sizes(const sl_xent_args* a, int64_t* prep, int64_t* forw
     const char* fn = "sl_xent_sizes";
     SL_REQUIRE(a && prep && forward && backward, fn, "NULL argument");
     SL_REQUIRE(known_dtype(a->dtype) && a->tokens >= 0 && a->dim >= 1 && a->vocab >= 1, fn, "bad shape or type");
-    const xent::Layout l = xent::layout(std::max<int64_t>(a->tokens, 1), a->dim, a->vocab, a->dtype, xent::copies_w(*a));
+    const xent::Layout l = xent::layout(std::max<int64_t>(a->tokens, 1), a->dim, a->vocab, a->dtype, xent::copies_x(*a), xent::copies_w(*a));
     *prep = l.prep;
     *forward = l.fwd;
     *backward = l.bwd;
@@ -406,7 +398,7 @@ extern "C" int sl_xent_forward(const sl_xent_args* a, void* stream) {
 extern "C" int sl_xent_backward(const sl_xent_args* a, void* stream) {
     if (int rc = xent::check(a, "sl_xent_backward")) return rc;
     if (a->tokens == 0) return SL_OK;
-    SL_REQUIRE(a->grad != nullptr, "sl_xent_backward", "NULL gradient");
+    SL_REQUIRE(a->grad != nullptr && a->train, "sl_xent_backward", "NULL gradient, or a forward call without train");
     SL_REQUIRE(!off_by(a->dx, dtype_bytes(a->dtype)) && !off_by(a->dweight, dtype_bytes(a->dtype)), "sl_xent_backward", "misaligned output");
     if (!a->dx && !a->dweight) return SL_OK;
     return xent::backward(*a, as_stream(stream));

@@ -38,7 +38,8 @@ struct Operand {
 
 struct Problem {
     Header* head;
-    const int* tgt;         // [T]
+    const int64_t* targets; // [T]
+    int64_t ignore;
     float* row_max;         // [T] the softmax's maximum of each row, and
     float* row_inv;         // [T] one over its sum
     float* zt;              // [T] logit of the target
@@ -50,6 +51,12 @@ struct Problem {
     bool f32;               // planes of fp16 pairs, scaled
     bool bf16;
 };
+
+// Target of token t; kIgnored, or kInvalid where there is no such column.
+__device__ __forceinline__ int target_of(const Problem& p, int64_t t) {
+    const int64_t v = p.targets[t];
+    return v == p.ignore ? kIgnored : v < 0 || v >= p.V ? kInvalid : static_cast<int>(v);
+}
 
 // How a product [M, N] with a sum of K is split over the sum, and the floats
 // that its parts leave to be joined (0: not split).

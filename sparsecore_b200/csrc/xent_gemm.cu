@@ -26,7 +26,7 @@ constexpr int kTile = 256;
 constexpr int kSlice = 64;                       // of the sum, in a stage: 128 bytes a row
 constexpr int kBox = 128 * kSlice * 2;           // bytes of one operand's plane in a stage
 constexpr int kRing = 12;                        // boxes in shared memory: 6 stages, or 3 of two planes
-constexpr int kChunk = 2;                        // stages added up in tensor memory for 32-bit operands
+constexpr int kChunk = 4;                        // stages added up in tensor memory for 32-bit operands
 constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // a warpgroup of loads and MMAs, two of results
 // Registers a thread: of 168 x 384 at launch, 40 x 128 stay with the first
@@ -79,13 +79,6 @@ __device__ __forceinline__ void store32(void* dst, const uint32_t (&v)[8]) {
                  : "memory");
 }
 
-__device__ __forceinline__ uint32_t pack2(__half a, __half b) {
-    return static_cast<uint32_t>(__half_as_ushort(a)) | static_cast<uint32_t>(__half_as_ushort(b)) << 16;
-}
-__device__ __forceinline__ uint32_t pack2(__nv_bfloat16 a, __nv_bfloat16 b) {
-    return static_cast<uint32_t>(__bfloat16_as_ushort(a)) | static_cast<uint32_t>(__bfloat16_as_ushort(b)) << 16;
-}
-
 constexpr float kLog2e = 1.4426950408889634f;
 
 // What brings a sum of 32-bit operands' planes back to the logit.
@@ -98,7 +91,7 @@ __device__ __forceinline__ float logit_scale(const Problem& p) {
 __device__ __forceinline__ void epilogue_stats(const Args& a, float (&z)[128], int64_t t, int64_t n0, float u) {
     const int n = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(128), a.N - n0)));
     if (t >= a.M || n == 0) return;
-    const int tg = a.p.tgt[t];
+    const int tg = target_of(a.p, t);
     if (tg >= n0 && tg < n0 + n) {
         const int at = static_cast<int>(tg - n0);
         float q = 0.f;
@@ -115,7 +108,7 @@ __device__ __forceinline__ void epilogue_stats(const Args& a, float (&z)[128], i
     for (int j = 0; j < 128; ++j) m = fmaxf(m, z[j]);
     m *= u;
 #pragma unroll
-    for (int j = 0; j < 128; ++j) s[j & 3] += exp2_fast((z[j] * u - m) * kLog2e);
+    for (int j = 0; j < 128; ++j) s[j & 3] += exp2_fast(fmaf(z[j], u, -m) * kLog2e);
     a.p.part[n0 / kPart * a.M + t] = make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
 }
 
@@ -124,35 +117,41 @@ template <int PL>
 __device__ __forceinline__ void epilogue_grad(const Args& a, float (&z)[128], int64_t t, int64_t n0, float u) {
     const int64_t room = min(static_cast<int64_t>(128), a.g_stride - n0);
     if (t >= a.M || room <= 0) return;
-    const int tg = a.p.tgt[t];
-    const int at = tg >= 0 && tg - a.v0 - n0 >= 0 && tg - a.v0 - n0 < 128 ? static_cast<int>(tg - a.v0 - n0) : -1;
+    const int tg = target_of(a.p, t);
     float one = a.p.bf16 ? 1.f : kGradScale;
     if (a.p.g_rows) {  // single losses' gradients, over the largest
         const float top = __uint_as_float(a.p.head->max_g);
         one = top > 0.f ? one * (a.p.g_rows[t] / top) : 0.f;
     }
+    if (tg == kIgnored) one = 0.f;  // its logits are zeros
     const float m = a.p.row_max[t], c = a.p.row_inv[t] * one;
-    const bool on = tg != kIgnored;
+    const int64_t from = tg - a.v0 - n0;
+    const int at = tg >= 0 && from >= 0 && from < 128 ? static_cast<int>(from) : -1;
     char* dst = static_cast<char*>(a.g) + 2 * (t * a.g_stride + n0);
 #pragma unroll
     for (int j = 0; j < 128; j += 16) {
         if (j >= room) break;
         uint32_t hi[8], lo[8];
+        float v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = exp2_fast(fmaf(z[j + k], u, -m) * kLog2e) * c;
+        if (at >> 4 == j >> 4) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) v[k] -= j + k == at ? one : 0.f;
+        }
 #pragma unroll
         for (int k = 0; k < 16; k += 2) {
-            float v[2];
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                v[q] = exp2_fast((z[j + k + q] * u - m) * kLog2e) * c - (j + k + q == at ? one : 0.f);
-                if (!on) v[q] = 0.f;
-            }
             if (PL == 1 && a.p.bf16) {
-                hi[k / 2] = pack2(__float2bfloat16_rn(v[0]), __float2bfloat16_rn(v[1]));
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[k], v[k + 1]);
+                hi[k / 2] = reinterpret_cast<const uint32_t&>(h);
             } else {
-                const __half h0 = __float2half_rn(v[0]), h1 = __float2half_rn(v[1]);
-                hi[k / 2] = pack2(h0, h1);
-                if (PL == 2)
-                    lo[k / 2] = pack2(__float2half_rn(v[0] - __half2float(h0)), __float2half_rn(v[1] - __half2float(h1)));
+                const __half2 h = __floats2half2_rn(v[k], v[k + 1]);
+                hi[k / 2] = reinterpret_cast<const uint32_t&>(h);
+                if (PL == 2) {
+                    const float2 f = __half22float2(h);
+                    const __half2 l = __floats2half2_rn(v[k] - f.x, v[k + 1] - f.y);
+                    lo[k / 2] = reinterpret_cast<const uint32_t&>(l);
+                }
             }
         }
         store32(dst + 2 * j, hi);
@@ -216,8 +215,9 @@ __device__ __forceinline__ void epilogue_out(const Args& a, float (&z)[128], int
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const float p = z[j + 2 * k] * scale, q = z[j + 2 * k + 1] * scale;
-                    v[k] = a.o.dtype == SL_BF16 ? pack2(__float2bfloat16_rn(p), __float2bfloat16_rn(q))
-                                                : pack2(__float2half_rn(p), __float2half_rn(q));
+                    const __nv_bfloat162 b = __floats2bfloat162_rn(p, q);
+                    const __half2 h = __floats2half2_rn(p, q);
+                    v[k] = a.o.dtype == SL_BF16 ? reinterpret_cast<const uint32_t&>(b) : reinterpret_cast<const uint32_t&>(h);
                 }
                 store32(dst + 2 * j, v);
             }
@@ -239,6 +239,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     Shared& sh = *reinterpret_cast<Shared*>(ring + kRing * kBox);
     const int warp = threadIdx.x >> 5, lane = lane_id();
     const uint32_t rank = cluster_rank();
+    if (MODE == kStats && blockIdx.x == 0 && threadIdx.x == 0) a.p.head->done = 0;  // for the finish
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&sh.full[s], 1);
@@ -390,21 +391,35 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     if (warp == 1) tmem_free_pair(tmem, 512);
 }
 
-// Sum of a split product's slabs, in their order.
+// Sum of a split product's slabs, in their order; W columns a thread.
+template <int W>
 __global__ void __launch_bounds__(256)
 join_kernel(Problem p, Output o, int64_t M, int64_t N, int64_t stride, int64_t slab, int splits, bool f32) {
     const float scale = out_scale(p, o.by_x, f32);
-    const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(256) + threadIdx.x; i < M * N; i += step) {
-        const int64_t m = i / N;
-        const float* q = o.slabs + m * stride + (i - m * N);
-        float v = 0.f;
-        for (int s = 0; s < splits; ++s) v += q[s * slab];
-        if (o.acc) {
-            if (!o.first) v += o.acc[i];
-            if (!o.last) o.acc[i] = v;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 256 * W;
+    const int across = static_cast<int>(N);
+    for (int64_t i = (blockIdx.x * static_cast<int64_t>(256) + threadIdx.x) * W; i < M * N; i += step) {
+        const int64_t m = i / across;
+        const float* q = o.slabs + m * stride + (i - m * across);
+        float v[W] = {}, f[W];
+#pragma unroll 8
+        for (int s = 0; s < splits; ++s) {
+            load_f<float, W>(q + s * slab, f);
+#pragma unroll
+            for (int k = 0; k < W; ++k) v[k] += f[k];
         }
-        if (o.last) store_out(o, i, v * scale);
+        if (o.acc) {
+            if (!o.first) {
+                load_f<float, W>(o.acc + i, f);
+#pragma unroll
+                for (int k = 0; k < W; ++k) v[k] += f[k];
+            }
+            if (!o.last) store_f<float, W>(o.acc + i, v);
+        }
+        if (o.last) {
+#pragma unroll
+            for (int k = 0; k < W; ++k) store_out(o, i + k, v[k] * scale);
+        }
     }
 }
 
@@ -446,8 +461,11 @@ int run(Args& a, const Operand& A, const Operand& B, cudaStream_t s) {
     }
     if (int rc = a.p.f32 ? launch<2, MODE>(A, B, a, s) : launch<1, MODE>(A, B, a, s)) return rc;
     if (a.splits > 1) {
-        const int64_t blocks = std::min<int64_t>((a.M * a.N + 255) / 256, num_sms() * 8);
-        join_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(a.p, a.o, a.M, a.N, static_cast<int64_t>(a.tiles_n) * kTile, a.slab_stride, a.splits, a.p.f32);
+        const int64_t stride = static_cast<int64_t>(a.tiles_n) * kTile;
+        const int w = a.N % 4 == 0 ? 4 : 1;
+        const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((a.M * a.N / w + 255) / 256, num_sms() * 16));
+        if (w == 4) join_kernel<4><<<blocks, 256, 0, s>>>(a.p, a.o, a.M, a.N, stride, a.slab_stride, a.splits, a.p.f32);
+        else join_kernel<1><<<blocks, 256, 0, s>>>(a.p, a.o, a.M, a.N, stride, a.slab_stride, a.splits, a.p.f32);
         SL_RETURN_IF_LAUNCH_FAILED("sl_xent");
     }
     return SL_OK;

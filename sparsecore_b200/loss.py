@@ -19,11 +19,10 @@ __all__ = ["linear_cross_entropy"]
 _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 
-def _args(x, weight, targets, ignore_index, reduction):
-    a = N.SlXentArgs()
-    a.x, a.weight, a.targets = N.ptr(x), N.ptr(weight), N.ptr(targets)
+def _args(x, weight, targets, ignore_index, reduction, train):
+    a = N.SlXentArgs(x.data_ptr(), weight.data_ptr(), targets.data_ptr())
     a.tokens, a.dim, a.vocab = x.shape[0], x.shape[1], weight.shape[0]
-    a.ignore_index, a.dtype, a.reduction = ignore_index, N.DTYPES[x.dtype], reduction
+    a.ignore_index, a.dtype, a.reduction, a.train = ignore_index, N.DTYPES[x.dtype], reduction, train
     return a
 
 
@@ -31,57 +30,63 @@ def _sizes(a):
     out = (ctypes.c_int64 * 3)()
     at = ctypes.addressof(out)
     N.call("sl_xent_sizes", N.byref(a), at, at + 8, at + 16)
-    return list(out)
+    return out
 
 
 def _buffer(n, device):
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
-def _forward(x, weight, targets, ignore_index, reduction):
-    x, weight, targets = x.contiguous(), weight.contiguous(), targets.contiguous()
-    a = _args(x, weight, targets, ignore_index, reduction)
+def _forward(x, weight, targets, ignore_index, reduction, train):
+    dim, dev = weight.shape[1], x.device
+    x, weight, targets = x.reshape(-1, dim).contiguous(), weight.contiguous(), targets.reshape(-1).contiguous()
+    T = x.shape[0]
+    a = _args(x, weight, targets, ignore_index, reduction, train)
     if reduction == 2:
-        loss = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
-        a.loss_rows = N.ptr(loss)
+        loss = torch.empty(T, dtype=torch.float32, device=dev)
+        a.loss_rows = loss.data_ptr()
+    elif T:
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        a.loss = loss.data_ptr()
     else:  # no tokens at all: the mean of nothing is NaN, their sum zero
-        loss = torch.full((), 0.0 if reduction else float("nan"), device=x.device) if x.shape[0] == 0 else \
-            torch.empty((), dtype=torch.float32, device=x.device)
-        a.loss = N.ptr(loss)
+        loss = torch.full((), 0.0 if reduction else float("nan"), device=dev)
     prep = None
-    if x.shape[0]:
+    if T:
         sizes = _sizes(a)
-        prep, scratch = _buffer(sizes[0], x.device), _buffer(sizes[1], x.device)
-        a.prep, a.scratch = N.ptr(prep), N.ptr(scratch)
-        N.call_on(x.device, "sl_xent_forward", N.byref(a))
+        prep, scratch = _buffer(sizes[0], dev), _buffer(sizes[1], dev)
+        a.prep, a.scratch = prep.data_ptr(), scratch.data_ptr()
+        N.call_on(dev, "sl_xent_forward", N.byref(a))
     return loss, (x, weight, targets, prep)
 
 
 class _LinearCrossEntropyFunction(torch.autograd.Function):
-    """Inputs ``(x, weight, targets, ignore_index, reduction)``, x [tokens, dim];
-    returns the loss.  The operands' 16-bit planes, each row's maximum and its
+    """Inputs ``(x, weight, targets, ignore_index, reduction)``; returns the loss.  The operands' 16-bit planes, each row's maximum and its
     sum are kept for the backward pass; the logits are made again there."""
 
     @staticmethod
     def forward(ctx, x, weight, targets, ignore_index, reduction):
-        loss, saved = _forward(x, weight, targets, ignore_index, reduction)
+        loss, saved = _forward(x, weight, targets, ignore_index, reduction, 1)
         ctx.save_for_backward(*saved)
-        ctx.opts = (ignore_index, reduction)
+        ctx.opts = (ignore_index, reduction, x.shape)
         return loss
 
     @staticmethod
     def backward(ctx, grad):
         x, weight, targets, prep = ctx.saved_tensors
+        ignore_index, reduction, shape = ctx.opts
         need = ctx.needs_input_grad
-        dx = torch.empty_like(x) if need[0] else None
+        dx = torch.empty(shape, dtype=x.dtype, device=x.device) if need[0] else None
         dw = torch.empty_like(weight) if need[1] else None
         if prep is None:
             return dx, None if dw is None else dw.zero_(), None, None, None
-        a = _args(x, weight, targets, *ctx.opts)
-        grad = grad.to(torch.float32).contiguous()
+        a = _args(x, weight, targets, ignore_index, reduction, 1)
+        grad = grad.contiguous()
         scratch = _buffer(_sizes(a)[2], x.device)
-        a.prep, a.scratch, a.grad = N.ptr(prep), N.ptr(scratch), N.ptr(grad)
-        a.dx, a.dweight = N.ptr(dx), N.ptr(dw)
+        a.prep, a.scratch, a.grad = prep.data_ptr(), scratch.data_ptr(), grad.data_ptr()
+        if dx is not None:
+            a.dx = dx.data_ptr()
+        if dw is not None:
+            a.dweight = dw.data_ptr()
         N.call_on(x.device, "sl_xent_backward", N.byref(a))
         return dx, dw, None, None, None
 
@@ -126,9 +131,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
         raise ValueError(f"linear_cross_entropy: targets must have shape {tuple(x.shape[:-1])}, got {tuple(targets.shape)}")
     if weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"linear_cross_entropy: weight must not be empty, got {tuple(weight.shape)}")
-    args = (x.reshape(-1, x.shape[-1]), weight, targets.reshape(-1), int(ignore_index), _REDUCTIONS[reduction])
+    code = _REDUCTIONS[reduction]
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        loss = _LinearCrossEntropyFunction.apply(*args)
+        loss = _LinearCrossEntropyFunction.apply(x, weight, targets, int(ignore_index), code)
     else:
-        loss, _ = _forward(*args)
-    return loss.view(targets.shape) if reduction == "none" else loss
+        loss, _ = _forward(x, weight, targets, int(ignore_index), code, 0)
+    return loss.view(targets.shape) if code == 2 and targets.dim() != 1 else loss
