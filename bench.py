@@ -44,6 +44,9 @@ def parse():
                          "set|rigl for two router updates)" % list(SHAPES))
     ap.add_argument("--workload", choices=["cfg5", "cfg4", "cfg2"], default="cfg5",
                     help="training workload (default cfg5, the headline configuration)")
+    ap.add_argument("--fused", action="store_true",
+                    help="cfg4 / cfg5: residual adds fused with the norms, the loss without the logits, "
+                         "AdamW over all tensors in one launch (off by default)")
     ap.add_argument("--graph", action="store_true",
                     help="replay the training step as a CUDA graph (re-captured after "
                          "topology updates); per-kernel timings then come from an eager pass")
@@ -282,7 +285,7 @@ class Workload:
     (on the host) and its loss.  `linear` builds the sparse projections (the
     library's SparseLinear on a GPU, the reference kernels on the CPU)."""
 
-    def __init__(self, name, device, rank, linear=None, batch=None, capturable=False):
+    def __init__(self, name, device, rank, linear=None, batch=None, capturable=False, fused=False):
         import sparsecore_b200 as sl
         from sparsecore_b200 import workloads as W
 
@@ -292,7 +295,7 @@ class Workload:
         if name in ("cfg5", "cfg4"):
             cfg = W.CFG5 if name == "cfg5" else W.CFG4
             self.cfg = cfg
-            self.model = W.MiniGPT(cfg, device=dev, linear=linear)
+            self.model = W.MiniGPT(cfg, device=dev, linear=linear, fused=fused)
             if cfg.router == "SET":
                 self.algo = sl.SET(sparsity=cfg.ffn_sparsity, drop_fraction=cfg.drop_fraction,
                                    update_freq=cfg.update_freq, seed=0)
@@ -302,8 +305,8 @@ class Workload:
                 # with the clones and one without.
                 self.algo = sl.RigL(sparsity=cfg.ffn_sparsity, drop_fraction=cfg.drop_fraction,
                                     update_freq=cfg.update_freq, seed=0, capture="update_step")
-            self.opt = torch.optim.AdamW(self.model.parameters(), lr=cfg.lr,
-                                         capturable=capturable)
+            self.opt = (sl.FusedAdamW(self.model, lr=cfg.lr, capturable=capturable) if fused else
+                        torch.optim.AdamW(self.model.parameters(), lr=cfg.lr, capturable=capturable))
             nb = batch or cfg.batch
             self.batch = (W.synthetic_tokens(cfg, nb, seed=1000 + rank),)
             self.units = nb * cfg.seq_len
@@ -316,7 +319,7 @@ class Workload:
                              f"{cfg.d_ff} at {int(cfg.ffn_sparsity * 100)}% / attention "
                              f"projections at {int(cfg.attn_sparsity * 100)}% sparsity (padded "
                              f"CSR, fp32), AdamW {cfg.lr}, {cfg.router} every {cfg.update_freq} "
-                             f"steps"),
+                             f"steps" + (", fused norms, loss and optimizer" if fused else "")),
                 "global_batch": cfg.batch, "seq_len": cfg.seq_len}
         else:  # cfg2: MLP 784 -> 512 -> 10, SGD 0.1, SET every 100 steps
             make = linear or (lambda fin, fout, s, bias=True: sl.SparseLinear(fin, fout, bias=bias,
@@ -401,7 +404,7 @@ def run_ours(args, rank, world, local_rank):
 
         torch.cuda.set_stream(critical_path_stream(dev))
     ceil = N.measure_ceilings(dev)  # before the workload, on an idle GPU
-    wl = Workload(args.workload, dev, rank, capturable=args.graph)
+    wl = Workload(args.workload, dev, rank, capturable=args.graph, fused=args.fused)
     model, algo, opt = wl.model, wl.algo, wl.opt
     ops.set_async_weight_grad(True)  # the loop below reads .grad after backward()
     # One batched exchange after the backward pass.  (The bucketed exchange

@@ -22,7 +22,9 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .loss import linear_cross_entropy
 from .nn import SparseLinear, sparse_mlp
+from .norm import residual_norm
 
 
 @dataclass(frozen=True)
@@ -103,11 +105,17 @@ class MiniGPT(nn.Module):
     attention projections and FFN.  ``linear(in, out, sparsity)`` builds each
     sparse projection (default: SparseLinear on ``device``); all parameters
     are drawn from torch's CPU generator in construction order and the dense
-    parts are then placed on ``device``."""
+    parts are then placed on ``device``.
 
-    def __init__(self, cfg: GPTConfig, device=None, linear=None):
+    ``fused``: each residual add runs together with the norm that follows it
+    (``residual_norm``), and ``lm_loss`` takes the loss without the logits
+    (``linear_cross_entropy``).  Same parameters and same formulas, rounded in
+    another order."""
+
+    def __init__(self, cfg: GPTConfig, device=None, linear=None, fused: bool = False):
         super().__init__()
         self.cfg = cfg
+        self.fused = fused
         dev = torch.device(device) if device is not None else None
         if linear is None:
             linear = _sparse_linear(device)
@@ -127,12 +135,23 @@ class MiniGPT(nn.Module):
             b.ln2.to(dev)
         self.pos_ids = self.pos_ids.to(dev)
 
-    def forward(self, idx):
+    def hidden(self, idx):
+        """What the head reads: the last norm's output."""
         B, T = idx.shape
         x = self.tok_emb(idx) + self.pos_emb(self.pos_ids[:T])
-        for blk in self.blocks:
-            x = blk(x)
-        return self.head(self.ln_f(x))
+        if not self.fused:
+            for blk in self.blocks:
+                x = blk(x)
+            return self.ln_f(x)
+        norms = [blk.ln1 for blk in self.blocks] + [self.ln_f]
+        h = norms[0](x)
+        for blk, after in zip(self.blocks, norms[1:]):
+            x, h = residual_norm(blk.attn(h), x, blk.ln2.weight, blk.ln2.bias, eps=blk.ln2.eps)
+            x, h = residual_norm(blk.ffn(h), x, after.weight, after.bias, eps=after.eps)
+        return h
+
+    def forward(self, idx):
+        return self.head(self.hidden(idx))
 
 
 def make_mlp(device=None) -> nn.Sequential:  # noqa: D401
@@ -149,6 +168,8 @@ def synthetic_tokens(cfg: GPTConfig, batch: int, seed: int) -> torch.Tensor:
 
 def lm_loss(model: MiniGPT, tokens: torch.Tensor) -> torch.Tensor:
     x, y = tokens[:, :-1], tokens[:, 1:]
+    if getattr(model, "fused", False):
+        return linear_cross_entropy(model.hidden(x), model.head.weight, y)
     logits = model(x)
     return F.cross_entropy(logits.reshape(-1, logits.size(-1)), y.reshape(-1))
 
