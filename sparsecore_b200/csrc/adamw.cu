@@ -90,26 +90,28 @@ __device__ __forceinline__ float sqrt_fast(float v) {
     return r;
 }
 
-// Eight e4m3 values times their scale.
-__device__ __forceinline__ void from_e4m3(uint2 c, float scale, float (&out)[kPer]) {
+// Eight e4m3 values.
+__device__ __forceinline__ void from_e4m3(uint2 c, float (&out)[kPer]) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const uint32_t w = (k < 2 ? c.x : c.y) >> (16 * (k & 1));
         const __half2 h(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xFFFFu), __NV_E4M3));
         const float2 f = __half22float2(h);
-        out[2 * k] = f.x * scale;
-        out[2 * k + 1] = f.y * scale;
+        out[2 * k] = f.x;
+        out[2 * k + 1] = f.y;
     }
 }
 
-// v (already over its scale, up to 448) rounded up or down to an e4m3 value
-// by 16 dither bits.  Adding the bits below the three kept mantissa bits and
-// cutting there rounds away from zero with the probability of the part cut
-// off; values below the smallest normal 2^-6 are moved out into the binade
-// above it, whose spacing 2^-9 is theirs, and back.
-__device__ __forceinline__ float dithered(float v, uint32_t bits16) {
-    const float by = fabsf(v) < 0.015625f ? copysignf(0.015625f, v) : 0.f;
-    return __uint_as_float((__float_as_uint(v + by) + (bits16 << 4)) & 0xFFF00000u) - by;
+// a >= 0 (already over its scale, up to 448) rounded up or down to an e4m3
+// value by 16 dither bits.  Adding the bits below the three kept mantissa bits
+// and cutting there rounds up with the probability of the part cut off; values
+// below the smallest normal 2^-6 are moved up into the binade above it, whose
+// spacing 2^-9 is theirs, and back.  Whether to is a saturated product, not a
+// comparison: the kernel is bound by the integer and logic units.
+__device__ __forceinline__ float dithered(float a, uint32_t bits16) {
+    const float small = __saturatef(fmaf(a, -0x1p100f, 0x1p94f));  // 1 below 2^-6, else 0
+    const uint32_t raw = __float_as_uint(fmaf(small, 0x1p-6f, a)) + bits16 * 16u;
+    return fmaf(small, -0x1p-6f, __uint_as_float(raw & 0xFFF00000u));
 }
 
 __device__ __forceinline__ uint2 to_e4m3(const float (&q)[kPer]) {
@@ -215,18 +217,22 @@ __device__ __forceinline__ void step8(const Item& d, const Hyper& h, int64_t i, 
     load(G, i, left, gv, g);
     const uint2 cm = load8(M, left, mv), cu = load8(U, left, uv);
     const uint32_t on = PLAIN ? 0xFFu : taking_part(d.live, i, left);
-    from_e4m3(cm, d.sm[block], m);
-    from_e4m3(cu, d.su[block], u);
+    from_e4m3(cm, m);
+    from_e4m3(cu, u);
+    // with m = its value x sm: b1 m + (1 - b1) g, and b2 (value x su)^2 + (1 - b2) g^2
+    const float sm = d.sm[block], su = d.su[block], sm1 = sm * (1.f - h.one_b1), su2 = su * su * h.b2;
     float tm = 0.f, tu = 0.f;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-        const float gf = g[k];
-        const float m1 = fmaf(gf - m[k], h.one_b1, m[k]);
-        const float root = sqrt_fast(fmaf(u[k] * u[k], h.b2, gf * gf * h.one_b2));
+        const float m1 = fmaf(m[k], sm1, g[k] * h.one_b1);
+        const float root = sqrt_fast(fmaf(u[k] * u[k], su2, g[k] * g[k] * h.one_b2));
         if (PLAIN || (on >> k & 1)) {
             p[k] = fmaf(-h.step_size, m1 * rcp_fast(fmaf(root, h.inv_root, h.eps)), p[k] * h.decay);
             m[k] = m1;
             u[k] = root;
+        } else {
+            m[k] *= sm;
+            u[k] *= su;
         }
         tm = max_nan(tm, fabsf(m[k]));
         tu = max_nan(tu, u[k]);
@@ -252,8 +258,8 @@ __device__ __forceinline__ void step8(const Item& d, const Hyper& h, int64_t i, 
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
         const uint32_t bits = mix32(first + k * 0x9E3779B1u);
-        const float floor = u[k] > 0.f ? 0.001953125f : 0.f;  // 2^-9, the smallest e4m3 value
-        m[k] = dithered(m[k] * im, bits & 0xFFFFu);
+        const float floor = __saturatef(u[k] * 0x1p126f) * 0x1p-9f;  // of what is not zero the smallest e4m3 value
+        m[k] = copysignf(dithered(fabsf(m[k]) * im, bits & 0xFFFFu), m[k]);
         u[k] = fmaxf(dithered(u[k] * iu, bits >> 16), floor);
     }
     if (bad) {
@@ -272,7 +278,7 @@ __device__ __forceinline__ void step8(const Item& d, const Hyper& h, int64_t i, 
 }
 
 template <typename T, bool EIGHT, int MAX>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
 adamw_multi_kernel(const __grid_constant__ Table<MAX> t, Hyper h, const Hyper* dev) {
     if (dev) h = *dev;
     int at = 0;
