@@ -108,10 +108,14 @@ __device__ __forceinline__ void from_e4m3(uint2 c, float (&out)[kPer]) {
 // below the smallest normal 2^-6 are moved up into the binade above it, whose
 // spacing 2^-9 is theirs, and back.  Whether to is a saturated product, not a
 // comparison: the kernel is bound by the integer and logic units.
-__device__ __forceinline__ float dithered(float a, uint32_t bits16) {
-    const float small = __saturatef(fmaf(a, -0x1p100f, 0x1p94f));  // 1 below 2^-6, else 0
-    const uint32_t raw = __float_as_uint(fmaf(small, 0x1p-6f, a)) + bits16 * 16u;
-    return fmaf(small, -0x1p-6f, __uint_as_float(raw & 0xFFF00000u));
+__device__ __forceinline__ void dithered(float (&a)[kPer], const uint32_t (&bits16)[kPer]) {
+    float small[kPer];  // 1 below 2^-6, else 0
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) small[k] = __saturatef(fmaf(a[k], -0x1p100f, 0x1p94f));
+    vfma(a, small, 0x1p-6f, a);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) a[k] = __uint_as_float((__float_as_uint(a[k]) + bits16[k] * 16u) & 0xFFF00000u);
+    vfma(a, small, -0x1p-6f, a);
 }
 
 __device__ __forceinline__ uint2 to_e4m3(const float (&q)[kPer]) {
@@ -221,19 +225,40 @@ __device__ __forceinline__ void step8(const Item& d, const Hyper& h, int64_t i, 
     from_e4m3(cu, u);
     // with m = its value x sm: b1 m + (1 - b1) g, and b2 (value x su)^2 + (1 - b2) g^2
     const float sm = d.sm[block], su = d.su[block], sm1 = sm * (1.f - h.one_b1), su2 = su * su * h.b2;
+    float m1[kPer], root[kPer], q[kPer];
+    vmul(m1, g, h.one_b1);
+    vfma(m1, m, sm1, m1);
+    vmul(g, g, g);
+    vmul(g, g, h.one_b2);
+    vmul(root, u, u);
+    vfma(root, root, su2, g);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) root[k] = sqrt_fast(root[k]);
+    vfma(q, root, h.inv_root, h.eps);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) q[k] = rcp_fast(q[k]);
+    vmul(q, q, m1);
+    if constexpr (PLAIN) {
+        vmul(p, p, h.decay);
+        vfma(p, q, -h.step_size, p);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) m[k] = m1[k], u[k] = root[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            if (on >> k & 1) {
+                p[k] = fmaf(-h.step_size, q[k], p[k] * h.decay);
+                m[k] = m1[k];
+                u[k] = root[k];
+            } else {
+                m[k] *= sm;
+                u[k] *= su;
+            }
+        }
+    }
     float tm = 0.f, tu = 0.f;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-        const float m1 = fmaf(m[k], sm1, g[k] * h.one_b1);
-        const float root = sqrt_fast(fmaf(u[k] * u[k], su2, g[k] * g[k] * h.one_b2));
-        if (PLAIN || (on >> k & 1)) {
-            p[k] = fmaf(-h.step_size, m1 * rcp_fast(fmaf(root, h.inv_root, h.eps)), p[k] * h.decay);
-            m[k] = m1;
-            u[k] = root;
-        } else {
-            m[k] *= sm;
-            u[k] *= su;
-        }
         tm = max_nan(tm, fabsf(m[k]));
         tu = max_nan(tu, u[k]);
     }
@@ -255,12 +280,28 @@ __device__ __forceinline__ void step8(const Item& d, const Hyper& h, int64_t i, 
     const float fm = fmaxf(__uint_as_float(bm), 0x1p-100f), fu = fmaxf(__uint_as_float(bu), 0x1p-100f);
     const float im = 448.f / fm, iu = 448.f / fu;
     const uint32_t key = mix32(h.key + 0x85EBCA77u * d.number), first = static_cast<uint32_t>(i) * 0x9E3779B1u + key;
+    uint32_t lo[kPer], hi[kPer];
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
         const uint32_t bits = mix32(first + k * 0x9E3779B1u);
-        const float floor = __saturatef(u[k] * 0x1p126f) * 0x1p-9f;  // of what is not zero the smallest e4m3 value
-        m[k] = copysignf(dithered(fabsf(m[k]) * im, bits & 0xFFFFu), m[k]);
-        u[k] = fmaxf(dithered(u[k] * iu, bits >> 16), floor);
+        lo[k] = bits & 0xFFFFu;
+        hi[k] = bits >> 16;
+    }
+    float am[kPer], floor[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        am[k] = fabsf(m[k]);
+        floor[k] = __saturatef(u[k] * 0x1p126f);  // of what is not zero the smallest e4m3 value
+    }
+    vmul(am, am, im);
+    vmul(u, u, iu);
+    vmul(floor, floor, 0x1p-9f);
+    dithered(am, lo);
+    dithered(u, hi);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        m[k] = copysignf(am[k], m[k]);
+        u[k] = fmaxf(u[k], floor[k]);
     }
     if (bad) {
 #pragma unroll

@@ -113,35 +113,27 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, int warps, float2* 
 template <int VE, int NV>
 __device__ __forceinline__ void row_stats(const float (&v)[NV][VE], int col, int step, int cols, int layer, float inv_d,
                                           float eps, int warps, float2* ws, int& flip, float& rstd, float& mean) {
-    float a = 0.f;
+    Sum a;
     mean = 0.f;
     if (layer) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            if (col + j * step >= cols) continue;
-#pragma unroll
-            for (int k = 0; k < VE; ++k) a += v[j][k];
-        }
-        mean = row_sum(a, warps, ws, flip) * inv_d;
-        a = 0.f;
+        for (int j = 0; j < NV; ++j)
+            if (col + j * step < cols) a.add(v[j]);
+        mean = row_sum(a.total(), warps, ws, flip) * inv_d;
+        a = Sum();
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             if (col + j * step >= cols) continue;
-#pragma unroll
-            for (int k = 0; k < VE; ++k) {
-                const float c = v[j][k] - mean;
-                a = fmaf(c, c, a);
-            }
+            float c[VE];
+            vadd(c, v[j], -mean);
+            a.template fma<VE>(c, c);
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            if (col + j * step >= cols) continue;
-#pragma unroll
-            for (int k = 0; k < VE; ++k) a = fmaf(v[j][k], v[j][k], a);
-        }
+        for (int j = 0; j < NV; ++j)
+            if (col + j * step < cols) a.template fma<VE>(v[j], v[j]);
     }
-    rstd = 1.f / sqrtf(fmaf(row_sum(a, warps, ws, flip), inv_d, eps));
+    rstd = 1.f / sqrtf(fmaf(row_sum(a.total(), warps, ws, flip), inv_d, eps));
 }
 
 // First element of the gate of row t (32-bit division: rows fit an int).
@@ -183,23 +175,23 @@ norm_fwd_kernel(Args<TY, TR> a) {
         yr.get(j, y);
         if (POST) {
             load_v<TY, VE>(a.pw, a.vec_f32, c, q);
-#pragma unroll
-            for (int k = 0; k < VE; ++k) y[k] = (y[k] - st.w) * st.z * q[k];
+            vadd(y, y, -st.w);
+            vmul(y, y, st.z);
             if (a.pb) {
-                load_v<TY, VE>(a.pb, a.vec_f32, c, q);
-#pragma unroll
-                for (int k = 0; k < VE; ++k) y[k] += q[k];
+                float b[VE];
+                load_v<TY, VE>(a.pb, a.vec_f32, c, b);
+                vfma(y, y, q, b);
+            } else {
+                vmul(y, y, q);
             }
         }
         if (a.gate) {
             load_v<TY, VE>(a.gate, a.gate_f32, gate_row + c, q);
-#pragma unroll
-            for (int k = 0; k < VE; ++k) y[k] *= q[k];
+            vmul(y, y, q);
         }
         // the stream is held in its own type, and the norm reads what it holds
         rr.get(j, q);
-#pragma unroll
-        for (int k = 0; k < VE; ++k) y[k] = fmaf(scale, y[k], q[k]);
+        vfma(y, y, scale, q);
         rr.v[j] = pack<TR, VE>(y);
         rr.get(j, r[j]);
         *reinterpret_cast<Pack<TR, VE>*>(a.out + t * a.D + c) = rr.v[j];
@@ -212,12 +204,14 @@ norm_fwd_kernel(Args<TY, TR> a) {
         if (c >= cols) continue;
         float w[VE], o[VE];
         load_v<TY, VE>(a.w, a.vec_f32, c, w);
-#pragma unroll
-        for (int k = 0; k < VE; ++k) o[k] = (r[j][k] - st.y) * st.x * w[k];
+        vadd(o, r[j], -st.y);
+        vmul(o, o, st.x);
         if (a.b) {
-            load_v<TY, VE>(a.b, a.vec_f32, c, w);
-#pragma unroll
-            for (int k = 0; k < VE; ++k) o[k] += w[k];
+            float b[VE];
+            load_v<TY, VE>(a.b, a.vec_f32, c, b);
+            vfma(o, o, w, b);
+        } else {
+            vmul(o, o, w);
         }
         store_f<TY, VE>(a.h + t * a.D + c, o);
     }
@@ -263,7 +257,7 @@ norm_bwd_kernel(Args<TY, TR> a) {
         nr.load(a.dh + row, col, step, cols);
         dr.load(a.dout + row, col, step, cols);
         const float4 st = a.stats[t];
-        float c1 = 0.f, c2 = 0.f;
+        Sum s1, s2;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = col + j * step;
@@ -272,16 +266,14 @@ norm_bwd_kernel(Args<TY, TR> a) {
             load_v<TY, VE>(a.w, a.vec_f32, c, w);
             xr.get(j, x);
             nr.get(j, d);
-#pragma unroll
-            for (int k = 0; k < VE; ++k) {
-                x[k] = fmaf(x[k], st.x, st.y);
-                aw[j][k] = fmaf(d[k], x[k], aw[j][k]);
-                ab[j][k] += d[k];
-                const float dn = d[k] * w[k];
-                c1 += dn;
-                c2 = fmaf(dn, x[k], c2);
-            }
+            vfma(x, x, st.x, st.y);
+            vfma(aw[j], d, x, aw[j]);
+            vadd(ab[j], ab[j], d);
+            vmul(d, d, w);
+            s1.add(d);
+            s2.template fma<VE>(d, x);
         }
+        float c1 = s1.total(), c2 = s2.total();
         row_sum2(c1, c2, warps, ws, flip);
         c1 = a.layer ? c1 * inv_d : 0.f;
         c2 *= inv_d;
@@ -294,12 +286,13 @@ norm_bwd_kernel(Args<TY, TR> a) {
             xr.get(j, x);
             nr.get(j, g);
             dr.get(j, d);
-#pragma unroll
-            for (int k = 0; k < VE; ++k) d[k] = fmaf(st.x, fmaf(g[k], w[k], -fmaf(fmaf(x[k], st.x, st.y), c2, c1)), d[k]);
+            vfma(x, x, st.x, st.y);
+            vfma(x, x, -c2, -c1);
+            vfma(g, g, w, x);
+            vfma(d, g, st.x, d);
             store_f<TR, VE>(a.dr + row + c, d);
             if (a.need_dy) {
-#pragma unroll
-                for (int k = 0; k < VE; ++k) d[k] *= scale;
+                vmul(d, d, scale);
                 store_f<TY, VE>(a.dy + row + c, d);
             }
         }
@@ -533,7 +526,7 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
             vec_keep(3, gate_row);
         }
         const char* const held = mine + stage * stage_bytes;
-        float s[4 * Q] = {};
+        Sum p[4 * Q];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             if (col + j * step >= cols) continue;
@@ -541,38 +534,35 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
             get(TR{}, kX, a.out, t, held, j, x);
             get(TY{}, kDn, a.dh, t, held, j, g);
             vector(0, 0, j, w);
-#pragma unroll
-            for (int k = 0; k < VE; ++k) {
-                x[k] = fmaf(x[k], st.x, st.y);
-                g[k] *= w[k];
-                s[0] = fmaf(g[k], x[k], s[0]);
-                if (L) s[1] += g[k];
-            }
+            vfma(x, x, st.x, st.y);
+            vmul(g, g, w);
+            p[0].template fma<VE>(g, x);
+            if (L) p[1].add(g);
             if (sums_dy) {
                 float q[VE], y[VE], d[VE];
                 vector(1, 0, j, q);
                 if (a.gate) {
                     gate(t, gate_row, held, j, d);
-#pragma unroll
-                    for (int k = 0; k < VE; ++k) q[k] *= d[k];
+                    vmul(q, q, d);
                 }
                 get(TR{}, kD, a.dout, t, held, j, d);
                 get(TY{}, kY, a.y, t, held, j, y);
-#pragma unroll
-                for (int k = 0; k < VE; ++k) {
-                    const float yq = fmaf(y[k], st.z, st.w) * q[k];
-                    d[k] = fmaf(st.x, g[k], d[k]);
-                    s[2] = fmaf(yq, d[k], s[2]);
-                    s[3] = fmaf(yq, x[k], s[3]);
-                    if constexpr (Q == 2) {
-                        s[4] += yq;
-                        s[5] = fmaf(q[k], d[k], s[5]);
-                        s[6] = fmaf(q[k], x[k], s[6]);
-                        s[7] += q[k];
-                    }
+                vfma(y, y, st.z, st.w);
+                vmul(y, y, q);
+                vfma(d, g, st.x, d);
+                p[2].template fma<VE>(y, d);
+                p[3].template fma<VE>(y, x);
+                if constexpr (Q == 2) {
+                    p[4].add(y);
+                    p[5].template fma<VE>(q, d);
+                    p[6].template fma<VE>(q, x);
+                    p[7].add(q);
                 }
             }
         }
+        float s[4 * Q];
+#pragma unroll
+        for (int k = 0; k < 4 * Q; ++k) s[k] = p[k].total();
         row_sums<Q>(s, warps, ws, flip);
         const float c2 = s[0] * inv_d, c1 = L && a.layer ? s[1] * inv_d : 0.f;
         float e1 = 0.f, e2 = 0.f;
@@ -594,25 +584,24 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
             get(TY{}, kDn, a.dh, t, held, j, g);
             get(TR{}, kD, a.dout, t, held, j, d);
             vector(0, 0, j, w);
-#pragma unroll
-            for (int k = 0; k < VE; ++k) {
-                x[k] = fmaf(x[k], st.x, st.y);
-                aw[j][k] = fmaf(g[k], x[k], aw[j][k]);
-                if (L) ab[j][k] += g[k];
-                const float v = fmaf(g[k], w[k], -c2 * x[k]);
-                d[k] = fmaf(st.x, L ? v - c1 : v, d[k]);
-            }
+            vfma(x, x, st.x, st.y);
+            vfma(aw[j], g, x, aw[j]);
+            if (L) vadd(ab[j], ab[j], g);
+            if (L) vfma(x, x, -c2, -c1);
+            else vmul(x, x, -c2);
+            vfma(g, g, w, x);
+            vfma(d, g, st.x, d);
             store_f<TR, VE>(a.dr + at, d);
             get(TY{}, kY, a.y, t, held, j, y);
             float u[VE], pw[VE];
             if (POST) {
                 vector(1, 0, j, pw);
-#pragma unroll
-                for (int k = 0; k < VE; ++k) y[k] = fmaf(y[k], st.z, st.w), u[k] = y[k] * pw[k];
+                vfma(y, y, st.z, st.w);
                 if (L && a.pb) {
                     vector(2, 0, j, x);
-#pragma unroll
-                    for (int k = 0; k < VE; ++k) u[k] += x[k];
+                    vfma(u, y, pw, x);
+                } else {
+                    vmul(u, y, pw);
                 }
             } else {
 #pragma unroll
@@ -623,27 +612,25 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
 #pragma unroll
                 for (int k = 0; k < VE; ++k) as = fmaf(d[k], a.gate ? x[k] * u[k] : u[k], as);
             }
-#pragma unroll
-            for (int k = 0; k < VE; ++k) d[k] *= scale;
+            vmul(d, d, scale);
             if (each) {
-#pragma unroll
-                for (int k = 0; k < VE; ++k) u[k] *= d[k], d[k] *= x[k];
+                vmul(u, u, d);
+                vmul(d, d, x);
                 if (a.need_gate) {
                     if (a.gate_f32) store_f<float, VE>(static_cast<float*>(a.dgate) + at, u);
                     else store_f<TY, VE>(static_cast<TY*>(a.dgate) + at, u);
                 }
             } else if (a.gate) {
-#pragma unroll
-                for (int k = 0; k < VE; ++k) ag[j][k] = fmaf(d[k], u[k], ag[j][k]), d[k] *= x[k];
+                vfma(ag[j], d, u, ag[j]);
+                vmul(d, d, x);
             }
             if (POST) {
-#pragma unroll
-                for (int k = 0; k < VE; ++k) {
-                    apw[j][k] = fmaf(d[k], y[k], apw[j][k]);
-                    if (L) apb[j][k] += d[k];
-                    const float v = fmaf(d[k], pw[k], -e2 * y[k]);
-                    d[k] = st.z * (L ? v - e1 : v);
-                }
+                vfma(apw[j], d, y, apw[j]);
+                if (L) vadd(apb[j], apb[j], d);
+                if (L) vfma(y, y, -e2, -e1);
+                else vmul(y, y, -e2);
+                vfma(d, d, pw, y);
+                vmul(d, d, st.z);
             }
             if (a.need_dy) store_f<TY, VE>(a.dy + at, d);
             if (a.gate_direct && (t + 1 == t1 || t + 1 == run_end)) {  // a run of rows ends

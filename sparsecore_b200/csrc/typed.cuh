@@ -78,6 +78,100 @@ __device__ __forceinline__ void store_f(T* dst, const float (&in)[N]) {
     *reinterpret_cast<Pack<T, N>*>(dst) = pack<T, N>(in);
 }
 
+// Arithmetic on arrays, two 32-bit numbers an instruction (f32x2, sm_100):
+// kernels with little memory traffic an element are bound by the number of
+// their instructions.  Odd counts go one by one.  An operand is an array, or
+// one number for all.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void f2_split(F2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+template <int N> __device__ __forceinline__ float at1(const float (&v)[N], int k) { return v[k]; }
+__device__ __forceinline__ float at1(float v, int) { return v; }
+template <int N> __device__ __forceinline__ F2 at2(const float (&v)[N], int k) { return f2(v[k], v[k + 1]); }
+__device__ __forceinline__ F2 at2(float v, int) { return f2(v, v); }
+
+// d = a b + c
+template <int N, typename A, typename B, typename C>
+__device__ __forceinline__ void vfma(float (&d)[N], const A& a, const B& b, const C& c) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < N; k += 2) f2_split(fma2(at2(a, k), at2(b, k), at2(c, k)), d[k], d[k + 1]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) d[k] = fmaf(at1(a, k), at1(b, k), at1(c, k));
+    }
+}
+// d = a b
+template <int N, typename A, typename B>
+__device__ __forceinline__ void vmul(float (&d)[N], const A& a, const B& b) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < N; k += 2) f2_split(mul2(at2(a, k), at2(b, k)), d[k], d[k + 1]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) d[k] = at1(a, k) * at1(b, k);
+    }
+}
+// d = a + b
+template <int N, typename A, typename B>
+__device__ __forceinline__ void vadd(float (&d)[N], const A& a, const B& b) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < N; k += 2) f2_split(add2(at2(a, k), at2(b, k)), d[k], d[k + 1]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) d[k] = at1(a, k) + at1(b, k);
+    }
+}
+// A sum that takes its terms in pairs.
+struct Sum {
+    F2 v = 0;
+    template <int N, typename A, typename B>
+    __device__ __forceinline__ void fma(const A& a, const B& b) {
+        if constexpr (N % 2 == 0) {
+#pragma unroll
+            for (int k = 0; k < N; k += 2) v = fma2(at2(a, k), at2(b, k), v);
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; ++k) v = fma2(f2(at1(a, k), 0.f), f2(at1(b, k), 0.f), v);
+        }
+    }
+    template <int N>
+    __device__ __forceinline__ void add(const float (&a)[N]) {
+        if constexpr (N % 2 == 0) {
+#pragma unroll
+            for (int k = 0; k < N; k += 2) v = add2(at2(a, k), v);
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; ++k) v = add2(f2(a[k], 0.f), v);
+        }
+    }
+    __device__ __forceinline__ float total() const {
+        float a, b;
+        f2_split(v, a, b);
+        return a + b;
+    }
+};
+
 inline int64_t dtype_bytes(int dtype) { return dtype == SL_F32 ? 4 : 2; }
 inline bool known_dtype(int dtype) { return dtype == SL_F32 || dtype == SL_BF16 || dtype == SL_F16; }
 inline bool off_by(const void* q, int64_t a) { return (reinterpret_cast<uintptr_t>(q) & (a - 1)) != 0; }
