@@ -143,77 +143,87 @@ __device__ __forceinline__ int64_t gate_offset(const A& a, int64_t t) {
 }
 
 // blockDim = (32 * warps a row, rows): one row a warp up to 32 elements a
-// lane, without a barrier; more warps a row beyond.
+// lane, without a barrier; more warps a row beyond.  A CTA takes row after
+// row; as many CTAs as an SM holds.
 template <typename TY, typename TR, int VE, int NV, bool POST>
-__global__ void __launch_bounds__(kMaxThreads)
+__global__ void __launch_bounds__(kMaxThreads, VE * NV <= 16 ? 2 : 1)
 norm_fwd_kernel(Args<TY, TR> a) {
     __shared__ float2 ws[64];
     int flip = 0;
     const int warps = blockDim.x >> 5, cols = static_cast<int>(a.D);
     const int col = threadIdx.x * VE, step = blockDim.x * VE;
-    const int64_t t = blockIdx.x * static_cast<int64_t>(blockDim.y) + threadIdx.y;
-    if (t >= a.T) return;  // with several rows a CTA there is no barrier
     const float inv_d = 1.f / static_cast<float>(cols);
     const float scale = a.scale_dev ? *a.scale_dev : a.scale;
     Row<TY, VE, NV> yr;
     Row<TR, VE, NV> rr;
-    yr.load(a.y + t * a.D, col, step, cols);
-    rr.load(a.r + t * a.D, col, step, cols);
-    float4 st = make_float4(0.f, 0.f, 1.f, 0.f);
-    float r[NV][VE];
-    if (POST) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) yr.get(j, r[j]);
-        row_stats<VE, NV>(r, col, step, cols, a.layer, inv_d, a.post_eps, warps, ws, flip, st.z, st.w);
+    int64_t t = blockIdx.x * static_cast<int64_t>(blockDim.y) + threadIdx.y;
+    if (t < a.T) {
+        yr.load(a.y + t * a.D, col, step, cols);
+        rr.load(a.r + t * a.D, col, step, cols);
     }
-    const int64_t gate_row = a.gate ? gate_offset(a, t) : 0;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int c = col + j * step;
-        if (c >= cols) continue;
-        float y[VE], q[VE];
-        yr.get(j, y);
+    for (; t < a.T; t += static_cast<int64_t>(gridDim.x) * blockDim.y) {
+        float4 st = make_float4(0.f, 0.f, 1.f, 0.f);
+        float r[NV][VE];
         if (POST) {
-            load_v<TY, VE>(a.pw, a.vec_f32, c, q);
-            vadd(y, y, -st.w);
-            vmul(y, y, st.z);
-            if (a.pb) {
-                float b[VE];
-                load_v<TY, VE>(a.pb, a.vec_f32, c, b);
-                vfma(y, y, q, b);
-            } else {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) yr.get(j, r[j]);
+            row_stats<VE, NV>(r, col, step, cols, a.layer, inv_d, a.post_eps, warps, ws, flip, st.z, st.w);
+        }
+        const int64_t gate_row = a.gate ? gate_offset(a, t) : 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = col + j * step;
+            if (c >= cols) continue;
+            float y[VE], q[VE];
+            yr.get(j, y);
+            if (POST) {
+                load_v<TY, VE>(a.pw, a.vec_f32, c, q);
+                vadd(y, y, -st.w);
+                vmul(y, y, st.z);
+                if (a.pb) {
+                    float b[VE];
+                    load_v<TY, VE>(a.pb, a.vec_f32, c, b);
+                    vfma(y, y, q, b);
+                } else {
+                    vmul(y, y, q);
+                }
+            }
+            if (a.gate) {
+                load_v<TY, VE>(a.gate, a.gate_f32, gate_row + c, q);
                 vmul(y, y, q);
             }
+            // the stream is held in its own type, and the norm reads what it holds
+            rr.get(j, q);
+            vfma(y, y, scale, q);
+            rr.v[j] = pack<TR, VE>(y);
+            rr.get(j, r[j]);
+            *reinterpret_cast<Pack<TR, VE>*>(a.out + t * a.D + c) = rr.v[j];
         }
-        if (a.gate) {
-            load_v<TY, VE>(a.gate, a.gate_f32, gate_row + c, q);
-            vmul(y, y, q);
+        // the next row's operands are on their way over the rest of this one
+        const int64_t next = t + static_cast<int64_t>(gridDim.x) * blockDim.y;
+        if (next < a.T) {
+            yr.load(a.y + next * a.D, col, step, cols);
+            rr.load(a.r + next * a.D, col, step, cols);
         }
-        // the stream is held in its own type, and the norm reads what it holds
-        rr.get(j, q);
-        vfma(y, y, scale, q);
-        rr.v[j] = pack<TR, VE>(y);
-        rr.get(j, r[j]);
-        *reinterpret_cast<Pack<TR, VE>*>(a.out + t * a.D + c) = rr.v[j];
-    }
-    row_stats<VE, NV>(r, col, step, cols, a.layer, inv_d, a.eps, warps, ws, flip, st.x, st.y);
-    if (a.stats && threadIdx.x == 0) a.stats[t] = make_float4(st.x, -st.y * st.x, st.z, -st.w * st.z);
+        row_stats<VE, NV>(r, col, step, cols, a.layer, inv_d, a.eps, warps, ws, flip, st.x, st.y);
+        if (a.stats && threadIdx.x == 0) a.stats[t] = make_float4(st.x, -st.y * st.x, st.z, -st.w * st.z);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int c = col + j * step;
-        if (c >= cols) continue;
-        float w[VE], o[VE];
-        load_v<TY, VE>(a.w, a.vec_f32, c, w);
-        vadd(o, r[j], -st.y);
-        vmul(o, o, st.x);
-        if (a.b) {
-            float b[VE];
-            load_v<TY, VE>(a.b, a.vec_f32, c, b);
-            vfma(o, o, w, b);
-        } else {
-            vmul(o, o, w);
+        for (int j = 0; j < NV; ++j) {
+            const int c = col + j * step;
+            if (c >= cols) continue;
+            float w[VE], o[VE];
+            load_v<TY, VE>(a.w, a.vec_f32, c, w);
+            vadd(o, r[j], -st.y);
+            vmul(o, o, st.x);
+            if (a.b) {
+                float b[VE];
+                load_v<TY, VE>(a.b, a.vec_f32, c, b);
+                vfma(o, o, w, b);
+            } else {
+                vmul(o, o, w);
+            }
+            store_f<TY, VE>(a.h + t * a.D + c, o);
         }
-        store_f<TY, VE>(a.h + t * a.D + c, o);
     }
 }
 
@@ -334,48 +344,46 @@ norm_bwd_kernel(Args<TY, TR> a) {
         }
 }
 
-// Sums of four or eight values, as row_sum2; one barrier.
-template <int Q>
-__device__ __forceinline__ void row_sums(float (&s)[4 * Q], int warps, float4 (*ws)[Q][32], int& flip) {
+// Sums of four or eight values over a row's warps in two steps with a barrier
+// of the caller's between them, as row_sum2.
+__device__ __forceinline__ float fold4(const float4& q) {  // lanes 0, 8, 16 and 24 end with the sums of x, y, z and w
     const int lane = threadIdx.x & 31;
     const bool up = lane & 16, high = lane & 8;
-    auto fold = [&](const float4& q) {  // lanes 0, 8, 16 and 24 end with the sums of x, y, z and w
-        const float a = (up ? q.z : q.x) + __shfl_xor_sync(0xffffffffu, up ? q.x : q.z, 16);
-        const float b = (up ? q.w : q.y) + __shfl_xor_sync(0xffffffffu, up ? q.y : q.w, 16);
-        float v = (high ? b : a) + __shfl_xor_sync(0xffffffffu, high ? a : b, 8);
+    const float a = (up ? q.z : q.x) + __shfl_xor_sync(0xffffffffu, up ? q.x : q.z, 16);
+    const float b = (up ? q.w : q.y) + __shfl_xor_sync(0xffffffffu, up ? q.y : q.w, 16);
+    float v = (high ? b : a) + __shfl_xor_sync(0xffffffffu, high ? a : b, 8);
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        return v;
-    };
-    float v[Q];
+    for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+template <int Q>
+__device__ __forceinline__ void sums_put(const float (&s)[4 * Q], float4 (*w)[32]) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int q = 0; q < Q; ++q) v[q] = fold(make_float4(s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]));
-    if (warps > 1) {
-        float4 (*w)[32] = ws[flip];
-        flip ^= 1;
-        if ((lane & 7) == 0) {
-#pragma unroll
-            for (int q = 0; q < Q; ++q) reinterpret_cast<float*>(&w[q][threadIdx.x >> 5])[lane >> 3] = v[q];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < Q; ++q) v[q] = fold(lane < warps ? w[q][lane] : make_float4(0.f, 0.f, 0.f, 0.f));
+    for (int q = 0; q < Q; ++q) {
+        const float v = fold4(make_float4(s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]));
+        if ((lane & 7) == 0) reinterpret_cast<float*>(&w[q][threadIdx.x >> 5])[lane >> 3] = v;
     }
+}
+template <int Q>
+__device__ __forceinline__ void sums_get(float (&s)[4 * Q], int warps, float4 (*w)[32]) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int q = 0; q < Q; ++q)
+    for (int q = 0; q < Q; ++q) {
+        const float v = fold4(lane < warps ? w[q][lane] : make_float4(0.f, 0.f, 0.f, 0.f));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s[4 * q + k] = __shfl_sync(0xffffffffu, v[q], 8 * k);
+        for (int k = 0; k < 4; ++k) s[4 * q + k] = __shfl_sync(0xffffffffu, v, 8 * k);
+    }
 }
 
 __device__ __forceinline__ void copy16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// All but the last `n` groups of this thread's copies have landed (n = 1 to 3).
+// All but the last `n` groups of this thread's copies have landed (n = 1 or 2).
 __device__ __forceinline__ void copies_wait(int n) {
     if (n == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else if (n == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
-    else asm volatile("cp.async.wait_group 3;" ::: "memory");
+    else asm volatile("cp.async.wait_group 2;" ::: "memory");
 }
 
 // Where a thread finds its part of a row's operands and of the vectors: in
@@ -385,12 +393,14 @@ enum Operand : int { kX, kDn, kD, kY, kG };
 template <typename TY, typename TR, int VE, int NV>
 struct Ring {
     static constexpr int kT = VE * sizeof(TY) / 16, kR = VE * sizeof(TR) / 16;  // granules of a vector
-    static constexpr int kGranules = NV * (3 * kT + 2 * kR), kVec = NV * VE / 4;
+    static constexpr int kVec = NV * VE / 4;
+    // 32-bit rows leave no room for the vectors (read from L1 instead, as no
+    // type has to be changed) nor for a gate a row.
+    static constexpr bool kVectors = sizeof(TY) == 2, kGates = sizeof(TY) == 2;
     __host__ __device__ static constexpr int first(int op) {
         return op == kX ? 0 : op == kDn ? NV * kR : op == kD ? NV * (kR + kT) : op == kY ? NV * (2 * kR + kT) : NV * (2 * kR + 2 * kT);
     }
-    static size_t stage_bytes(int threads) { return static_cast<size_t>(kGranules) * threads * 16; }
-    static size_t vector_bytes(int threads) { return static_cast<size_t>(4 * kVec) * threads * 16; }
+    __host__ __device__ static constexpr int granules(bool gate) { return NV * (2 * kR + (gate ? 3 : 2) * kT); }
 };
 
 // Backward with a norm, a gate or a learned scale after the block (and of
@@ -404,6 +414,8 @@ struct Ring {
 // nothing but the packed operands is needed on its other side.  Those wait in
 // shared memory, copied there rows ahead; the gradients of the vectors (two
 // to five a column) stay in registers, which leave room for one CTA an SM.
+// Between two barriers a warp has the sums of the next row and the results
+// of this one to work on, which hide each other's latencies.
 // L: LayerNorm, or a bias.
 template <typename TY, typename TR, int VE, int NV, bool POST, bool L, bool RING>
 __global__ void __launch_bounds__(kMaxThreads)
@@ -412,12 +424,12 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
     __shared__ float4 ws[2][Q][32];
     extern __shared__ __align__(16) char mem[];
     using R = Ring<TY, TR, VE, NV>;
-    int flip = 0;
+    constexpr bool KEEP = RING && R::kVectors;
     const int warps = blockDim.x >> 5, cols = static_cast<int>(a.D);
     const int col = threadIdx.x * VE, step = blockDim.x * VE;
     const float inv_d = 1.f / static_cast<float>(cols);
     const float scale = a.scale_dev ? *a.scale_dev : a.scale;
-    const bool each = a.gate && a.gate_rows == 1, ring_gate = RING && each && a.gate_f32 == (sizeof(TY) == 4);
+    const bool each = a.gate && a.gate_rows == 1, ring_gate = RING && R::kGates && each && !a.gate_f32;
     float aw[NV][VE] = {}, ag[NV][VE] = {}, apw[POST ? NV : 1][VE] = {};
     float ab[L ? NV : 1][VE] = {}, apb[L && POST ? NV : 1][VE] = {};
     float as = 0.f;
@@ -426,7 +438,7 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
 
     const int lap = blockDim.x * 16;  // bytes from a thread's granule to its next
     char* const mine = mem + threadIdx.x * 16;
-    const int stage_bytes = R::kGranules * lap;
+    const int stage_bytes = R::granules(ring_gate) * lap;
     char* const vectors = mine + stages * stage_bytes;
     auto vector_slot = [&](int which, int j, int q) {
         return reinterpret_cast<float4*>(vectors + (which * R::kVec + j * (VE / 4) + q) * lap);
@@ -470,7 +482,7 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
     const int vec_f32[4] = {a.vec_f32, a.vec_f32, a.vec_f32, a.gate_f32};
     auto vec_read = [&](int which, int64_t from, int j, float (&o)[VE]) { load_v<TY, VE>(vec_src[which], vec_f32[which], from + col + j * step, o); };
     auto vec_keep = [&](int which, int64_t from) {
-        if constexpr (RING) {
+        if constexpr (KEEP) {
             if (vec_src[which] == nullptr) return;
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
@@ -483,7 +495,7 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
         }
     };
     auto vector = [&](int which, int64_t from, int j, float (&o)[VE]) {
-        if constexpr (RING) {
+        if constexpr (KEEP) {
 #pragma unroll
             for (int q = 0; q < VE / 4; ++q) {
                 const float4 f = *vector_slot(which, j, q);
@@ -498,34 +510,9 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
         else if (ring_gate) get(TY{}, kG, static_cast<const TY*>(a.gate), t, held, j, o);
         else load_v<TY, VE>(a.gate, a.gate_f32, t * a.D + col + j * step, o);
     };
-    auto statistics = [&](int64_t t) {  // 1/deviation and -mean/deviation of out's norm, of y's
-        return t < t1 ? a.stats[t] : make_float4(0.f, 0.f, 0.f, 0.f);
-    };
-
-    if constexpr (RING) {
-        for (int k = 0; k < stages - 1; ++k) fetch(t0 + k, k);
-        vec_keep(0, 0);
-        vec_keep(1, 0);
-        vec_keep(2, 0);
-    }
-    float4 next = statistics(t0);
-    int stage = 0;
-    int64_t gate_row = 0, run_end = t0;
+    // The rows' sums; gates shared by a run of rows are those of `from`.
     const bool sums_dy = POST && a.need_dy;
-    for (int64_t t = t0; t < t1; ++t) {
-        const float4 st = next;
-        next = statistics(t + 1);
-        if constexpr (RING) {
-            fetch(t + stages - 1, stage == 0 ? stages - 1 : stage - 1);
-            copies_wait(stages - 1);
-        }
-        if (a.gate && !each && t == run_end) {  // another run's gate; the first time too
-            const int64_t run = static_cast<uint32_t>(t) / static_cast<uint32_t>(a.gate_rows);
-            gate_row = run * a.D;
-            run_end = (run + 1) * a.gate_rows;
-            vec_keep(3, gate_row);
-        }
-        const char* const held = mine + stage * stage_bytes;
+    auto sums = [&](int64_t t, int64_t from, const float4& st, const char* held, float4 (*to)[32]) {
         Sum p[4 * Q];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -542,7 +529,7 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
                 float q[VE], y[VE], d[VE];
                 vector(1, 0, j, q);
                 if (a.gate) {
-                    gate(t, gate_row, held, j, d);
+                    gate(t, from, held, j, d);
                     vmul(q, q, d);
                 }
                 get(TR{}, kD, a.dout, t, held, j, d);
@@ -563,7 +550,37 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
         float s[4 * Q];
 #pragma unroll
         for (int k = 0; k < 4 * Q; ++k) s[k] = p[k].total();
-        row_sums<Q>(s, warps, ws, flip);
+        sums_put<Q>(s, to);
+    };
+    auto statistics = [&](int64_t t) { return a.stats[min(t, t1 - 1)]; };
+    auto run_of = [&](int64_t t) { return a.gate && !each ? static_cast<int64_t>(static_cast<uint32_t>(t) / static_cast<uint32_t>(a.gate_rows)) : 0; };
+
+    if (t0 < t1) {
+    if constexpr (RING)
+        for (int k = 0; k < stages - 1; ++k) fetch(t0 + k, k);
+    for (int k = 0; k < 3; ++k) vec_keep(k, 0);
+    int64_t run = run_of(t0), gate_row = run * a.D, run_end = (run + 1) * a.gate_rows;
+    vec_keep(3, gate_row);
+    if constexpr (RING) copies_wait(stages - 2);
+    float4 st = statistics(t0);
+    int stage = 0, flip = 0;
+    sums(t0, gate_row, st, mine, ws[0]);
+    for (int64_t t = t0; t < t1; ++t) {
+        const char* const held = mine + stage * stage_bytes;
+        const int after = stage + 1 == stages ? 0 : stage + 1;
+        if constexpr (RING) {
+            fetch(t + stages - 1, stage == 0 ? stages - 1 : stage - 1);
+            copies_wait(stages - 2);  // row t + 1 is here
+        }
+        const float4 next = statistics(t + 1);
+        if (warps > 1) __syncthreads();
+        else __syncwarp();
+        float s[4 * Q];
+        sums_get<Q>(s, warps, ws[flip]);
+        flip ^= 1;
+        // A run's last row is finished before the next run's gate takes its place.
+        const bool turn = a.gate && !each && t + 1 == run_end;
+        if (t + 1 < t1 && !turn) sums(t + 1, gate_row, next, mine + after * stage_bytes, ws[flip]);
         const float c2 = s[0] * inv_d, c1 = L && a.layer ? s[1] * inv_d : 0.f;
         float e1 = 0.f, e2 = 0.f;
         if (POST) {
@@ -640,7 +657,15 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
                 for (int k = 0; k < VE; ++k) ag[j][k] = 0.f;
             }
         }
-        if (++stage == stages) stage = 0;
+        if (turn && t + 1 < t1) {
+            gate_row += a.D;
+            run_end += a.gate_rows;
+            vec_keep(3, gate_row);
+            sums(t + 1, gate_row, next, mine + after * stage_bytes, ws[flip]);
+        }
+        st = next;
+        stage = after;
+    }
     }
     const int64_t plane = a.ctas * a.D;
 #pragma unroll
@@ -655,7 +680,10 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
         }
     if (a.need_scale) {
         float z[4 * Q] = {as};
-        row_sums<Q>(z, warps, ws, flip);
+        __syncthreads();
+        sums_put<Q>(z, ws[0]);
+        __syncthreads();
+        sums_get<Q>(z, warps, ws[0]);
         if (threadIdx.x == 0) a.part_s[blockIdx.x] = z[0];
     }
 }
@@ -764,9 +792,8 @@ int forward(const sl_norm_args& n, cudaStream_t s) {
     const Args<TY, TR> a = make_args<TY, TR>(n);
     const Plan p = forward_plan(n.cols, wide_ok<TY, TR>(n), sizeof(TY));
     const dim3 block(32 * p.warps, p.warps == 1 ? 4 : 1);
-    const int64_t ctas = (n.rows + block.y - 1) / block.y;
-    SL_REQUIRE(ctas <= INT_MAX, "sl_norm_forward", "too many rows");
-    const unsigned grid = static_cast<unsigned>(ctas);
+    const int64_t beside = std::max<int64_t>(1, (p.ve * p.nv <= 16 ? 1024 : 512) / (block.x * block.y));
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((n.rows + block.y - 1) / block.y, num_sms() * beside));
     return with_plan<TY>(p, [&](auto ve, auto nv) {
         if (n.post_weight) norm_fwd_kernel<TY, TR, ve, nv, true><<<grid, block, 0, s>>>(a);
         else norm_fwd_kernel<TY, TR, ve, nv, false><<<grid, block, 0, s>>>(a);
@@ -792,13 +819,15 @@ int backward(const sl_norm_args& n, cudaStream_t s) {
             using G = Ring<TY, TR, ve, nv>;
             size_t bytes = 0;
             int stages = 1;
-            if constexpr (ring) {  // two to four rows under way
-                bytes = G::vector_bytes(block.x);
-                stages = static_cast<int>(std::min<size_t>(4, (kFullSmem - bytes) / G::stage_bytes(block.x)));
-                bytes += stages * G::stage_bytes(block.x);
+            if constexpr (ring) {  // this row, the next, and one or two on their way
+                const size_t lap = 16 * block.x, stage = G::granules(G::kGates && n.gate && a.gate_rows == 1 && !a.gate_f32) * lap;
+                bytes = G::kVectors ? 4 * G::kVec * lap : 0;
+                stages = static_cast<int>(std::min<size_t>(4, (kFullSmem - bytes) / stage));
+                if (stages < 3) return fail(SL_ERR_UNSUPPORTED, "sl_norm_backward: rows do not fit");
+                bytes += stages * stage;
             }
             auto go = [&](auto kernel) {
-                if (bytes > 48 * 1024)
+                if (bytes > 40 * 1024)  // with what the kernel has besides, beyond the default
                     if (int e = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)), "sl_norm_backward"))
                         return e;
                 kernel<<<grid, block, bytes, s>>>(a, stages);
