@@ -37,7 +37,7 @@ struct Layout {
 
 int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
-Layout layout(int64_t T, int64_t D, int64_t V, int dtype, bool copy_x, bool copy_w) {
+Layout layout(int64_t T, int64_t D, int64_t V, int dtype, bool copy_x, bool copy_w, bool one_tile) {
     Layout l{};
     const int64_t planes = dtype == SL_F32 ? 2 : 1;
     l.dp = up(D, 64);
@@ -47,12 +47,13 @@ Layout layout(int64_t T, int64_t D, int64_t V, int dtype, bool copy_x, bool copy
     l.row_inv = take(4 * T);
     l.x = take(copy_x ? planes * T * l.dp * 2 : 0);
     l.w = take(copy_w ? planes * V * l.dp * 2 : 0);
+    if (one_tile) l.g = take(planes * T * up(V, 64) * 2);
     l.prep = o;
     o = 0;
     l.zt = take(4 * T);
     l.part = take((V + kPart - 1) / kPart * T * 8);
-    l.sums = take(8 * ((T + 31) / 32));
-    l.counts = take(4 * ((T + 31) / 32));
+    l.sums = take(8 * std::max<int64_t>((T + 31) / 32, kMostCtas));
+    l.counts = take(4 * std::max<int64_t>((T + 31) / 32, kMostCtas));
     l.maxima = take(4 * kMaxBlocks * 2);
     l.fwd = o;
     o = 0;
@@ -61,7 +62,7 @@ Layout layout(int64_t T, int64_t D, int64_t V, int dtype, bool copy_x, bool copy
     const int64_t pieces = std::max<int64_t>(1, (V + most - 1) / most);
     l.piece = up((V + pieces - 1) / pieces, 256);
     l.gp = up(std::min(l.piece, V), 64);
-    l.g = take(planes * T * l.gp * 2);
+    if (!one_tile) l.g = take(planes * T * l.gp * 2);
     l.acc = take(V > l.piece ? 4 * T * D : 0);
     const bool two = dtype == SL_F32;
     const int64_t rest = V - (V - 1) / l.piece * l.piece;  // of the last piece
@@ -69,7 +70,7 @@ Layout layout(int64_t T, int64_t D, int64_t V, int dtype, bool copy_x, bool copy
     for (const int64_t cols : {std::min(l.piece, V), rest})
         floats = std::max({floats, split_sum(T, D, cols, two).floats, split_sum(cols, D, T, two).floats});
     l.slabs = take(4 * floats);
-    l.bwd = o;
+    l.bwd = std::max<int64_t>(o, 256);
     return l;
 }
 
@@ -142,6 +143,7 @@ planes_kernel(Source q, int64_t dp, const unsigned* part, int x_blocks, int w_bl
         scale_w = exp2f(static_cast<float>(plane_exponent(mw)));
         if (blockIdx.x == 0 && threadIdx.x == 0) head->max_x = mx, head->max_w = mw;
     }
+    if (blockIdx.x == 0 && threadIdx.x == 0) head->done = 0;
     const int64_t rows = q.T + (wp ? q.V : 0), step = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
     for (int64_t r = blockIdx.x * static_cast<int64_t>(kThreads / 32) + (threadIdx.x >> 5); r < rows; r += step) {
         const bool is_w = r >= q.T;
@@ -207,46 +209,55 @@ __global__ void __launch_bounds__(1024)
 finish_kernel(Problem p, int parts, float* __restrict__ rows, float* loss, double* sums, int* counts) {
     __shared__ float2 s[32][33];
     __shared__ double total[32];
+    __shared__ int found[32];
     __shared__ bool last;
-    const int64_t t = blockIdx.x * static_cast<int64_t>(32) + threadIdx.x;
+    const int64_t t0 = blockIdx.x * static_cast<int64_t>(32);
     float2 q = make_float2(-INFINITY, 0.f);
-    if (t < p.T)
-        for (int k = threadIdx.y; k < parts; k += blockDim.y) q = join(q, p.part[k * p.T + t]);
+    if (t0 + threadIdx.x < p.T) {
+#pragma unroll 4
+        for (int k = threadIdx.y; k < parts; k += blockDim.y) q = join(q, p.part[k * p.T + t0 + threadIdx.x]);
+    }
     s[threadIdx.y][threadIdx.x] = q;
     __syncthreads();
-    if (threadIdx.y == 0) {
-        for (int k = 1; k < blockDim.y; ++k) q = join(q, s[k][threadIdx.x]);
-        const int tg = t < p.T ? target_of(p, t) : kIgnored;
+    double a = 0.0;
+    int n = 0;
+    for (int r = threadIdx.y; r < 32; r += blockDim.y) {  // a warp a row
+        const int64_t t = t0 + r;
+        if (t >= p.T) break;
+        q = threadIdx.x < blockDim.y ? s[threadIdx.x][r] : make_float2(-INFINITY, 0.f);
+        for (int o = 1; o < blockDim.y; o <<= 1)
+            q = join(q, make_float2(__shfl_xor_sync(0xffffffffu, q.x, o), __shfl_xor_sync(0xffffffffu, q.y, o)));
+        const int tg = target_of(p, t);
         const float nan = __int_as_float(0x7fffffff);  // of a target that does not exist
         const float l = tg == kIgnored ? 0.f : tg == kInvalid ? nan : q.x + logf(q.y) - p.zt[t];
-        if (t < p.T) {
+        if (threadIdx.x == 0) {
             p.row_max[t] = q.x;
             p.row_inv[t] = tg == kInvalid ? nan : 1.f / q.y;
             if (rows) rows[t] = l;
         }
-        double a = l;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-        const int n = __popc(__ballot_sync(0xffffffffu, tg != kIgnored));
-        if (threadIdx.x == 0) {
-            sums[blockIdx.x] = a;
-            counts[blockIdx.x] = n;
-            __threadfence();
-            last = atomicAdd(&p.head->done, 1u) == gridDim.x - 1;
-        }
+        a += l;
+        n += tg != kIgnored;
+    }
+    if (threadIdx.x == 0) total[threadIdx.y] = a, found[threadIdx.y] = n;
+    __syncthreads();
+    if (threadIdx.x == 0 && threadIdx.y == 0) {
+        for (int k = 1; k < blockDim.y; ++k) a += total[k], n += found[k];
+        sums[blockIdx.x] = a;
+        counts[blockIdx.x] = n;
+        __threadfence();
+        last = atomicAdd(&p.head->done, 1u) == gridDim.x - 1;
     }
     __syncthreads();
     if (!last) return;
     __threadfence();
     // The CTA that comes last adds all sums in their order, whoever it is.
     const int tid = threadIdx.y * 32 + threadIdx.x, threads = blockDim.y * 32;
-    double a = 0.0;
-    int n = 0;
+    a = 0.0;
+    n = 0;
     for (int64_t k = tid; k < gridDim.x; k += threads) a += __ldcg(sums + k), n += __ldcg(counts + k);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
     n = __reduce_add_sync(0xffffffffu, n);
-    __shared__ int found[32];
     if (threadIdx.x == 0) total[threadIdx.y] = a, found[threadIdx.y] = n;
     __syncthreads();
     if (tid) return;
@@ -261,6 +272,17 @@ bool copies_w(const sl_xent_args& a) { return a.dtype == SL_F32 || a.dim % 8 != 
 // x too, where no gradient is asked for: rows that do not count then need
 // not be zeros, since a row of logits depends on its own row of x alone.
 bool copies_x(const sl_xent_args& a) { return a.train || a.dtype == SL_F32 || a.dim % 8 != 0 || off_by(a.x, 16); }
+
+// A vocabulary of one tile: the forward pass has a row's logits together and
+// leaves G (of all tokens: at most 256 columns) for the backward pass, which
+// then has no logits to make again.  Single losses' gradients are not known
+// in time.  16384 x 768 x 256 fp32: two launches less and 153 -> 120 us.
+bool one_tile(const sl_xent_args& a) {
+    return a.vocab <= kOneTile && copies_x(a) && !(a.train && a.reduction == SL_XENT_NONE);
+}
+Layout layout(const sl_xent_args& a) {
+    return layout(std::max<int64_t>(a.tokens, 1), a.dim, a.vocab, a.dtype, copies_x(a), copies_w(a), one_tile(a));
+}
 
 int check(const sl_xent_args* a, const char* fn) {
     SL_REQUIRE(a != nullptr, fn, "NULL arguments");
@@ -286,7 +308,7 @@ struct Setup {
 Setup setup(const sl_xent_args& a) {
     Setup s;
     const bool copy = copies_w(a);
-    s.l = layout(a.tokens, a.dim, a.vocab, a.dtype, copies_x(a), copy);
+    s.l = layout(a);
     s.prep = static_cast<char*>(a.prep);
     s.scratch = static_cast<char*>(a.scratch);
     s.p = Problem{};
@@ -331,13 +353,18 @@ int forward(const sl_xent_args& a, cudaStream_t st) {
         else planes_kernel<__half><<<blocks, kThreads, 0, st>>>(src, s.l.dp, nullptr, 0, 0, s.p.head, xp, wp, vec);
     }
     SL_RETURN_IF_LAUNCH_FAILED("sl_xent_forward");
+    double* sums = reinterpret_cast<double*>(s.scratch + s.l.sums);
+    int* counts = reinterpret_cast<int*>(s.scratch + s.l.counts);
+    if (one_tile(a)) {
+        const Operand g{a.train ? s.prep + s.l.g : nullptr, T, V, s.l.gp, T * s.l.gp};
+        return gemm_losses(s.p, s.x, s.w, g, {a.loss, a.loss_rows, sums, counts}, st);
+    }
     if (int rc = gemm_stats(s.p, s.x, s.w, st)) return rc;
     const int parts = static_cast<int>((V + kPart - 1) / kPart);
     int groups = 1;
     while (groups < parts && groups < 32) groups *= 2;
     finish_kernel<<<static_cast<unsigned>((T + 31) / 32), dim3(32, groups), 0, st>>>(
-        s.p, parts, a.loss_rows, a.loss, reinterpret_cast<double*>(s.scratch + s.l.sums),
-        reinterpret_cast<int*>(s.scratch + s.l.counts));
+        s.p, parts, a.loss_rows, a.loss, sums, counts);
     SL_RETURN_IF_LAUNCH_FAILED("sl_xent_forward");
     return SL_OK;
 }
@@ -353,10 +380,12 @@ int backward(const sl_xent_args& a, cudaStream_t st) {
         s.p.grad = a.grad;
     }
     float* slabs = reinterpret_cast<float*>(s.scratch + s.l.slabs);
+    const bool one = one_tile(a);  // the forward call left G
     for (int64_t v0 = 0; v0 < V; v0 += s.l.piece) {
         const int64_t cols = std::min(s.l.piece, V - v0);
-        const Operand g{s.scratch + s.l.g, T, cols, s.l.gp, T * s.l.gp};
-        if (int rc = gemm_grad(s.p, s.x, s.w, v0, cols, g, st)) return rc;
+        const Operand g{(one ? s.prep : s.scratch) + s.l.g, T, cols, s.l.gp, T * s.l.gp};
+        if (!one)
+            if (int rc = gemm_grad(s.p, s.x, s.w, v0, cols, g, st)) return rc;
         if (a.dx) {
             const Output o{a.dx, a.dtype, V > s.l.piece ? reinterpret_cast<float*>(s.scratch + s.l.acc) : nullptr, v0 == 0,
                            v0 + cols == V, slabs, false};
@@ -381,7 +410,7 @@ extern "C" int sl_xent_sizes(const sl_xent_args* a, int64_t* prep, int64_t* forw
     const char* fn = "sl_xent_sizes";
     SL_REQUIRE(a && prep && forward && backward, fn, "NULL argument");
     SL_REQUIRE(known_dtype(a->dtype) && a->tokens >= 0 && a->dim >= 1 && a->vocab >= 1, fn, "bad shape or type");
-    const xent::Layout l = xent::layout(std::max<int64_t>(a->tokens, 1), a->dim, a->vocab, a->dtype, xent::copies_x(*a), xent::copies_w(*a));
+    const xent::Layout l = xent::layout(*a);
     *prep = l.prep;
     *forward = l.fwd;
     *backward = l.bwd;

@@ -68,6 +68,16 @@ SplitSum split_sum(int64_t M, int64_t N, int64_t K, bool two_planes);
 
 // C[m, n] = sum over k of A . B^T, and what becomes of it.
 int gemm_stats(const Problem& p, const Operand& x, const Operand& w, cudaStream_t s);
+// A vocabulary of one tile (up to 256): losses, their sum and the gradient of
+// the logits (if g.base) at once.  loss, rows: written where set; sums,
+// counts: one for each of the launch's CTAs (kMostCtas at most).
+constexpr int kOneTile = 256, kMostCtas = 512;
+struct Losses {
+    float *loss, *rows;
+    double* sums;
+    int* counts;
+};
+int gemm_losses(const Problem& p, const Operand& x, const Operand& w, const Operand& g, const Losses& l, cudaStream_t s);
 // Columns [v0, v0 + cols) of the gradient of the logits, as planes in g.
 int gemm_grad(const Problem& p, const Operand& x, const Operand& w, int64_t v0, int64_t cols, const Operand& g,
               cudaStream_t s);

@@ -33,9 +33,9 @@ constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // a warpgroup of loads and
 // warpgroup and 232 x 256 hold the results (128 sums a thread).
 constexpr int kRegsLow = 40, kRegsHigh = 232;
 static_assert(kRegsLow * 128 + kRegsHigh * 256 <= 168 * kThreads, "registers of the launch");
-constexpr size_t kSmem = kRing * kBox + 1024 + 256;
+constexpr size_t kSmem = kRing * kBox + 1024 + 4096;
 
-enum Mode : int { kStats, kGrad, kOut };
+enum Mode : int { kStats, kGrad, kOut, kLosses };
 
 struct Args {
     Problem p;
@@ -46,6 +46,7 @@ struct Args {
     void* g;
     int64_t g_stride, g_plane;
     Output o;
+    Losses l;
     int64_t slab_stride;
     unsigned* status;
 };
@@ -53,7 +54,21 @@ struct Args {
 struct Shared {
     uint64_t full[kRing / 2], empty[kRing / 2], tmem_full[2], tmem_empty[2];
     uint32_t tmem;
+    // kLosses: what the two threads of a row tell each other, and the CTA's sums
+    float most[2][128], sum[2][128], target[2][128];
+    double loss[kEpilogueWarps];
+    int count[kEpilogueWarps], last;
 };
+static_assert(sizeof(Shared) <= 4096, "room behind the ring");
+
+// Whether all the epilogue's warps got their sums: they wait for one another.
+__device__ __forceinline__ bool epilogue_agrees(bool ok) {
+    int all;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n bar.red.and.pred q, 1, %2, p;\n selp.b32 %0, 1, 0, q;\n}\n" : "=r"(all) : "r"(static_cast<int>(ok)), "n"(32 * kEpilogueWarps) : "memory");
+    return all;
+}
+// A barrier of the epilogue's warps alone.
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory"); }
 
 // Tiles in groups of 8 rows of tiles, down the columns of a group: what runs
 // at one time shares few operand rows.
@@ -112,21 +127,11 @@ __device__ __forceinline__ void epilogue_stats(const Args& a, float (&z)[128], i
     a.p.part[n0 / kPart * a.M + t] = make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
 }
 
-// G = exp(z - m) / s - [target], as planes.
+// 128 columns of G (less the `one` of the target column `at`), as planes:
+// v = e * c, from e in z.
 template <int PL>
-__device__ __forceinline__ void epilogue_grad(const Args& a, float (&z)[128], int64_t t, int64_t n0, float u) {
+__device__ __forceinline__ void store_grad(const Args& a, const float (&z)[128], int64_t t, int64_t n0, float c, int at, float one) {
     const int64_t room = min(static_cast<int64_t>(128), a.g_stride - n0);
-    if (t >= a.M || room <= 0) return;
-    const int tg = target_of(a.p, t);
-    float one = a.p.bf16 ? 1.f : kGradScale;
-    if (a.p.g_rows) {  // single losses' gradients, over the largest
-        const float top = __uint_as_float(a.p.head->max_g);
-        one = top > 0.f ? one * (a.p.g_rows[t] / top) : 0.f;
-    }
-    if (tg == kIgnored) one = 0.f;  // its logits are zeros
-    const float m = a.p.row_max[t], c = a.p.row_inv[t] * one;
-    const int64_t from = tg - a.v0 - n0;
-    const int at = tg >= 0 && from >= 0 && from < 128 ? static_cast<int>(from) : -1;
     char* dst = static_cast<char*>(a.g) + 2 * (t * a.g_stride + n0);
 #pragma unroll
     for (int j = 0; j < 128; j += 16) {
@@ -134,7 +139,7 @@ __device__ __forceinline__ void epilogue_grad(const Args& a, float (&z)[128], in
         uint32_t hi[8], lo[8];
         float v[16];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = exp2_fast(fmaf(z[j + k], u, -m) * kLog2e) * c;
+        for (int k = 0; k < 16; ++k) v[k] = z[j + k] * c;
         if (at >> 4 == j >> 4) {
 #pragma unroll
             for (int k = 0; k < 16; ++k) v[k] -= j + k == at ? one : 0.f;
@@ -156,6 +161,100 @@ __device__ __forceinline__ void epilogue_grad(const Args& a, float (&z)[128], in
         }
         store32(dst + 2 * j, hi);
         if (PL == 2) store32(dst + 2 * (a.g_plane + j), lo);
+    }
+}
+
+// G = exp(z - m) / s - [target].
+template <int PL>
+__device__ __forceinline__ void epilogue_grad(const Args& a, float (&z)[128], int64_t t, int64_t n0, float u) {
+    if (t >= a.M || n0 >= a.g_stride) return;
+    const int tg = target_of(a.p, t);
+    float one = a.p.bf16 ? 1.f : kGradScale;
+    if (a.p.g_rows) {  // single losses' gradients, over the largest
+        const float top = __uint_as_float(a.p.head->max_g);
+        one = top > 0.f ? one * (a.p.g_rows[t] / top) : 0.f;
+    }
+    if (tg == kIgnored) one = 0.f;  // its logits are zeros
+    const float m = a.p.row_max[t];
+    const int64_t from = tg - a.v0 - n0;
+    const int at = tg >= 0 && from >= 0 && from < 128 ? static_cast<int>(from) : -1;
+#pragma unroll
+    for (int j = 0; j < 128; ++j) z[j] = exp2_fast(fmaf(z[j], u, -m) * kLog2e);
+    store_grad<PL>(a, z, t, n0, a.p.row_inv[t] * one, at, one);
+}
+
+// A row of at most 256 columns, in two threads that exchange their maxima and
+// sums: its loss and, where asked for, its G.
+template <int PL>
+__device__ __forceinline__ void epilogue_losses(const Args& a, Shared& sh, float (&z)[128], int64_t t, int row, int half, float u,
+                                                double& loss, int& count) {
+    const int n = max(0, min(128, static_cast<int>(a.N) - half * 128));
+    const int tg = t < a.M ? target_of(a.p, t) : kIgnored;
+    const int at = tg >= half * 128 && tg < half * 128 + 128 ? tg - half * 128 : -1;
+    float m = -INFINITY, zt = 0.f, s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 128; ++j) {
+        z[j] = j < n ? z[j] * u : -INFINITY;
+        m = fmaxf(m, z[j]);
+    }
+    if (at >= 0) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j) zt = j == at ? z[j] : zt;
+    }
+    sh.most[half][row] = m;
+    sh.target[half][row] = zt;
+    epilogue_sync();
+    m = fmaxf(sh.most[0][row], sh.most[1][row]);
+#pragma unroll
+    for (int j = 0; j < 128; ++j) {
+        z[j] = exp2_fast((z[j] - m) * kLog2e);
+        s[j & 3] += z[j];
+    }
+    sh.sum[half][row] = (s[0] + s[1]) + (s[2] + s[3]);
+    epilogue_sync();
+    const float total = sh.sum[0][row] + sh.sum[1][row], nan = __int_as_float(0x7fffffff);
+    if (half == 0 && t < a.M) {
+        const float l = tg == kIgnored ? 0.f : tg == kInvalid ? nan : m + logf(total) - (sh.target[0][row] + sh.target[1][row]);
+        if (a.l.rows) a.l.rows[t] = l;
+        loss += l;
+        count += tg != kIgnored;
+    }
+    epilogue_sync();  // before the next tile's maxima
+    if (a.g == nullptr || t >= a.M || half * 128 >= a.g_stride) return;
+    const float one = tg == kIgnored ? 0.f : a.p.bf16 ? 1.f : kGradScale;
+    store_grad<PL>(a, z, t, half * 128, tg == kInvalid ? nan : one / total, at, one);
+}
+
+// The sum of all losses: every CTA's in its place, and the CTA that comes last
+// adds them up in their order.
+__device__ __forceinline__ void finish_losses(const Args& a, Shared& sh, double loss, int count) {
+    const int warp = (threadIdx.x >> 5) - 4, lane = lane_id();
+    auto sum = [&]() {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+        count = __reduce_add_sync(0xffffffffu, count);
+        if (lane == 0) sh.loss[warp] = loss, sh.count[warp] = count;
+        epilogue_sync();
+        loss = 0.0, count = 0;
+        for (int k = 0; k < kEpilogueWarps; ++k) loss += sh.loss[k], count += sh.count[k];
+        epilogue_sync();
+    };
+    sum();
+    if (warp == 0 && lane == 0) {
+        a.l.sums[blockIdx.x] = loss;
+        a.l.counts[blockIdx.x] = count;
+        __threadfence();
+        sh.last = atomicAdd(&a.p.head->done, 1u) == gridDim.x - 1;
+    }
+    epilogue_sync();
+    if (!sh.last) return;
+    __threadfence();
+    loss = 0.0, count = 0;
+    for (int k = warp * 32 + lane; k < gridDim.x; k += 32 * kEpilogueWarps) loss += __ldcg(a.l.sums + k), count += __ldcg(a.l.counts + k);
+    sum();
+    if (warp == 0 && lane == 0) {
+        a.p.head->count = count;
+        if (a.l.loss) *a.l.loss = static_cast<float>(a.p.mean ? loss / count : loss);
     }
 }
 
@@ -353,6 +452,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         const float u = MODE == kOut ? out_scale(a.p, a.o.by_x, PL == 2) : PL == 2 ? logit_scale(a.p) : 1.f;
         uint32_t done = 0;
         bool ok = true;
+        double loss = 0.0;
+        int count = 0;
         for (int id = pair; id < tiles && ok; id += pairs) {
             int tm, tn, split;
             locate(a, id, tm, tn, split);
@@ -375,13 +476,16 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(leader_addr(&sh.tmem_empty[buf]));
             }
+            if (MODE == kLosses) ok = epilogue_agrees(ok);
             if (!ok) break;
             const int64_t t = static_cast<int64_t>(tm) * kTile + rank * 128 + quarter * 32 + lane;
             const int64_t n0 = static_cast<int64_t>(tn) * kTile + half * 128;
             if (MODE == kStats) epilogue_stats(a, z, t, n0, u);
             else if (MODE == kGrad) epilogue_grad<PL>(a, z, t, n0, u);
+            else if (MODE == kLosses) epilogue_losses<PL>(a, sh, z, t, quarter * 32 + lane, half, u, loss, count);
             else epilogue_out(a, z, t, n0, split, u);
         }
+        if (MODE == kLosses && ok) finish_losses(a, sh, loss, count);
     }
     __syncwarp();
     tc_fence_before();
@@ -436,7 +540,7 @@ int launch(const Operand& A, const Operand& B, const Args& a, cudaStream_t s) {
     };
     if (!map(&ma, A, a.a_mn) || !map(&mb, B, a.b_mn)) return fail(SL_ERR_CUDA, "sl_xent: tensor map could not be made");
     const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits;
-    const int64_t pairs = std::min<int64_t>(tiles, std::max(1, num_sms() / 2));
+    const int64_t pairs = std::min<int64_t>(tiles, std::min(kMostCtas / 2, std::max(1, num_sms() / 2)));
     gemm_kernel<PL, MODE><<<static_cast<unsigned>(2 * pairs), kThreads, kSmem, s>>>(ma, mb, a);
     SL_RETURN_IF_LAUNCH_FAILED("sl_xent");
     return SL_OK;
@@ -507,6 +611,13 @@ int gemm_stats(const Problem& p, const Operand& x, const Operand& w, cudaStream_
     Args a{};
     a.p = p; a.M = p.T; a.N = p.V; a.K = p.D;
     return run<kStats>(a, x, w, s);
+}
+
+int gemm_losses(const Problem& p, const Operand& x, const Operand& w, const Operand& g, const Losses& l, cudaStream_t s) {
+    Args a{};
+    a.p = p; a.M = p.T; a.N = p.V; a.K = p.D; a.l = l;
+    a.g = const_cast<void*>(g.base); a.g_stride = g.stride; a.g_plane = g.plane;
+    return run<kLosses>(a, x, w, s);
 }
 
 int gemm_grad(const Problem& p, const Operand& x, const Operand& w, int64_t v0, int64_t cols, const Operand& g, cudaStream_t s) {
