@@ -207,7 +207,7 @@ __device__ __forceinline__ void step32(const Item& d, const Hyper& h, int64_t i,
 // of p's update), and padding, ends and odd addresses are kept out of the
 // ordinary path.
 template <typename T, bool PLAIN>
-__device__ __forceinline__ void step8(const Item& d, const Hyper& h, int64_t i, int64_t block, int left) {
+__device__ __forceinline__ void step8(const Item& d, const Hyper& h, uint32_t key, int64_t i, int64_t block, int left) {
     T* P = static_cast<T*>(d.p);
     const T* G = static_cast<const T*>(d.g);
     uint8_t* M = static_cast<uint8_t*>(d.m) + i;
@@ -278,8 +278,8 @@ __device__ __forceinline__ void step8(const Item& d, const Hyper& h, int64_t i, 
         bu = __reduce_max_sync(0xffffffffu, bu);
     }
     const float fm = fmaxf(__uint_as_float(bm), 0x1p-100f), fu = fmaxf(__uint_as_float(bu), 0x1p-100f);
-    const float im = 448.f / fm, iu = 448.f / fu;
-    const uint32_t key = mix32(h.key + 0x85EBCA77u * d.number), first = static_cast<uint32_t>(i) * 0x9E3779B1u + key;
+    const float im = 448.f * rcp_fast(fm), iu = 448.f * rcp_fast(fu);
+    const uint32_t first = static_cast<uint32_t>(i) * 0x9E3779B1u + key;
     uint32_t lo[kPer], hi[kPer];
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
@@ -290,10 +290,9 @@ __device__ __forceinline__ void step8(const Item& d, const Hyper& h, int64_t i, 
     float am[kPer], floor[kPer];
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-        am[k] = fabsf(m[k]);
+        am[k] = fabsf(m[k]) * im;
         floor[k] = __saturatef(u[k] * 0x1p126f);  // of what is not zero the smallest e4m3 value
     }
-    vmul(am, am, im);
     vmul(u, u, iu);
     vmul(floor, floor, 0x1p-9f);
     dithered(am, lo);
@@ -324,6 +323,7 @@ adamw_multi_kernel(const __grid_constant__ Table<MAX> t, Hyper h, const Hyper* d
     if (dev) h = *dev;
     int at = 0;
     int64_t end = 0;
+    uint32_t key = 0;
     for (int64_t tile = blockIdx.x; tile < t.tiles; tile += gridDim.x) {
         if (tile >= end) {  // the last tensor whose first tile is not behind this one
             int hi = t.count;
@@ -332,6 +332,7 @@ adamw_multi_kernel(const __grid_constant__ Table<MAX> t, Hyper h, const Hyper* d
                 if (t.item[mid].first <= tile) at = mid; else hi = mid;
             }
             end = at + 1 < t.count ? t.item[at + 1].first : t.tiles;
+            key = mix32(h.key + 0x85EBCA77u * t.item[at].number);
         }
         const Item& d = t.item[at];
         const int64_t i = (tile - d.first) * kTile + threadIdx.x * kPer;
@@ -340,8 +341,8 @@ adamw_multi_kernel(const __grid_constant__ Table<MAX> t, Hyper h, const Hyper* d
         const int left = rest >= kPer ? kPer : rest > 0 ? static_cast<int>(rest) : 0;
         if constexpr (EIGHT) {
             const int64_t block = (tile - d.first) * (kTile / kBlock) + (threadIdx.x >> 5);
-            if (full && d.plain) step8<T, true>(d, h, i, block, kPer);
-            else if (block * kBlock < d.n) step8<T, false>(d, h, i, block, left);
+            if (full && d.plain) step8<T, true>(d, h, key, i, block, kPer);
+            else if (block * kBlock < d.n) step8<T, false>(d, h, key, i, block, left);
         } else {
             if (full && d.plain) step32<T, true>(d, h, i, kPer);
             else if (left) step32<T, false>(d, h, i, left);
