@@ -83,11 +83,21 @@ __device__ __forceinline__ void store(T* dst, int64_t i, int left, bool vec, con
     }
 }
 
-// Square root to 2^-22 of it; of a subnormal number 0.
-__device__ __forceinline__ float sqrt_fast(float v) {
-    float r;
-    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-    return r;
+// Square roots to half a step but for rare cases (one Newton step on an
+// approximate 1 / root, so that what the 8-bit values are cut from is as exact
+// as a 32-bit number can be); of a subnormal number 0.
+__device__ __forceinline__ void roots(float (&v)[kPer]) {
+    float y[kPer], r[kPer], e[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y[k]) : "f"(v[k]));
+        y[k] = fminf(y[k], 1e19f);  // of 0: no infinity
+    }
+    vmul(r, v, y);
+    vmul(e, r, -1.f);
+    vfma(e, e, r, v);
+    vmul(y, y, 0.5f);
+    vfma(v, e, y, r);
 }
 
 // Eight e4m3 values.
@@ -203,8 +213,8 @@ __device__ __forceinline__ void step32(const Item& d, const Hyper& h, int64_t i,
 
 // Eight elements of a block with 8-bit moments; a warp has the whole block.
 // The kernel is bound by its instructions as much as by its bytes (10 of a
-// 16-bit weight), so square root and quotient are the approximate ones (2^-22
-// of p's update), and padding, ends and odd addresses are kept out of the
+// 16-bit weight), so the quotient is an approximate one (2^-22 of p's update),
+// and padding, ends and odd addresses are kept out of the
 // ordinary path.
 template <typename T, bool PLAIN>
 __device__ __forceinline__ void step8(const Item& d, const Hyper& h, uint32_t key, int64_t i, int64_t block, int left) {
@@ -223,17 +233,25 @@ __device__ __forceinline__ void step8(const Item& d, const Hyper& h, uint32_t ke
     const uint32_t on = PLAIN ? 0xFFu : taking_part(d.live, i, left);
     from_e4m3(cm, m);
     from_e4m3(cu, u);
-    // with m = its value x sm: b1 m + (1 - b1) g, and b2 (value x su)^2 + (1 - b2) g^2
-    const float sm = d.sm[block], su = d.su[block], sm1 = sm * (1.f - h.one_b1), su2 = su * su * h.b2;
+    // Each step is rounded by itself, in the formula's order: the 8-bit values
+    // are then those of the formula in 32-bit operations, and not now and then
+    // their neighbours.  (The additions one by one: in pairs they would be made
+    // one with the products before them.)
     float m1[kPer], root[kPer], q[kPer];
-    vmul(m1, g, h.one_b1);
-    vfma(m1, m, sm1, m1);
+    vmul(m, m, d.sm[block]);
+    vfma(m1, m, -1.f, g);
+    vmul(m1, m1, h.one_b1);
+    vmul(u, u, d.su[block]);
+    vmul(root, u, u);
+    vmul(root, root, h.b2);
     vmul(g, g, g);
     vmul(g, g, h.one_b2);
-    vmul(root, u, u);
-    vfma(root, root, su2, g);
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) root[k] = sqrt_fast(root[k]);
+    for (int k = 0; k < kPer; ++k) {
+        m1[k] = __fadd_rn(m[k], m1[k]);
+        root[k] = __fadd_rn(root[k], g[k]);
+    }
+    roots(root);
     vfma(q, root, h.inv_root, h.eps);
 #pragma unroll
     for (int k = 0; k < kPer; ++k) q[k] = rcp_fast(q[k]);
@@ -250,9 +268,6 @@ __device__ __forceinline__ void step8(const Item& d, const Hyper& h, uint32_t ke
                 p[k] = fmaf(-h.step_size, q[k], p[k] * h.decay);
                 m[k] = m1[k];
                 u[k] = root[k];
-            } else {
-                m[k] *= sm;
-                u[k] *= su;
             }
         }
     }
@@ -278,7 +293,7 @@ __device__ __forceinline__ void step8(const Item& d, const Hyper& h, uint32_t ke
         bu = __reduce_max_sync(0xffffffffu, bu);
     }
     const float fm = fmaxf(__uint_as_float(bm), 0x1p-100f), fu = fmaxf(__uint_as_float(bu), 0x1p-100f);
-    const float im = 448.f * rcp_fast(fm), iu = 448.f * rcp_fast(fu);
+    const float im = __frcp_rn(fm) * 448.f, iu = __frcp_rn(fu) * 448.f;
     const uint32_t first = static_cast<uint32_t>(i) * 0x9E3779B1u + key;
     uint32_t lo[kPer], hi[kPer];
 #pragma unroll

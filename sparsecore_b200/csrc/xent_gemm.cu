@@ -26,7 +26,12 @@ constexpr int kTile = 256;
 constexpr int kSlice = 64;                       // of the sum, in a stage: 128 bytes a row
 constexpr int kBox = 128 * kSlice * 2;           // bytes of one operand's plane in a stage
 constexpr int kRing = 12;                        // boxes in shared memory: 6 stages, or 3 of two planes
-constexpr int kChunk = 4;                        // stages added up in tensor memory for 32-bit operands
+// Stages added up in tensor memory before the epilogue takes the sum out.  Of
+// two planes: 2 where the sum is the result (errors of 4e-7 of it; 4 stages:
+// 9e-7), 4 where the logits' epilogue is long and has to be covered.  Of one
+// plane: 8 for the logits, whose loss is given in 32 bits.
+template <int PL, int MODE>
+constexpr int kChunk = MODE == 2 ? (PL == 2 ? 2 : INT_MAX) : PL == 2 ? 4 : 8;
 constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // a warpgroup of loads and MMAs, two of results
 // Registers a thread: of 168 x 384 at launch, 40 x 128 stay with the first
@@ -358,7 +363,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     const uint32_t tmem = sh.tmem;
     const int tiles = a.tiles_m * a.tiles_n * a.splits, pairs = gridDim.x / 2, pair = blockIdx.x / 2;
     const int all = static_cast<int>((a.K + kSlice - 1) / kSlice);
-    const int chunk = PL == 2 ? kChunk : all;
+    const int chunk = min(all, kChunk<PL, MODE>);
 
     if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
@@ -470,7 +475,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     tmem_load32(at + j, r);
                     tmem_load_wait();
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) z[j + k] = PL == 1 ? __uint_as_float(r[k]) : z[j + k] + __uint_as_float(r[k]);
+                    for (int k = 0; k < 32; ++k) z[j + k] += __uint_as_float(r[k]);
                 }
                 tc_fence_before();
                 __syncwarp();

@@ -126,6 +126,60 @@ def test_moments_in_8_bits(dtype, sizes):
                 assert bool(((held.double() * val) >= 0).all())
 
 
+def _mixed(v):
+    for shift, factor in ((16, 0x5B2C9E6D), (13, 0x3F4A7C15)):
+        v = (v ^ (v >> shift)) * factor & 0xFFFFFFFF
+    return v ^ (v >> 16)
+
+
+def _cut(val, bits, keep):
+    """Values over their block's scale, up or down by 16 bits, in 32-bit operations."""
+    b = _blocked(val)
+    top = b.abs().amax(1, keepdim=True).clamp_min(2.0 ** -100)
+    x = (b.abs() * (448.0 / top)).clamp_max(448.0)
+    low = torch.where(x < 2.0 ** -6, 2.0 ** -6, 0.0).float()
+    q = (((x + low).view(torch.int32) + (_blocked(bits).to(torch.int32) << 4)) & ~0xFFFFF).view(torch.float32) - low
+    if keep:
+        q = torch.where(b > 0, q.clamp_min(2.0 ** -9), q)
+    q = torch.where(b < 0, -q, q)
+    return q.to(torch.float8_e4m3fn).view(-1)[:val.numel()], (top * (1.0 / 448.0))[:, 0]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_8_bit_moments_are_the_formulas_bit_for_bit(dtype):
+    """Each operation of the formula rounded to 32 bits by itself gives the held bytes and scales
+    exactly, step after step: what is held does not depend on how the kernel groups its work."""
+    import sparsecore_b200 as sl
+
+    sizes = [70000, 2048, 300, 1]
+    ps, gs, live = _tensors(sizes, dtype, 11, sparse=(2,))
+    st = [_state8(n) for n in sizes]
+    b1, b2 = HYPER["betas"]
+    ref = [[m.clone(), v.clone(), (s[0].clone(), s[1].clone())] for m, v, s in st]
+    for step in range(1, 6):
+        gs = [g * (1 + 0.3 * step) for g in gs]
+        sl.adamw_step(ps, gs, [s[0] for s in st], [s[1] for s in st], step=step, live=live, scales=[s[2] for s in st], seed=9, **HYPER)
+        for i, (g, c, r, n) in enumerate(zip(gs, live, ref, sizes)):
+            mf = (_blocked(r[0].float()) * r[2][0][:, None]).view(-1)[:n]
+            vf = (_blocked(r[1].float()) * r[2][1][:, None]).view(-1)[:n].square()
+            gf = g.float()
+            m1 = mf + (gf - mf) * (1 - b1)
+            v1 = vf * b2 + gf * gf * (1 - b2)
+            root = v1.sqrt()
+            if c is not None:
+                held = (_blocked(r[1].float()) * r[2][1][:, None]).view(-1)[:n]
+                m1, root = torch.where(c < 0, mf, m1), torch.where(c < 0, held, root)
+            key = _mixed((9 + 0x9E3779B1 * step + 0x85EBCA77 * i) & 0xFFFFFFFF)
+            bits = _mixed((torch.arange(n, device=dev()) * 0x9E3779B1 + key) & 0xFFFFFFFF)
+            r[0], sm = _cut(m1, bits & 0xFFFF, False)
+            r[1], sv = _cut(root, bits >> 16, True)
+            r[2] = (sm, sv)
+            m, v, s = st[i]
+            assert torch.equal(m.view(torch.uint8), r[0].view(torch.uint8)) and torch.equal(v.view(torch.uint8), r[1].view(torch.uint8))
+            assert torch.equal(s[0], sm) and torch.equal(s[1], sv)
+
+
 @gpu
 def test_8_bit_values_are_right_on_average():
     """1000 times the same moments under other seeds: the mean of the held values
