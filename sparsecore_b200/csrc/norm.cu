@@ -29,7 +29,7 @@ int check(const sl_norm_args* n, const char* fn, bool back) {
                           static_cast<const void*>(n->dbias), static_cast<const void*>(n->dpost_weight),
                           static_cast<const void*>(n->dpost_bias)})
         SL_REQUIRE(!off_by(q, ew), fn, "misaligned vector");
-    SL_REQUIRE(!off_by(n->gate, eg) && !off_by(n->dgate, eg) && !off_by(n->workspace, 16) && !off_by(n->stats, 4), fn,
+    SL_REQUIRE(!off_by(n->gate, eg) && !off_by(n->dgate, eg) && !off_by(n->workspace, 16) && !off_by(n->stats, 16), fn,
                "misaligned operand");
     return SL_OK;
 }

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as N
 
@@ -71,6 +72,7 @@ class _LinearCrossEntropyFunction(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         x, weight, targets, prep = ctx.saved_tensors
         ignore_index, reduction, shape = ctx.opts

@@ -13,6 +13,7 @@ follows, so the stream is read and written once between two blocks.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as N
 
@@ -78,6 +79,7 @@ class _ResidualNormFunction(torch.autograd.Function):
         return out, h
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, dh):
         y, out, weight, bias, gate, scale_t, pw, pb, stats = ctx.saved_tensors
         dtype, opts = ctx.opts

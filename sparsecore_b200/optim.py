@@ -318,7 +318,8 @@ class FusedAdamW(torch.optim.Optimizer):
             if not params:
                 continue
             for p in params:
-                if not self.state[p]:
+                st = self.state[p]
+                if not st or st["exp_avg"].numel() != p.numel():  # new, or a layer drawn again at another capacity
                     self._init_state(p)
             plan = self._plan(k, params, cols)
             grads = [p.grad for p in params]
@@ -350,6 +351,9 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, but the moments keep their own types (torch casts a state to its parameter's type)."""
+        needed = "exp_avg_sq" if self.state_bits == 32 else "exp_avg_sq_root"
+        if any(needed not in st for st in state_dict["state"].values()):
+            raise ValueError(f"FusedAdamW: the state is not one of {self.state_bits}-bit moments")
         super().load_state_dict(state_dict)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(ids, [p for g in self.param_groups for p in g["params"]]):

@@ -368,6 +368,24 @@ def test_state_goes_through_a_checkpoint(bits):
             assert u.shape == p.shape and torch.equal(u, w)
 
 
+@gpu
+def test_a_layer_drawn_again_and_a_state_of_other_bits():
+    import sparsecore_b200 as sl
+
+    model, x = _model(), torch.randn(40, 96, device=dev())
+    opts = {bits: sl.FusedAdamW(model, state_bits=bits) for bits in (32, 8)}
+    for _ in range(2):
+        for o in opts.values():
+            o.zero_grad()
+            model(x).square().mean().backward()
+            o.step()
+        model[0].reset_parameters()  # another mask: another number of slots
+    assert torch.isfinite(model(x)).all() and not model[0]._values[model[0]._csr.col_indices < 0].any()
+    for a, b in ((32, 8), (8, 32)):
+        with pytest.raises(ValueError):
+            opts[a].load_state_dict(opts[b].state_dict())
+
+
 def test_refusals_without_a_gpu():
     import sparsecore_b200 as sl
 

@@ -272,6 +272,19 @@ def test_runs_are_repeatable_and_replay_in_a_graph():
     assert all(torch.equal(a, b) for a, b in zip(held, want))
 
 
+@gpu
+def test_second_derivatives_are_refused():
+    """The gradients are not differentiable again, and say so."""
+    import sparsecore_b200 as sl
+
+    y, w = torch.randn(4, 8, device=dev(), requires_grad=True), torch.ones(8, device=dev(), requires_grad=True)
+    t = torch.zeros(4, dtype=torch.int64, device=dev())
+    for out in (sl.residual_norm(y, y.detach(), w)[1].square().sum(), sl.linear_cross_entropy(y, w.expand(5, 8), t)):
+        (g,) = torch.autograd.grad(out, (y,), create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
+
+
 def test_refusals():
     import sparsecore_b200 as sl
 
