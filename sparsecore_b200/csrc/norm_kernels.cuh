@@ -144,8 +144,9 @@ __device__ __forceinline__ int64_t gate_offset(const A& a, int64_t t) {
 
 // blockDim = (32 * warps a row, rows): one row a warp up to 32 elements a
 // lane, without a barrier; more warps a row beyond.  A CTA takes row after
-// row; as many CTAs as an SM holds.
-template <typename TY, typename TR, int VE, int NV, bool POST>
+// row; as many CTAs as an SM holds.  TV: type of the vectors (asked for at run
+// time it cost 10 of 73 us on 8191 x 4096 bf16 rows with a norm on both sides).
+template <typename TY, typename TR, typename TV, int VE, int NV, bool POST>
 __global__ void __launch_bounds__(kMaxThreads, VE * NV <= 16 ? 2 : 1)
 norm_fwd_kernel(Args<TY, TR> a) {
     __shared__ float2 ws[64];
@@ -177,12 +178,12 @@ norm_fwd_kernel(Args<TY, TR> a) {
             float y[VE], q[VE];
             yr.get(j, y);
             if (POST) {
-                load_v<TY, VE>(a.pw, a.vec_f32, c, q);
+                load_f<TV, VE>(static_cast<const TV*>(a.pw) + c, q);
                 vadd(y, y, -st.w);
                 vmul(y, y, st.z);
                 if (a.pb) {
                     float b[VE];
-                    load_v<TY, VE>(a.pb, a.vec_f32, c, b);
+                    load_f<TV, VE>(static_cast<const TV*>(a.pb) + c, b);
                     vfma(y, y, q, b);
                 } else {
                     vmul(y, y, q);
@@ -212,12 +213,12 @@ norm_fwd_kernel(Args<TY, TR> a) {
             const int c = col + j * step;
             if (c >= cols) continue;
             float w[VE], o[VE];
-            load_v<TY, VE>(a.w, a.vec_f32, c, w);
+            load_f<TV, VE>(static_cast<const TV*>(a.w) + c, w);
             vadd(o, r[j], -st.y);
             vmul(o, o, st.x);
             if (a.b) {
                 float b[VE];
-                load_v<TY, VE>(a.b, a.vec_f32, c, b);
+                load_f<TV, VE>(static_cast<const TV*>(a.b) + c, b);
                 vfma(o, o, w, b);
             } else {
                 vmul(o, o, w);
@@ -709,7 +710,8 @@ norm_reduce_kernel(ReduceList list) {
     for (int64_t g = blockIdx.y; g < q.groups; g += gridDim.y) {
         float a = 0.f;
         if (c < q.n)
-            for (int64_t k = threadIdx.y; k < q.seg; k += 32) a += q.src[(g * q.seg + k) * q.n + c];
+#pragma unroll 8
+            for (int k = threadIdx.y; k < q.seg; k += 32) a += q.src[(g * q.seg + k) * q.n + c];
         __syncthreads();
         s[threadIdx.y][threadIdx.x] = a;
         __syncthreads();
@@ -794,12 +796,18 @@ int forward(const sl_norm_args& n, cudaStream_t s) {
     const dim3 block(32 * p.warps, p.warps == 1 ? 4 : 1);
     const int64_t beside = std::max<int64_t>(1, (p.ve * p.nv <= 16 ? 1024 : 512) / (block.x * block.y));
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>((n.rows + block.y - 1) / block.y, num_sms() * beside));
-    return with_plan<TY>(p, [&](auto ve, auto nv) {
-        if (n.post_weight) norm_fwd_kernel<TY, TR, ve, nv, true><<<grid, block, 0, s>>>(a);
-        else norm_fwd_kernel<TY, TR, ve, nv, false><<<grid, block, 0, s>>>(a);
-        SL_RETURN_IF_LAUNCH_FAILED("sl_norm_forward");
-        return static_cast<int>(SL_OK);
-    });
+    auto launch = [&](auto tv) {
+        using TV = decltype(tv);
+        return with_plan<TY>(p, [&](auto ve, auto nv) {
+            if (n.post_weight) norm_fwd_kernel<TY, TR, TV, ve, nv, true><<<grid, block, 0, s>>>(a);
+            else norm_fwd_kernel<TY, TR, TV, ve, nv, false><<<grid, block, 0, s>>>(a);
+            SL_RETURN_IF_LAUNCH_FAILED("sl_norm_forward");
+            return static_cast<int>(SL_OK);
+        });
+    };
+    if constexpr (sizeof(TY) == 2)
+        if (n.weight_dtype == SL_F32) return launch(float{});
+    return launch(TY{});
 }
 
 template <typename TY, typename TR>
