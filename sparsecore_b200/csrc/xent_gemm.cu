@@ -99,6 +99,13 @@ __device__ __forceinline__ void store32(void* dst, const uint32_t (&v)[8]) {
                  : "memory");
 }
 
+__device__ __forceinline__ void load32(const void* src, uint32_t (&v)[8]) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "l"(src)
+                 : "memory");
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 // What brings a sum of 32-bit operands' planes back to the logit.
@@ -294,12 +301,29 @@ __device__ __forceinline__ void epilogue_out(const Args& a, float (&z)[128], int
     const int64_t row = m * a.N + n0;
     if (a.o.acc) {
         float* q = a.o.acc + row;
+        if (n == 128 && (reinterpret_cast<uintptr_t>(q) & 31) == 0) {
 #pragma unroll
-        for (int j = 0; j < 128; ++j)
-            if (j < n) {
-                if (!a.o.first) z[j] += q[j];
-                if (!a.o.last) q[j] = z[j];
+            for (int j = 0; j < 128; j += 8) {
+                uint32_t v[8];
+                if (!a.o.first) {
+                    load32(q + j, v);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) z[j + k] += __uint_as_float(v[k]);
+                }
+                if (!a.o.last) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = __float_as_uint(z[j + k]);
+                    store32(q + j, v);
+                }
             }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 128; ++j)
+                if (j < n) {
+                    if (!a.o.first) z[j] += q[j];
+                    if (!a.o.last) q[j] = z[j];
+                }
+        }
         if (!a.o.last) return;
     }
     const int64_t bytes = a.o.dtype == SL_F32 ? 4 : 2;
