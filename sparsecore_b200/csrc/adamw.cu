@@ -13,6 +13,12 @@
 // number, the tensor's number, the step and the caller's seed), which keeps
 // every moment right on average.  A root above zero is never held as zero:
 // its element's next update would be divided by eps alone.
+//
+// 32-bit moments are bound by memory: 12.2 M weights in padded arrays (32
+// bytes a slot, padding read too) take 67 us, 5.8 TB/s.  8-bit ones are bound
+// by instructions, about 65 an element, half of them integer and logic ones
+// for the dither: 335 M bf16 weights take 0.89 ms where their 10 bytes each
+// would take 0.52.
 #include <cuda_fp8.h>
 
 #include <cmath>

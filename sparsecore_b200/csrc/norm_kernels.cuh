@@ -145,7 +145,9 @@ __device__ __forceinline__ int64_t gate_offset(const A& a, int64_t t) {
 // blockDim = (32 * warps a row, rows): one row a warp up to 32 elements a
 // lane, without a barrier; more warps a row beyond.  A CTA takes row after
 // row; as many CTAs as an SM holds.  TV: type of the vectors (asked for at run
-// time it cost 10 of 73 us on 8191 x 4096 bf16 rows with a norm on both sides).
+// time it cost 10 of 73 us on 8191 x 4096 bf16 rows with a norm on both sides,
+// 63 us of 41 for 268 MB, bound by instructions: 45 an element).  16384 x 768
+// fp32: 33 us of 31 for 201 MB, bound by memory.
 template <typename TY, typename TR, typename TV, int VE, int NV, bool POST>
 __global__ void __launch_bounds__(kMaxThreads, VE * NV <= 16 ? 2 : 1)
 norm_fwd_kernel(Args<TY, TR> a) {
@@ -417,7 +419,12 @@ struct Ring {
 // to five a column) stay in registers, which leave room for one CTA an SM.
 // Between two barriers a warp has the sums of the next row and the results
 // of this one to work on, which hide each other's latencies.
-// L: LayerNorm, or a bias.
+//
+// 8191 x 4096 bf16 with both norms and a gate a channel: 100 us of 62 for its
+// 403 MB; 220 us with two barriers a row and no ring, 121 us before the next
+// row's sums were taken beside this row's results.  Bound by the latency of
+// sixteen warps with one row under way (the scheduler issues in half of the
+// clocks).  L: LayerNorm, or a bias.
 template <typename TY, typename TR, int VE, int NV, bool POST, bool L, bool RING>
 __global__ void __launch_bounds__(kMaxThreads)
 norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
@@ -557,116 +564,116 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
     auto run_of = [&](int64_t t) { return a.gate && !each ? static_cast<int64_t>(static_cast<uint32_t>(t) / static_cast<uint32_t>(a.gate_rows)) : 0; };
 
     if (t0 < t1) {
-    if constexpr (RING)
-        for (int k = 0; k < stages - 1; ++k) fetch(t0 + k, k);
-    for (int k = 0; k < 3; ++k) vec_keep(k, 0);
-    int64_t run = run_of(t0), gate_row = run * a.D, run_end = (run + 1) * a.gate_rows;
-    vec_keep(3, gate_row);
-    if constexpr (RING) copies_wait(stages - 2);
-    float4 st = statistics(t0);
-    int stage = 0, flip = 0;
-    sums(t0, gate_row, st, mine, ws[0]);
-    for (int64_t t = t0; t < t1; ++t) {
-        const char* const held = mine + stage * stage_bytes;
-        const int after = stage + 1 == stages ? 0 : stage + 1;
-        if constexpr (RING) {
-            fetch(t + stages - 1, stage == 0 ? stages - 1 : stage - 1);
-            copies_wait(stages - 2);  // row t + 1 is here
-        }
-        const float4 next = statistics(t + 1);
-        if (warps > 1) __syncthreads();
-        else __syncwarp();
-        float s[4 * Q];
-        sums_get<Q>(s, warps, ws[flip]);
-        flip ^= 1;
-        // A run's last row is finished before the next run's gate takes its place.
-        const bool turn = a.gate && !each && t + 1 == run_end;
-        if (t + 1 < t1 && !turn) sums(t + 1, gate_row, next, mine + after * stage_bytes, ws[flip]);
-        const float c2 = s[0] * inv_d, c1 = L && a.layer ? s[1] * inv_d : 0.f;
-        float e1 = 0.f, e2 = 0.f;
-        if (POST) {
-            e2 = s[2] - st.x * c2 * s[3];
-            if constexpr (Q == 2) {
-                e2 -= st.x * c1 * s[4];
-                e1 = a.layer ? (s[5] - st.x * (c2 * s[6] + c1 * s[7])) * (scale * inv_d) : 0.f;
+        if constexpr (RING)
+            for (int k = 0; k < stages - 1; ++k) fetch(t0 + k, k);
+        for (int k = 0; k < 3; ++k) vec_keep(k, 0);
+        int64_t run = run_of(t0), gate_row = run * a.D, run_end = (run + 1) * a.gate_rows;
+        vec_keep(3, gate_row);
+        if constexpr (RING) copies_wait(stages - 2);
+        float4 st = statistics(t0);
+        int stage = 0, flip = 0;
+        sums(t0, gate_row, st, mine, ws[0]);
+        for (int64_t t = t0; t < t1; ++t) {
+            const char* const held = mine + stage * stage_bytes;
+            const int after = stage + 1 == stages ? 0 : stage + 1;
+            if constexpr (RING) {
+                fetch(t + stages - 1, stage == 0 ? stages - 1 : stage - 1);
+                copies_wait(stages - 2);  // row t + 1 is here
             }
-            e2 *= scale * inv_d;
-        }
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int c = col + j * step;
-            if (c >= cols) continue;
-            const int64_t at = t * a.D + c;
-            float x[VE], g[VE], d[VE], w[VE], y[VE];
-            get(TR{}, kX, a.out, t, held, j, x);
-            get(TY{}, kDn, a.dh, t, held, j, g);
-            get(TR{}, kD, a.dout, t, held, j, d);
-            vector(0, 0, j, w);
-            vfma(x, x, st.x, st.y);
-            vfma(aw[j], g, x, aw[j]);
-            if (L) vadd(ab[j], ab[j], g);
-            if (L) vfma(x, x, -c2, -c1);
-            else vmul(x, x, -c2);
-            vfma(g, g, w, x);
-            vfma(d, g, st.x, d);
-            store_f<TR, VE>(a.dr + at, d);
-            get(TY{}, kY, a.y, t, held, j, y);
-            float u[VE], pw[VE];
+            const float4 next = statistics(t + 1);
+            if (warps > 1) __syncthreads();
+            else __syncwarp();
+            float s[4 * Q];
+            sums_get<Q>(s, warps, ws[flip]);
+            flip ^= 1;
+            // A run's last row is finished before the next run's gate takes its place.
+            const bool turn = a.gate && !each && t + 1 == run_end;
+            if (t + 1 < t1 && !turn) sums(t + 1, gate_row, next, mine + after * stage_bytes, ws[flip]);
+            const float c2 = s[0] * inv_d, c1 = L && a.layer ? s[1] * inv_d : 0.f;
+            float e1 = 0.f, e2 = 0.f;
             if (POST) {
-                vector(1, 0, j, pw);
-                vfma(y, y, st.z, st.w);
-                if (L && a.pb) {
-                    vector(2, 0, j, x);
-                    vfma(u, y, pw, x);
+                e2 = s[2] - st.x * c2 * s[3];
+                if constexpr (Q == 2) {
+                    e2 -= st.x * c1 * s[4];
+                    e1 = a.layer ? (s[5] - st.x * (c2 * s[6] + c1 * s[7])) * (scale * inv_d) : 0.f;
+                }
+                e2 *= scale * inv_d;
+            }
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = col + j * step;
+                if (c >= cols) continue;
+                const int64_t at = t * a.D + c;
+                float x[VE], g[VE], d[VE], w[VE], y[VE];
+                get(TR{}, kX, a.out, t, held, j, x);
+                get(TY{}, kDn, a.dh, t, held, j, g);
+                get(TR{}, kD, a.dout, t, held, j, d);
+                vector(0, 0, j, w);
+                vfma(x, x, st.x, st.y);
+                vfma(aw[j], g, x, aw[j]);
+                if (L) vadd(ab[j], ab[j], g);
+                if (L) vfma(x, x, -c2, -c1);
+                else vmul(x, x, -c2);
+                vfma(g, g, w, x);
+                vfma(d, g, st.x, d);
+                store_f<TR, VE>(a.dr + at, d);
+                get(TY{}, kY, a.y, t, held, j, y);
+                float u[VE], pw[VE];
+                if (POST) {
+                    vector(1, 0, j, pw);
+                    vfma(y, y, st.z, st.w);
+                    if (L && a.pb) {
+                        vector(2, 0, j, x);
+                        vfma(u, y, pw, x);
+                    } else {
+                        vmul(u, y, pw);
+                    }
                 } else {
-                    vmul(u, y, pw);
+#pragma unroll
+                    for (int k = 0; k < VE; ++k) u[k] = y[k];
                 }
-            } else {
+                if (a.gate) gate(t, gate_row, held, j, x);
+                if (a.need_scale) {
 #pragma unroll
-                for (int k = 0; k < VE; ++k) u[k] = y[k];
-            }
-            if (a.gate) gate(t, gate_row, held, j, x);
-            if (a.need_scale) {
-#pragma unroll
-                for (int k = 0; k < VE; ++k) as = fmaf(d[k], a.gate ? x[k] * u[k] : u[k], as);
-            }
-            vmul(d, d, scale);
-            if (each) {
-                vmul(u, u, d);
-                vmul(d, d, x);
-                if (a.need_gate) {
-                    if (a.gate_f32) store_f<float, VE>(static_cast<float*>(a.dgate) + at, u);
-                    else store_f<TY, VE>(static_cast<TY*>(a.dgate) + at, u);
+                    for (int k = 0; k < VE; ++k) as = fmaf(d[k], a.gate ? x[k] * u[k] : u[k], as);
                 }
-            } else if (a.gate) {
-                vfma(ag[j], d, u, ag[j]);
-                vmul(d, d, x);
-            }
-            if (POST) {
-                vfma(apw[j], d, y, apw[j]);
-                if (L) vadd(apb[j], apb[j], d);
-                if (L) vfma(y, y, -e2, -e1);
-                else vmul(y, y, -e2);
-                vfma(d, d, pw, y);
-                vmul(d, d, st.z);
-            }
-            if (a.need_dy) store_f<TY, VE>(a.dy + at, d);
-            if (a.gate_direct && (t + 1 == t1 || t + 1 == run_end)) {  // a run of rows ends
-                if (a.gate_f32) store_f<float, VE>(static_cast<float*>(a.dgate) + gate_row + c, ag[j]);
-                else store_f<TY, VE>(static_cast<TY*>(a.dgate) + gate_row + c, ag[j]);
+                vmul(d, d, scale);
+                if (each) {
+                    vmul(u, u, d);
+                    vmul(d, d, x);
+                    if (a.need_gate) {
+                        if (a.gate_f32) store_f<float, VE>(static_cast<float*>(a.dgate) + at, u);
+                        else store_f<TY, VE>(static_cast<TY*>(a.dgate) + at, u);
+                    }
+                } else if (a.gate) {
+                    vfma(ag[j], d, u, ag[j]);
+                    vmul(d, d, x);
+                }
+                if (POST) {
+                    vfma(apw[j], d, y, apw[j]);
+                    if (L) vadd(apb[j], apb[j], d);
+                    if (L) vfma(y, y, -e2, -e1);
+                    else vmul(y, y, -e2);
+                    vfma(d, d, pw, y);
+                    vmul(d, d, st.z);
+                }
+                if (a.need_dy) store_f<TY, VE>(a.dy + at, d);
+                if (a.gate_direct && (t + 1 == t1 || t + 1 == run_end)) {  // a run of rows ends
+                    if (a.gate_f32) store_f<float, VE>(static_cast<float*>(a.dgate) + gate_row + c, ag[j]);
+                    else store_f<TY, VE>(static_cast<TY*>(a.dgate) + gate_row + c, ag[j]);
 #pragma unroll
-                for (int k = 0; k < VE; ++k) ag[j][k] = 0.f;
+                    for (int k = 0; k < VE; ++k) ag[j][k] = 0.f;
+                }
             }
+            if (turn && t + 1 < t1) {
+                gate_row += a.D;
+                run_end += a.gate_rows;
+                vec_keep(3, gate_row);
+                sums(t + 1, gate_row, next, mine + after * stage_bytes, ws[flip]);
+            }
+            st = next;
+            stage = after;
         }
-        if (turn && t + 1 < t1) {
-            gate_row += a.D;
-            run_end += a.gate_rows;
-            vec_keep(3, gate_row);
-            sums(t + 1, gate_row, next, mine + after * stage_bytes, ws[flip]);
-        }
-        st = next;
-        stage = after;
-    }
     }
     const int64_t plane = a.ctas * a.D;
 #pragma unroll

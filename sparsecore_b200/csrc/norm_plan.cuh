@@ -49,7 +49,9 @@ constexpr int64_t kSimpleCols = 8192;
 inline Plan backward_plan(int64_t D, bool wide, int64_t elem, bool full) {
     return make_plan(D, wide, elem, full ? 8 : D > 4096 ? 32 : 16);
 }
-inline int backward_rows(const Plan& p, bool full) { return full ? 1 : std::max(1, 4 / p.warps); }
+// Rows a CTA takes at a time: several only where a row is one warp's, since
+// the sums of a row of more warps pass a barrier of the CTA.
+inline int backward_rows(const Plan& p, bool full) { return !full && p.warps == 1 ? 4 : 1; }
 
 // The backward pass's split of the rows over CTAs of `rows` rows at a time.
 struct Split {

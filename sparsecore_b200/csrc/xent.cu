@@ -9,7 +9,8 @@
 // Forward: a matrix product whose epilogue leaves, of every 128 columns of
 // a row, their maximum and the sum of exponentials below it; a second small
 // kernel joins them.  Backward: pieces of the vocabulary, each with its
-// logits made again, turned into G in the epilogue, and multiplied twice.
+// logits made again, turned into G in the epilogue, and multiplied twice:
+// 8 T D V operations in all, where keeping the logits would leave 6.
 //
 // 16-bit inputs are multiplied as they are.  32-bit ones are split into two
 // fp16 planes, a = 2^-k (a_hi + a_lo) with 22 bits between them (2^-k from
@@ -102,7 +103,8 @@ __device__ __forceinline__ unsigned finite_bits(float v) {
 
 // Largest finite magnitudes of 32-bit operands, a warp a row: CTAs below
 // `x_blocks` take x (rows of tokens that do not count are left out), the
-// others w; one value a CTA, joined by planes_kernel.
+// others w; one value a CTA, joined by planes_kernel.  16384 x 768 and 256 x
+// 768: 13 us of 8 for 51 MB (the pass after it finds x in L2: 20 us).
 __global__ void __launch_bounds__(kThreads)
 absmax_kernel(Source q, int x_blocks, unsigned* part, int vec) {
     __shared__ unsigned s[kThreads / 32];

@@ -10,9 +10,17 @@
 //
 // 32-bit operands come as two fp16 planes, a stage holding both, and are
 // multiplied as lo.hi, hi.lo and hi.hi.  The matrix units cut rather than
-// round when they add to a sum, so for these a sum in tensor memory is at
-// most kChunk stages long; the epilogue's warps add the chunks in registers,
-// rounding to nearest.
+// round when they add to a sum, so a sum in tensor memory is at most kChunk
+// stages long; the epilogue's warps add the chunks in registers, rounding to
+// nearest.
+//
+// What bounds it: the tensor cores.  Losses of 4096 tokens over 50001 columns
+// of 768 in 32 bits take 636 us, 1483 TFLOP/s of fp16 products; of 8192 tokens
+// over 128000 columns of 2048 in bf16 2.92 ms, 1471 TFLOP/s (0.90 and 0.89 of
+// the 1646 measured for a library product in a burst).  256 x 256 tiles of a
+// pair load 128 operand bytes a clock and SM, half of what a 128 x 256 tile
+// of one SM would.  Small problems are bound by a tile's own latency: 16384 x
+// 768 over 256 columns has 64 tiles for 74 pairs.
 #include <algorithm>
 
 #include "umma.cuh"
@@ -21,6 +29,8 @@
 namespace slb {
 namespace xent {
 namespace {
+
+enum Mode : int { kStats, kGrad, kOut, kLosses };
 
 constexpr int kTile = 256;
 constexpr int kSlice = 64;                       // of the sum, in a stage: 128 bytes a row
@@ -31,7 +41,7 @@ constexpr int kRing = 12;                        // boxes in shared memory: 6 st
 // 9e-7), 4 where the logits' epilogue is long and has to be covered.  Of one
 // plane: 8 for the logits, whose loss is given in 32 bits.
 template <int PL, int MODE>
-constexpr int kChunk = MODE == 2 ? (PL == 2 ? 2 : INT_MAX) : PL == 2 ? 4 : 8;
+constexpr int kChunk = MODE == kOut ? (PL == 2 ? 2 : INT_MAX) : PL == 2 ? 4 : 8;
 constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // a warpgroup of loads and MMAs, two of results
 // Registers a thread: of 168 x 384 at launch, 40 x 128 stay with the first
@@ -39,8 +49,6 @@ constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // a warpgroup of loads and
 constexpr int kRegsLow = 40, kRegsHigh = 232;
 static_assert(kRegsLow * 128 + kRegsHigh * 256 <= 168 * kThreads, "registers of the launch");
 constexpr size_t kSmem = kRing * kBox + 1024 + 4096;
-
-enum Mode : int { kStats, kGrad, kOut, kLosses };
 
 struct Args {
     Problem p;
@@ -69,9 +77,13 @@ static_assert(sizeof(Shared) <= 4096, "room behind the ring");
 // Whether all the epilogue's warps got their sums: they wait for one another.
 __device__ __forceinline__ bool epilogue_agrees(bool ok) {
     int all;
-    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n bar.red.and.pred q, 1, %2, p;\n selp.b32 %0, 1, 0, q;\n}\n" : "=r"(all) : "r"(static_cast<int>(ok)), "n"(32 * kEpilogueWarps) : "memory");
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n bar.red.and.pred q, 1, %2, p;\n selp.b32 %0, 1, 0, q;\n}\n"
+                 : "=r"(all)
+                 : "r"(static_cast<int>(ok)), "n"(32 * kEpilogueWarps)
+                 : "memory");
     return all;
 }
+
 // A barrier of the epilogue's warps alone.
 __device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory"); }
 
@@ -390,90 +402,90 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     const int chunk = min(all, kChunk<PL, MODE>);
 
     if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
-    if (warp == 0 && lane == 0) {  // loads
-        uint32_t stage = 0, phase = 0;
-        bool ok = true;
-        for (int id = pair; id < tiles && ok; id += pairs) {
-            int tm, tn, split;
-            locate(a, id, tm, tn, split);
-            const int row_a = tm * kTile + static_cast<int>(rank) * 128, row_b = tn * kTile + static_cast<int>(rank) * 128;
-            const int k1 = min(all, (split + 1) * a.per_split);
-            for (int k = split * a.per_split; k < k1; ++k) {
-                if (!mbar_wait(&sh.empty[stage], phase ^ 1, a.status)) { ok = false; break; }
-                if (rank == 0) mbar_expect_tx(&sh.full[stage], 2 * kStageBytes);
-                const uint32_t bar = leader_addr(&sh.full[stage]);
-                char* dst = ring + stage * kStageBytes;
-                const int x = k * kSlice;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
+        if (warp == 0 && lane == 0) {  // loads
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            for (int id = pair; id < tiles && ok; id += pairs) {
+                int tm, tn, split;
+                locate(a, id, tm, tn, split);
+                const int row_a = tm * kTile + static_cast<int>(rank) * 128, row_b = tn * kTile + static_cast<int>(rank) * 128;
+                const int k1 = min(all, (split + 1) * a.per_split);
+                for (int k = split * a.per_split; k < k1; ++k) {
+                    if (!mbar_wait(&sh.empty[stage], phase ^ 1, a.status)) { ok = false; break; }
+                    if (rank == 0) mbar_expect_tx(&sh.full[stage], 2 * kStageBytes);
+                    const uint32_t bar = leader_addr(&sh.full[stage]);
+                    char* dst = ring + stage * kStageBytes;
+                    const int x = k * kSlice;
 #pragma unroll
-                for (int pl = 0; pl < PL; ++pl, dst += 2 * kBox) {
-                    if (a.a_mn) {
-                        tma_load_3d_pair(dst, &map_a, row_a, x, pl, bar);
-                        tma_load_3d_pair(dst + kBox / 2, &map_a, row_a + 64, x, pl, bar);
-                    } else {
-                        tma_load_3d_pair(dst, &map_a, x, row_a, pl, bar);
-                    }
-                    if (a.b_mn) {
-                        tma_load_3d_pair(dst + kBox, &map_b, row_b, x, pl, bar);
-                        tma_load_3d_pair(dst + kBox + kBox / 2, &map_b, row_b + 64, x, pl, bar);
-                    } else {
-                        tma_load_3d_pair(dst + kBox, &map_b, x, row_b, pl, bar);
-                    }
-                }
-                if (++stage == kStages) stage = 0, phase ^= 1;
-            }
-        }
-        // The last stages are free again before the CTA ends: every commit of
-        // the other CTA's thread has then arrived here.
-        for (int s = 0; s < kStages && ok; ++s) {
-            ok = mbar_wait(&sh.empty[stage], phase ^ 1, a.status);
-            if (++stage == kStages) stage = 0, phase ^= 1;
-        }
-        if (!ok)  // given up: let the copies in flight land before the CTA may end
-            for (int i = 0; i < 2000; ++i) __nanosleep(1000);
-    } else if (warp == 1 && lane == 0 && rank == 0) {  // MMAs of both CTAs
-        const uint32_t idesc = umma_idesc(a.p.bf16, a.a_mn, a.b_mn, kTile);
-        const uint32_t step_a = (a.a_mn ? 16 * 128 : 32) >> 4, step_b = (a.b_mn ? 16 * 128 : 32) >> 4;
-        uint32_t stage = 0, phase = 0, done = 0;
-        bool ok = true;
-        for (int id = pair; id < tiles && ok; id += pairs) {
-            int tm, tn, split;
-            locate(a, id, tm, tn, split);
-            const int k1 = min(all, (split + 1) * a.per_split);
-            for (int k0 = split * a.per_split; k0 < k1 && ok; k0 += chunk, ++done) {
-                const uint32_t buf = done & 1;
-                if (!mbar_wait_cluster(&sh.tmem_empty[buf], ((done >> 1) & 1) ^ 1, a.status)) { ok = false; break; }
-                tc_fence_after();
-                const uint32_t d = tmem + buf * kTile;
-                uint32_t add = 0;
-                const int end = min(k1, k0 + chunk);
-                for (int k = k0; k < end; ++k) {
-                    if (!mbar_wait_cluster(&sh.full[stage], phase, a.status)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint32_t base = smem_addr(ring + stage * kStageBytes);
-                    uint64_t da[PL], db[PL];
-#pragma unroll
-                    for (int pl = 0; pl < PL; ++pl) {
-                        da[pl] = umma_desc(base + pl * 2 * kBox, a.a_mn);
-                        db[pl] = umma_desc(base + pl * 2 * kBox + kBox, a.b_mn);
-                    }
-                    // the small products first, while the sum is small
-#pragma unroll
-                    for (int pr = PL == 2 ? 0 : 2; pr < 3; ++pr) {
-                        const uint64_t qa = da[pr == 0 ? PL - 1 : 0], qb = db[pr == 1 ? PL - 1 : 0];
-#pragma unroll
-                        for (int i = 0; i < kSlice / 16; ++i) {
-                            umma_pair(d, qa + i * step_a, qb + i * step_b, idesc, add);
-                            add = 1;
+                    for (int pl = 0; pl < PL; ++pl, dst += 2 * kBox) {
+                        if (a.a_mn) {
+                            tma_load_3d_pair(dst, &map_a, row_a, x, pl, bar);
+                            tma_load_3d_pair(dst + kBox / 2, &map_a, row_a + 64, x, pl, bar);
+                        } else {
+                            tma_load_3d_pair(dst, &map_a, x, row_a, pl, bar);
+                        }
+                        if (a.b_mn) {
+                            tma_load_3d_pair(dst + kBox, &map_b, row_b, x, pl, bar);
+                            tma_load_3d_pair(dst + kBox + kBox / 2, &map_b, row_b + 64, x, pl, bar);
+                        } else {
+                            tma_load_3d_pair(dst + kBox, &map_b, x, row_b, pl, bar);
                         }
                     }
-                    umma_commit_pair(&sh.empty[stage]);
                     if (++stage == kStages) stage = 0, phase ^= 1;
                 }
-                umma_commit_pair(&sh.tmem_full[buf]);
+            }
+            // The last stages are free again before the CTA ends: every commit of
+            // the other CTA's thread has then arrived here.
+            for (int s = 0; s < kStages && ok; ++s) {
+                ok = mbar_wait(&sh.empty[stage], phase ^ 1, a.status);
+                if (++stage == kStages) stage = 0, phase ^= 1;
+            }
+            if (!ok)  // given up: let the copies in flight land before the CTA may end
+                for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+        } else if (warp == 1 && lane == 0 && rank == 0) {  // MMAs of both CTAs
+            const uint32_t idesc = umma_idesc(a.p.bf16, a.a_mn, a.b_mn, kTile);
+            const uint32_t step_a = (a.a_mn ? 16 * 128 : 32) >> 4, step_b = (a.b_mn ? 16 * 128 : 32) >> 4;
+            uint32_t stage = 0, phase = 0, done = 0;
+            bool ok = true;
+            for (int id = pair; id < tiles && ok; id += pairs) {
+                int tm, tn, split;
+                locate(a, id, tm, tn, split);
+                const int k1 = min(all, (split + 1) * a.per_split);
+                for (int k0 = split * a.per_split; k0 < k1 && ok; k0 += chunk, ++done) {
+                    const uint32_t buf = done & 1;
+                    if (!mbar_wait_cluster(&sh.tmem_empty[buf], ((done >> 1) & 1) ^ 1, a.status)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t d = tmem + buf * kTile;
+                    uint32_t add = 0;
+                    const int end = min(k1, k0 + chunk);
+                    for (int k = k0; k < end; ++k) {
+                        if (!mbar_wait_cluster(&sh.full[stage], phase, a.status)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint32_t base = smem_addr(ring + stage * kStageBytes);
+                        uint64_t da[PL], db[PL];
+#pragma unroll
+                        for (int pl = 0; pl < PL; ++pl) {
+                            da[pl] = umma_desc(base + pl * 2 * kBox, a.a_mn);
+                            db[pl] = umma_desc(base + pl * 2 * kBox + kBox, a.b_mn);
+                        }
+                        // the small products first, while the sum is small
+#pragma unroll
+                        for (int pr = PL == 2 ? 0 : 2; pr < 3; ++pr) {
+                            const uint64_t qa = da[pr == 0 ? PL - 1 : 0], qb = db[pr == 1 ? PL - 1 : 0];
+#pragma unroll
+                            for (int i = 0; i < kSlice / 16; ++i) {
+                                umma_pair(d, qa + i * step_a, qb + i * step_b, idesc, add);
+                                add = 1;
+                            }
+                        }
+                        umma_commit_pair(&sh.empty[stage]);
+                        if (++stage == kStages) stage = 0, phase ^= 1;
+                    }
+                    umma_commit_pair(&sh.tmem_full[buf]);
+                }
             }
         }
-    }
     } else {  // results
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
         const int quarter = warp & 3, half = (warp - 4) >> 2;

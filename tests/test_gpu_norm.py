@@ -48,12 +48,12 @@ def _spread(gate, T):
     return gate.repeat_interleave(T // gate.shape[0], 0)
 
 
-def _check(c, scale=0.7, eps=1e-5, grads=True, call=None):
+def _check(c, scale=0.7, eps=1e-5, grads=True, learned=True):
     import sparsecore_b200 as sl
 
     names = [k for k in ("y", "r", "w", "b", "gate", "pw", "pb") if c[k] is not None]
     leaf = {k: c[k].clone().requires_grad_(grads) for k in names}
-    st = torch.full((1,), scale, device=dev(), requires_grad=grads)
+    st = torch.full((1,), scale, device=dev(), requires_grad=grads) if learned else scale
     gate, y, r = leaf.get("gate"), leaf["y"], leaf["r"]
     if gate is not None and gate.shape[0] != y.shape[0]:  # a gate per sequence, of as many equal sequences
         G = gate.shape[0]
@@ -64,7 +64,8 @@ def _check(c, scale=0.7, eps=1e-5, grads=True, call=None):
     assert out.dtype == c["r"].dtype and h.dtype == c["y"].dtype
     a = {k: c[k].double() for k in names}
     T, D = a["y"].shape
-    scale = float(st.detach())
+    if learned:
+        scale = float(st.detach())  # as held in 32 bits
     pn = pmag = torch.zeros_like(a["y"])
     u, umag, prstd = a["y"], a["y"].abs(), None
     if "pw" in a:
@@ -80,7 +81,8 @@ def _check(c, scale=0.7, eps=1e-5, grads=True, call=None):
     _within(h, href, href.abs() + a["w"].abs() * nmag)
     if not grads:
         return
-    got = dict(zip(names + ["scale"], torch.autograd.grad((out, h), [leaf[k] for k in names] + [st], (c["dout"], c["dh"]))))
+    named = {k: leaf[k] for k in names} | ({"scale": st} if learned else {})
+    got = dict(zip(named, torch.autograd.grad((out, h), list(named.values()), (c["dout"], c["dh"]))))
     do, dh = c["dout"].double(), c["dh"].double()
 
     def back(d, dmag, n, nmag, w, rstd):
@@ -98,7 +100,8 @@ def _check(c, scale=0.7, eps=1e-5, grads=True, call=None):
     _within(got["w"], (dh * n).sum(0), (dh.abs() * nmag).sum(0), rows)
     if "b" in a:
         _within(got["b"], dh.sum(0), dh.abs().sum(0), rows)
-    _within(got["scale"], (d * ga * u).sum().reshape(1), (dmag * ga.abs() * umag).sum().reshape(1), 64 + T + D)
+    if learned:
+        _within(got["scale"], (d * ga * u).sum().reshape(1), (dmag * ga.abs() * umag).sum().reshape(1), 64 + T + D)
     du, dumag = scale * d, scale * dmag
     if "gate" in a:
         G = a["gate"].shape[0]
@@ -117,6 +120,18 @@ def _check(c, scale=0.7, eps=1e-5, grads=True, call=None):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_widths(D, dtype):
     _check(_case(5, D, dtype, D, kind="rms" if D % 2 else "layer", post=D % 3 == 0, gate=(1,)))
+
+
+@gpu
+@pytest.mark.parametrize("D", [1, 5, 32, 96, 200, 384, 513, 768, 1000, 1024, 1280, 2048, 2500, 4096, 6000, 8192, 16384])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T", [3, 1337])
+def test_a_plain_residual_and_norm(D, dtype, T):
+    """Nothing after the block: the pass back that most models take, at every width it is spread differently."""
+    c = _case(T, D, dtype, D + T, kind="rms" if D % 5 == 0 else "layer")
+    _check(c, scale=1.0, learned=False)
+    if T == 3:
+        _check(c, scale=0.5, learned=False)
 
 
 @gpu

@@ -116,6 +116,7 @@ def test_pieces_of_the_vocabulary():
     """Enough tokens for the gradient to be taken in one large piece, and in several (planes above 512 MB)."""
     _check(*_case(17000, 40, 8300, torch.float32, 18))
     _check(*_case(40000, 33, 7001, torch.bfloat16, 19))
+    _check(*_case(17000, 256, 8300, torch.float32, 20))
     _check(*_case(9000, 64, 8300, torch.float32, 4))
     _check(*_case(20000, 40, 7000, torch.bfloat16, 5))
 
