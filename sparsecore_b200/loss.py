@@ -20,11 +20,9 @@ __all__ = ["linear_cross_entropy"]
 _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 
-def _args(x, weight, targets, ignore_index, reduction, train):
-    a = N.SlXentArgs(x.data_ptr(), weight.data_ptr(), targets.data_ptr())
-    a.tokens, a.dim, a.vocab = x.shape[0], x.shape[1], weight.shape[0]
-    a.ignore_index, a.dtype, a.reduction, a.train = ignore_index, N.DTYPES[x.dtype], reduction, train
-    return a
+def _args(x, weight, targets, loss, rows, prep, scratch, grad, dx, dw, ignore_index, reduction, train):
+    return N.SlXentArgs(x.data_ptr(), weight.data_ptr(), targets.data_ptr(), loss, rows, prep, scratch, grad, dx, dw,
+                        x.shape[0], x.shape[1], weight.shape[0], ignore_index, N.DTYPES[x.dtype], reduction, train)
 
 
 def _sizes(a):
@@ -42,27 +40,55 @@ def _forward(x, weight, targets, ignore_index, reduction, train):
     dim, dev = weight.shape[1], x.device
     x, weight, targets = x.reshape(-1, dim).contiguous(), weight.contiguous(), targets.reshape(-1).contiguous()
     T = x.shape[0]
-    a = _args(x, weight, targets, ignore_index, reduction, train)
     if reduction == 2:
         loss = torch.empty(T, dtype=torch.float32, device=dev)
-        a.loss_rows = loss.data_ptr()
     elif T:
         loss = torch.empty((), dtype=torch.float32, device=dev)
-        a.loss = loss.data_ptr()
     else:  # no tokens at all: the mean of nothing is NaN, their sum zero
         loss = torch.full((), 0.0 if reduction else float("nan"), device=dev)
     prep = None
     if T:
+        at = loss.data_ptr()
+        a = _args(x, weight, targets, None if reduction == 2 else at, at if reduction == 2 else None, None, None, None, None,
+                  None, ignore_index, reduction, train)
         sizes = _sizes(a)
-        prep, scratch = _buffer(sizes[0], dev), _buffer(sizes[1], dev)
-        a.prep, a.scratch = prep.data_ptr(), scratch.data_ptr()
+        if sizes[1] <= 1 << 20:  # one buffer for both, where keeping the scratch too costs little
+            prep = _buffer(sizes[0] + sizes[1], dev)
+            a.prep = prep.data_ptr()
+            a.scratch = a.prep + sizes[0]
+        else:
+            prep, scratch = _buffer(sizes[0], dev), _buffer(sizes[1], dev)
+            a.prep, a.scratch = prep.data_ptr(), scratch.data_ptr()
         N.call_on(dev, "sl_xent_forward", N.byref(a))
     return loss, (x, weight, targets, prep)
 
 
+def _backward(ctx, grad):
+    x, weight, targets, prep = ctx.saved_tensors
+    ignore_index, reduction, shape = ctx.opts
+    need = ctx.needs_input_grad
+    dev = x.device
+    dx = torch.empty(shape, dtype=x.dtype, device=dev) if need[0] else None
+    dw = torch.empty_like(weight) if need[1] else None
+    if prep is None:
+        return dx, None if dw is None else dw.zero_(), None, None, None
+    grad = grad.contiguous()
+    a = _args(x, weight, targets, None, None, prep.data_ptr(), None, grad.data_ptr(), None if dx is None else dx.data_ptr(),
+              None if dw is None else dw.data_ptr(), ignore_index, reduction, 1)
+    scratch = _buffer(_sizes(a)[2], dev)
+    a.scratch = scratch.data_ptr()
+    N.call_on(dev, "sl_xent_backward", N.byref(a))
+    return dx, dw, None, None, None
+
+
+_backward_once = once_differentiable(_backward)
+
+
 class _LinearCrossEntropyFunction(torch.autograd.Function):
-    """Inputs ``(x, weight, targets, ignore_index, reduction)``; returns the loss.  The operands' 16-bit planes, each row's maximum and its
-    sum are kept for the backward pass; the logits are made again there."""
+    """Inputs ``(x, weight, targets, ignore_index, reduction)``; returns the loss.
+    The operands' 16-bit planes, each row's maximum and its sum are kept for the
+    backward pass; the logits are made again there (of a vocabulary of one
+    tile their gradient is kept)."""
 
     @staticmethod
     def forward(ctx, x, weight, targets, ignore_index, reduction):
@@ -72,25 +98,8 @@ class _LinearCrossEntropyFunction(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
-        x, weight, targets, prep = ctx.saved_tensors
-        ignore_index, reduction, shape = ctx.opts
-        need = ctx.needs_input_grad
-        dx = torch.empty(shape, dtype=x.dtype, device=x.device) if need[0] else None
-        dw = torch.empty_like(weight) if need[1] else None
-        if prep is None:
-            return dx, None if dw is None else dw.zero_(), None, None, None
-        a = _args(x, weight, targets, ignore_index, reduction, 1)
-        grad = grad.contiguous()
-        scratch = _buffer(_sizes(a)[2], x.device)
-        a.prep, a.scratch, a.grad = prep.data_ptr(), scratch.data_ptr(), grad.data_ptr()
-        if dx is not None:
-            a.dx = dx.data_ptr()
-        if dw is not None:
-            a.dweight = dw.data_ptr()
-        N.call_on(x.device, "sl_xent_backward", N.byref(a))
-        return dx, dw, None, None, None
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, grad)
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100,
@@ -114,11 +123,11 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
             raise TypeError(f"linear_cross_entropy: {name} must be a torch.Tensor, got {type(t).__name__}")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise RuntimeError(f"linear_cross_entropy: x must be on a CUDA device (got device={x.device}). "
                            f"sparsecore_b200 has no CPU path.")
     for t, name in ((weight, "weight"), (targets, "targets")):
-        if t.device != x.device:
+        if t.get_device() != x.get_device():
             raise RuntimeError(f"linear_cross_entropy: {name} is on {t.device} but x is on {x.device}")
     if x.dtype not in N.DTYPES:
         raise ValueError(f"linear_cross_entropy: x must be float32, bfloat16 or float16, got {x.dtype}")

@@ -12,6 +12,8 @@ follows, so the stream is read and written once between two blocks.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -26,7 +28,7 @@ MAX_COLS = 16384
 def _vector(t, name, D, y):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"residual_norm: {name} must be a torch.Tensor, got {type(t).__name__}")
-    if t.device != y.device:
+    if t.get_device() != y.get_device():
         raise RuntimeError(f"residual_norm: {name} is on {t.device} but y is on {y.device}")
     if t.shape != (D,):
         raise ValueError(f"residual_norm: {name} must have shape ({D},), got {tuple(t.shape)}")
@@ -42,7 +44,13 @@ def _solid(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
 
-def _sizes(dtype, rdtype, weight, gate, scale_t, T, D, opts):
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(device, T, D, groups):
+    """A function of the sizes and of the device's SM count."""
+    return int(N.lib_on(device).sl_norm_workspace_bytes(T, D, groups))
+
+
+def _sizes(dtype, rdtype, weight, gate, T, D, opts):
     """The plain numbers of sl_norm_args."""
     kind, eps, post_eps, scale = opts
     kinds = N.DTYPES
@@ -52,16 +60,62 @@ def _sizes(dtype, rdtype, weight, gate, scale_t, T, D, opts):
 
 
 def _forward(y, residual, weight, bias, gate, scale_t, pw, pb, opts, keep_stats):
-    D = y.shape[-1]
+    D = weight.shape[0]
     T = y.numel() // D
-    y, residual, weight, bias, gate, pw, pb = (_solid(t) for t in (y, residual, weight, bias, gate, pw, pb))
+    y, residual, weight, bias, gate, pw, pb = map(_solid, (y, residual, weight, bias, gate, pw, pb))
     out, h = torch.empty_like(residual), torch.empty_like(y)
     stats = torch.empty(4 * T, dtype=torch.float32, device=y.device) if keep_stats else None
     a = N.SlNormArgs(y.data_ptr(), residual.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(gate), _ptr(pw), _ptr(pb),
                      out.data_ptr(), h.data_ptr(), _ptr(stats), _ptr(scale_t), None, None, None, None, None, None, None,
-                     None, None, None, None, *_sizes(y.dtype, residual.dtype, weight, gate, scale_t, T, D, opts))
+                     None, None, None, None, *_sizes(y.dtype, residual.dtype, weight, gate, T, D, opts))
     N.call_on(y.device, "sl_norm_forward", N.byref(a))
     return out, h, (y, weight, bias, gate, pw, pb, stats)
+
+
+def _backward(ctx, dout, dh):
+    dtype, opts, (has_bias, has_pb) = ctx.opts
+    if ctx.after:
+        y, out, weight, gate, scale_t, pw, pb, stats = ctx.saved_tensors
+    else:
+        out, weight, stats = ctx.saved_tensors
+        y = gate = scale_t = pw = pb = None
+    need = ctx.needs_input_grad
+    D, dev = weight.shape[0], out.device
+    T = out.numel() // D
+    dout = torch.zeros_like(out) if dout is None else _solid(dout)  # an output that nothing used
+    dh = torch.zeros(out.shape, dtype=dtype, device=dev) if dh is None else _solid(dh)
+    dr = torch.empty_like(out)
+    # Without a norm, a gate or a scale after the block both gradients are the same numbers.
+    same = not ctx.after and opts[3] == 1.0 and dtype == out.dtype
+    dy = torch.empty(out.shape, dtype=dtype, device=dev) if need[0] and not same else None
+    dw = torch.empty_like(weight) if need[2] else None
+    db = torch.empty_like(weight) if has_bias and need[3] else None
+    dgate = ds = dpw = dpb = None
+    if ctx.after:
+        dgate = torch.empty_like(gate) if gate is not None and need[4] else None
+        ds = torch.empty_like(scale_t) if scale_t is not None and need[5] else None
+        dpw = torch.empty_like(pw) if pw is not None and need[6] else None
+        dpb = torch.empty_like(pb) if has_pb and need[7] else None
+    if T:
+        sizes = _sizes(dtype, out.dtype, weight, gate, T, D, opts)
+        ws = torch.empty(_workspace_bytes(dev, T, D, sizes[2]), dtype=torch.uint8, device=dev)
+        w = weight.data_ptr()
+        # of the bias its presence is all that is asked for
+        a = N.SlNormArgs((out if y is None else y).data_ptr(), None, w, w if has_bias else None, _ptr(gate), _ptr(pw),
+                         _ptr(pb), out.data_ptr(), None, stats.data_ptr(), _ptr(scale_t), dout.data_ptr(), dh.data_ptr(),
+                         dr.data_ptr(), _ptr(dy), _ptr(dgate), _ptr(dw), _ptr(db), _ptr(dpw), _ptr(dpb), _ptr(ds),
+                         ws.data_ptr(), *sizes)
+        N.call_on(dev, "sl_norm_backward", N.byref(a))
+    else:
+        for t in (dw, db, dpw, dpb, dgate, ds):
+            if t is not None:
+                t.zero_()
+    if same and need[0]:
+        dy = dr
+    return dy, dr if need[1] else None, dw, db, dgate, ds, dpw, dpb, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class _ResidualNormFunction(torch.autograd.Function):
@@ -71,44 +125,20 @@ class _ResidualNormFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, y, residual, weight, bias, gate, scale_t, pw, pb, opts):
-        out, h, (y, weight, bias, gate, pw, pb, stats) = _forward(y, residual, weight, bias, gate, scale_t, pw, pb, opts, True)
-        plain = pw is None and gate is None and scale_t is None
-        ctx.save_for_backward(None if plain else y, out, weight, bias, gate, scale_t, pw, pb, stats)
-        ctx.opts = (y.dtype, opts)
+        dtype = y.dtype
+        out, h, (y, weight, _, gate, pw, pb, stats) = _forward(y, residual, weight, bias, gate, scale_t, pw, pb, opts, True)
+        ctx.after = pw is not None or gate is not None or scale_t is not None  # something after the block
+        if ctx.after:
+            ctx.save_for_backward(y, out, weight, gate, scale_t, pw, pb, stats)
+        else:
+            ctx.save_for_backward(out, weight, stats)
+        ctx.opts = (dtype, opts, (bias is not None, pb is not None))
         ctx.set_materialize_grads(False)
         return out, h
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout, dh):
-        y, out, weight, bias, gate, scale_t, pw, pb, stats = ctx.saved_tensors
-        dtype, opts = ctx.opts
-        need = ctx.needs_input_grad
-        D = out.shape[-1]
-        T = out.numel() // D
-        dev = out.device
-        dout = torch.zeros_like(out) if dout is None else _solid(dout)  # an output that nothing used
-        dh = torch.zeros(out.shape, dtype=dtype, device=dev) if dh is None else _solid(dh)
-        dr = torch.empty_like(out)
-        # Without a norm, a gate or a scale after the block both gradients are the same numbers.
-        same = pw is None and gate is None and scale_t is None and opts[3] == 1.0 and dtype == out.dtype
-        like = lambda t, i: torch.empty_like(t) if t is not None and need[i] else None  # noqa: E731
-        dy = torch.empty(out.shape, dtype=dtype, device=dev) if need[0] and not same else None
-        dw, db, dpw, dpb, dgate, ds = (like(t, i) for t, i in ((weight, 2), (bias, 3), (pw, 6), (pb, 7), (gate, 4), (scale_t, 5)))
-        if T:
-            sizes = _sizes(dtype, out.dtype, weight, gate, scale_t, T, D, opts)
-            ws = torch.empty(int(N.lib_on(dev).sl_norm_workspace_bytes(T, D, sizes[2])), dtype=torch.uint8, device=dev)
-            a = N.SlNormArgs((out if y is None else y).data_ptr(), None, weight.data_ptr(), _ptr(bias), _ptr(gate), _ptr(pw), _ptr(pb), out.data_ptr(),
-                             None, stats.data_ptr(), _ptr(scale_t), dout.data_ptr(), dh.data_ptr(), dr.data_ptr(), _ptr(dy),
-                             _ptr(dgate), _ptr(dw), _ptr(db), _ptr(dpw), _ptr(dpb), _ptr(ds), ws.data_ptr(), *sizes)
-            N.call_on(dev, "sl_norm_backward", N.byref(a))
-        else:
-            for t in (dw, db, dpw, dpb, dgate, ds):
-                if t is not None:
-                    t.zero_()
-        if same and need[0]:
-            dy = dr
-        return dy, dr if need[1] else None, dw, db, dgate, ds, dpw, dpb, None
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dout, dh)
 
 
 def residual_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -136,19 +166,21 @@ def residual_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
             raise TypeError(f"residual_norm: {name} must be a torch.Tensor, got {type(t).__name__}")
     if kind not in _KINDS:
         raise ValueError(f"residual_norm: kind must be 'layer' or 'rms', got {kind!r}")
-    if y.device.type != "cuda":
+    if not y.is_cuda:
         raise RuntimeError(f"residual_norm: y must be on a CUDA device (got device={y.device}). "
                            f"sparsecore_b200 has no CPU path.")
-    if residual.device != y.device:
+    if residual.get_device() != y.get_device():
         raise RuntimeError(f"residual_norm: residual is on {residual.device} but y is on {y.device}")
-    if y.dtype not in N.DTYPES:
-        raise ValueError(f"residual_norm: y must be float32, bfloat16 or float16, got {y.dtype}")
-    if residual.dtype not in (y.dtype, torch.float32):
-        raise ValueError(f"residual_norm: residual must be {y.dtype} or torch.float32, got {residual.dtype}")
-    if y.dim() < 1 or y.shape != residual.shape:
-        raise ValueError(f"residual_norm: y and residual must have one shape [..., D], got {tuple(y.shape)} "
+    dtype = y.dtype
+    if dtype not in N.DTYPES:
+        raise ValueError(f"residual_norm: y must be float32, bfloat16 or float16, got {dtype}")
+    if residual.dtype not in (dtype, torch.float32):
+        raise ValueError(f"residual_norm: residual must be {dtype} or torch.float32, got {residual.dtype}")
+    shape = y.shape
+    if not shape or shape != residual.shape:
+        raise ValueError(f"residual_norm: y and residual must have one shape [..., D], got {tuple(shape)} "
                          f"and {tuple(residual.shape)}")
-    D = y.shape[-1]
+    D = shape[-1]
     if not 1 <= D <= MAX_COLS:
         raise ValueError(f"residual_norm: the last dimension must be 1 to {MAX_COLS}, got {D}")
     _vector(weight, "weight", D, y)
@@ -172,11 +204,11 @@ def residual_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
         if gate.dim() < 1 or gate.shape[-1] != D:
             raise ValueError(f"residual_norm: gate's last dimension must be {D}, got shape {tuple(gate.shape)}")
         groups = gate.numel() // D
-        shape = tuple(gate.shape)
-        whole = shape == tuple(y.shape)
-        runs = gate.dim() == y.dim() and shape[0] == y.shape[0] and all(n == 1 for n in shape[1:-1])
+        got = tuple(gate.shape)
+        whole = got == tuple(shape)
+        runs = len(got) == len(shape) and got[0] == shape[0] and all(n == 1 for n in got[1:-1])
         if not (groups == 1 or whole or runs):
-            raise ValueError(f"residual_norm: gate of shape {shape} is not [D], y's shape {tuple(y.shape)}, or "
+            raise ValueError(f"residual_norm: gate of shape {got} is not [D], y's shape {tuple(shape)}, or "
                              f"[y.shape[0], 1, ..., D]")
     scale_t = None
     if isinstance(scale, torch.Tensor):
