@@ -696,6 +696,252 @@ norm_bwd_full_kernel(Args<TY, TR> a, int stages) {
     }
 }
 
+// The same where all rows of a CTA share their gate (or have none), as almost
+// always.  What lies behind the stream is then one vector, q = scale gate pw,
+// and every gradient of the vectors follows from two sums a column over the
+// rows, d yhat and d, multiplied out once at the end:
+//   dpw = scale gate S1, dpb = scale gate S0, dgate = scale (pw S1 + pb S0),
+//   dscale = sum of gate (pw S1 + pb S0).
+// yhat = y where there is no norm behind the block.  Fewer sums, vectors and
+// operations a row (46 instructions an element instead of 53): 8191 x 4096
+// bf16 with both norms and a gate a channel take 92 us instead of 100.
+template <typename TY, typename TR, int VE, int NV, bool POST, bool L>
+__global__ void __launch_bounds__(kMaxThreads)
+norm_bwd_shared_kernel(Args<TY, TR> a, int stages) {
+    constexpr int Q = L && POST ? 2 : 1;
+    constexpr int kT = VE * sizeof(TY) / 16, kR = VE * sizeof(TR) / 16;  // granules of a vector
+    constexpr int kVec = NV * VE / 4;
+    constexpr int oX = 0, oN = NV * kR, oD = NV * (kR + kT), oY = NV * (2 * kR + kT), kGranules = NV * 2 * (kR + kT);
+    __shared__ float4 ws[2][Q][32];
+    extern __shared__ __align__(16) char mem[];
+    const int warps = blockDim.x >> 5, cols = static_cast<int>(a.D);
+    const int col = threadIdx.x * VE, step = blockDim.x * VE;
+    const float inv_d = 1.f / static_cast<float>(cols);
+    const float scale = a.scale_dev ? *a.scale_dev : a.scale;
+    float aw[NV][VE] = {}, s1[NV][VE] = {}, ab[L ? NV : 1][VE] = {}, s0[L ? NV : 1][VE] = {};
+    int64_t t0, t1;
+    my_rows(a, blockIdx.x, t0, t1);
+    const int64_t gate_row = a.seg > 0 ? blockIdx.x / a.seg * a.D : 0;
+
+    const int lap = blockDim.x * 16;
+    char* const mine = mem + threadIdx.x * 16;
+    const int stage_bytes = kGranules * lap;
+    char* const vectors = mine + stages * stage_bytes;
+    auto keep = [&](int which, int j, const float (&o)[VE]) {
+#pragma unroll
+        for (int q = 0; q < VE / 4; ++q)
+            *reinterpret_cast<float4*>(vectors + (which * kVec + j * (VE / 4) + q) * lap) = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+    };
+    auto kept = [&](int which, int j, float (&o)[VE]) {
+#pragma unroll
+        for (int q = 0; q < VE / 4; ++q) {
+            const float4 f = *reinterpret_cast<const float4*>(vectors + (which * kVec + j * (VE / 4) + q) * lap);
+            o[4 * q] = f.x; o[4 * q + 1] = f.y; o[4 * q + 2] = f.z; o[4 * q + 3] = f.w;
+        }
+    };
+    auto fetch = [&](int64_t t, int stage) {
+        char* const to = mine + stage * stage_bytes;
+        if (t < t1) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = col + j * step;
+                if (c >= cols) continue;
+                const int64_t i = t * a.D + c;
+                auto put = [&](int at, const void* src, int size) {
+#pragma unroll
+                    for (int q = 0; q < size; ++q) copy16(to + (at + j * size + q) * lap, static_cast<const char*>(src) + 16 * q);
+                };
+                put(oX, a.out + i, kR);
+                put(oN, a.dh + i, kT);
+                put(oD, a.dout + i, kR);
+                put(oY, a.y + i, kT);
+            }
+        }
+        copies_commit();
+    };
+    auto get = [&](auto type, int at, const char* held, int j, float (&o)[VE]) {
+        using T = decltype(type);
+        constexpr int size = VE * sizeof(T) / 16;
+        Pack<T, VE> p;
+#pragma unroll
+        for (int q = 0; q < size; ++q) reinterpret_cast<uint4*>(&p)[q] = *reinterpret_cast<const uint4*>(held + (at + j * size + q) * lap);
+        unpack(p, o);
+    };
+    const bool sums_dy = POST && a.need_dy;
+    auto sums = [&](const float4& st, const char* held, float4 (*to)[32]) {
+        Sum p[4 * Q];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            if (col + j * step >= cols) continue;
+            float x[VE], g[VE], w[VE];
+            get(TR{}, oX, held, j, x);
+            get(TY{}, oN, held, j, g);
+            kept(0, j, w);
+            vfma(x, x, st.x, st.y);
+            vmul(g, g, w);
+            p[0].template fma<VE>(g, x);
+            if (L) p[1].add(g);
+            if (sums_dy) {
+                float q[VE], y[VE], d[VE];
+                kept(1, j, q);
+                get(TR{}, oD, held, j, d);
+                get(TY{}, oY, held, j, y);
+                vfma(y, y, st.z, st.w);
+                vmul(y, y, q);
+                vfma(d, g, st.x, d);
+                p[2].template fma<VE>(y, d);
+                p[3].template fma<VE>(y, x);
+                if constexpr (Q == 2) {
+                    p[4].add(y);
+                    p[5].template fma<VE>(q, d);
+                    p[6].template fma<VE>(q, x);
+                    p[7].add(q);
+                }
+            }
+        }
+        float s[4 * Q];
+#pragma unroll
+        for (int k = 0; k < 4 * Q; ++k) s[k] = p[k].total();
+        sums_put<Q>(s, to);
+    };
+
+    if (t0 < t1) {
+        for (int k = 0; k < stages - 1; ++k) fetch(t0 + k, k);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = col + j * step;
+            if (c >= cols) continue;
+            float o[VE], g[VE];
+            load_v<TY, VE>(a.w, a.vec_f32, c, o);
+            keep(0, j, o);
+#pragma unroll
+            for (int k = 0; k < VE; ++k) o[k] = scale;
+            if (POST) {
+                load_v<TY, VE>(a.pw, a.vec_f32, c, g);
+                vmul(o, o, g);
+            }
+            if (a.gate) {
+                load_v<TY, VE>(a.gate, a.gate_f32, gate_row + c, g);
+                vmul(o, o, g);
+            }
+            keep(1, j, o);
+        }
+        copies_wait(stages - 2);
+        float4 st = a.stats[t0];
+        int stage = 0, flip = 0;
+        sums(st, mine, ws[0]);
+        for (int64_t t = t0; t < t1; ++t) {
+            const char* const held = mine + stage * stage_bytes;
+            const int after = stage + 1 == stages ? 0 : stage + 1;
+            fetch(t + stages - 1, stage == 0 ? stages - 1 : stage - 1);
+            copies_wait(stages - 2);  // row t + 1 is here
+            const float4 next = a.stats[min(t + 1, t1 - 1)];
+            if (warps > 1) __syncthreads();
+            else __syncwarp();
+            float s[4 * Q];
+            sums_get<Q>(s, warps, ws[flip]);
+            flip ^= 1;
+            if (t + 1 < t1) sums(next, mine + after * stage_bytes, ws[flip]);
+            const float c2 = s[0] * inv_d, c1 = L && a.layer ? s[1] * inv_d : 0.f;
+            float e1 = 0.f, e2 = 0.f;
+            if (POST) {
+                e2 = s[2] - st.x * c2 * s[3];
+                if constexpr (Q == 2) {
+                    e2 -= st.x * c1 * s[4];
+                    e1 = a.layer ? (s[5] - st.x * (c2 * s[6] + c1 * s[7])) * inv_d : 0.f;
+                }
+                e2 *= inv_d;
+            }
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = col + j * step;
+                if (c >= cols) continue;
+                const int64_t at = t * a.D + c;
+                float x[VE], g[VE], d[VE], w[VE], y[VE];
+                get(TR{}, oX, held, j, x);
+                get(TY{}, oN, held, j, g);
+                get(TR{}, oD, held, j, d);
+                kept(0, j, w);
+                vfma(x, x, st.x, st.y);
+                vfma(aw[j], g, x, aw[j]);
+                if (L) vadd(ab[j], ab[j], g);
+                if (L) vfma(x, x, -c2, -c1);
+                else vmul(x, x, -c2);
+                vfma(g, g, w, x);
+                vfma(d, g, st.x, d);
+                store_f<TR, VE>(a.dr + at, d);
+                get(TY{}, oY, held, j, y);
+                if (POST) vfma(y, y, st.z, st.w);
+                vfma(s1[j], d, y, s1[j]);
+                if (L) vadd(s0[j], s0[j], d);
+                if (a.need_dy) {
+                    kept(1, j, w);
+                    if (POST) {
+                        if (L) vfma(y, y, -e2, -e1);
+                        else vmul(y, y, -e2);
+                        vfma(d, d, w, y);
+                        vmul(d, d, st.z);
+                    } else {
+                        vmul(d, d, w);
+                    }
+                    store_f<TY, VE>(a.dy + at, d);
+                }
+            }
+            st = next;
+            stage = after;
+        }
+    }
+    const int64_t plane = a.ctas * a.D;
+    float as = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = col + j * step;
+        if (c >= cols) continue;
+        float* part = a.part + blockIdx.x * a.D + c;
+        store_f<float, VE>(part, aw[j]);
+        if constexpr (L) store_f<float, VE>(part + plane, ab[j]);
+        float g[VE], u[VE], o[VE];
+#pragma unroll
+        for (int k = 0; k < VE; ++k) g[k] = 1.f;
+        if (a.gate) load_v<TY, VE>(a.gate, a.gate_f32, gate_row + c, g);
+        if constexpr (POST) {
+            vmul(o, g, s1[j]);
+            vmul(o, o, scale);
+            store_f<float, VE>(part + 2 * plane, o);
+            if constexpr (L) {
+                vmul(o, g, s0[j]);
+                vmul(o, o, scale);
+                store_f<float, VE>(part + 3 * plane, o);
+            }
+            load_v<TY, VE>(a.pw, a.vec_f32, c, o);
+            vmul(u, o, s1[j]);
+            if constexpr (L) {
+                if (a.pb) {
+                    load_v<TY, VE>(a.pb, a.vec_f32, c, o);
+                    vfma(u, o, s0[j], u);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < VE; ++k) u[k] = s1[j][k];
+        }
+#pragma unroll
+        for (int k = 0; k < VE; ++k) as = fmaf(g[k], u[k], as);
+        if (a.need_gate) {
+            vmul(u, u, scale);
+            store_f<float, VE>(part + 4 * plane, u);
+        }
+    }
+    if (a.need_scale) {
+        float z[4 * Q] = {as};
+        __syncthreads();
+        sums_put<Q>(z, ws[0]);
+        __syncthreads();
+        sums_get<Q>(z, warps, ws[0]);
+        if (threadIdx.x == 0) a.part_s[blockIdx.x] = z[0];
+    }
+}
+
 // dst[g][c] = sum over the CTAs of run g of part[cta][c]: 32 columns a CTA,
 // 32 rows of threads striding over the CTAs, joined in a fixed order.
 struct Reduce {
@@ -834,9 +1080,11 @@ int backward(const sl_norm_args& n, cudaStream_t s) {
             using G = Ring<TY, TR, ve, nv>;
             size_t bytes = 0;
             int stages = 1;
+            // Gates of whole runs of rows: one run a CTA (always so where its gradient is asked for).
+            const bool shared = !n.gate || (a.gate_rows > 1 && (a.gate_rows == a.T || sp.seg > 0));
             if constexpr (ring) {  // this row, the next, and one or two on their way
-                const size_t lap = 16 * block.x, stage = G::granules(G::kGates && n.gate && a.gate_rows == 1 && !a.gate_f32) * lap;
-                bytes = G::kVectors ? 4 * G::kVec * lap : 0;
+                const size_t lap = 16 * block.x, stage = G::granules(!shared && G::kGates && a.gate_rows == 1 && !a.gate_f32) * lap;
+                bytes = (shared ? 2 : G::kVectors ? 4 : 0) * G::kVec * lap;
                 stages = static_cast<int>(std::min<size_t>(4, (kFullSmem - bytes) / stage));
                 if (stages < 3) return fail(SL_ERR_UNSUPPORTED, "sl_norm_backward: rows do not fit");
                 bytes += stages * stage;
@@ -850,6 +1098,10 @@ int backward(const sl_norm_args& n, cudaStream_t s) {
                 return static_cast<int>(SL_OK);
             };
             const bool l = a.layer || n.bias || n.post_bias;
+            if constexpr (ring) {
+                if (shared && n.post_weight) return l ? go(norm_bwd_shared_kernel<TY, TR, ve, nv, true, true>) : go(norm_bwd_shared_kernel<TY, TR, ve, nv, true, false>);
+                if (shared) return l ? go(norm_bwd_shared_kernel<TY, TR, ve, nv, false, true>) : go(norm_bwd_shared_kernel<TY, TR, ve, nv, false, false>);
+            }
             if (n.post_weight) return l ? go(norm_bwd_full_kernel<TY, TR, ve, nv, true, true, ring>) : go(norm_bwd_full_kernel<TY, TR, ve, nv, true, false, ring>);
             return l ? go(norm_bwd_full_kernel<TY, TR, ve, nv, false, true, ring>) : go(norm_bwd_full_kernel<TY, TR, ve, nv, false, false, ring>);
         });

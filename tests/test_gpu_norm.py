@@ -145,8 +145,27 @@ def test_rows(T, post, kind):
 @gpu
 @pytest.mark.parametrize("groups", [1, 2, 6, 40, 600, 1200])
 @pytest.mark.parametrize("D", [96, 50])
-def test_gates_shared_by_runs_of_rows(groups, D):
-    _check(_case(1200, D, torch.float32, groups, gate=(groups,), post=True))
+@pytest.mark.parametrize("post", [True, False])
+def test_gates_shared_by_runs_of_rows(groups, D, post):
+    c = _case(1200, D, torch.float32, groups, gate=(groups,), post=post)
+    _check(c)
+    _check(c, scale=0.5, learned=False)
+    _check({k: v.bfloat16() if torch.is_tensor(v) else v for k, v in c.items()} | {"kind": "rms"})
+
+
+@gpu
+@pytest.mark.parametrize("groups", [1, 4, 600, 1200])
+def test_a_gate_that_asks_for_no_gradient(groups):
+    """Then a CTA's rows may cross from one sequence's gate to the next."""
+    import sparsecore_b200 as sl
+
+    c = _case(1200, 96, torch.float32, groups + 7, gate=(groups,))
+    y, r, w = (c[k].clone().requires_grad_() for k in ("y", "r", "w"))
+    S = 1200 // groups
+    gate = c["gate"][:, None] if groups > 1 else c["gate"][0]
+    out, h = sl.residual_norm(y.view(groups, S, 96), r.view(groups, S, 96), w, gate=gate, kind="rms")
+    gy, gr, gw = torch.autograd.grad((out, h), (y, r, w), (c["dout"].view(groups, S, 96), c["dh"].view(groups, S, 96)))
+    _within(gy, gr.double() * _spread(c["gate"].double(), 1200), gr.double().abs() * _spread(c["gate"].double(), 1200).abs())
 
 
 @gpu
