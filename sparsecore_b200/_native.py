@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -39,26 +40,15 @@ class SlCsr(ctypes.Structure):
     ]
 
 
-class SlNormArgs(ctypes.Structure):
-    """Mirror of `sl_norm_args`."""
-
-    _fields_ = ([(n, P) for n in ("y", "residual", "weight", "bias", "gate", "post_weight", "post_bias", "out", "h",
-                                  "stats", "scale_dev", "dout", "dh", "dresidual", "dy", "dgate", "dweight", "dbias",
-                                  "dpost_weight", "dpost_bias", "dscale", "workspace")]
-                + [(n, I64) for n in ("rows", "cols", "gate_groups")] + [(n, F32) for n in ("scale", "eps", "post_eps")]
-                + [(n, I32) for n in ("kind", "dtype", "residual_dtype", "weight_dtype", "gate_dtype")])
-
-
-class SlXentArgs(ctypes.Structure):
-    """Mirror of `sl_xent_args`."""
-
-    _fields_ = ([(n, P) for n in ("x", "weight", "targets", "loss", "loss_rows", "prep", "scratch", "grad", "dx", "dweight")]
-                + [(n, I64) for n in ("tokens", "dim", "vocab", "ignore_index")] + [("dtype", I32), ("reduction", I32), ("train", I32)])
+# Mirrors of `sl_norm_args` and `sl_xent_args` (fields in the header's order, a
+# missing pointer 0).  Their packed bytes are passed as they are: making them
+# takes half the time of a ctypes structure.
+NORM_ARGS = struct.Struct("@22P3q3f5i")
+XENT_ARGS = struct.Struct("@10P4q3i4x")
 
 
 # Element types of the training step's dense operators (SL_F32 ...).
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-byref = ctypes.byref
 
 # name -> (restype, argtypes); every symbol the header declares.
 SIGNATURES: dict[str, tuple] = {

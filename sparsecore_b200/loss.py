@@ -9,6 +9,7 @@ time.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -21,15 +22,25 @@ _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 
 def _args(x, weight, targets, loss, rows, prep, scratch, grad, dx, dw, ignore_index, reduction, train):
-    return N.SlXentArgs(x.data_ptr(), weight.data_ptr(), targets.data_ptr(), loss, rows, prep, scratch, grad, dx, dw,
-                        x.shape[0], x.shape[1], weight.shape[0], ignore_index, N.DTYPES[x.dtype], reduction, train)
+    """The bytes of sl_xent_args; pointers as numbers, 0 where there is none."""
+    return N.XENT_ARGS.pack(x.data_ptr(), weight.data_ptr(), targets.data_ptr(), loss, rows, prep, scratch, grad, dx, dw,
+                            x.shape[0], x.shape[1], weight.shape[0], ignore_index, N.DTYPES[x.dtype], reduction, train)
 
 
-def _sizes(a):
+@functools.lru_cache(maxsize=256)
+def _sizes_of(tokens, dim, vocab, dtype, reduction, train, x_off, w_off):
     out = (ctypes.c_int64 * 3)()
     at = ctypes.addressof(out)
-    N.call("sl_xent_sizes", N.byref(a), at, at + 8, at + 16)
-    return out
+    a = N.XENT_ARGS.pack(x_off, w_off, 0, 0, 0, 0, 0, 0, 0, 0, tokens, dim, vocab, 0, dtype, reduction, train)
+    N.call("sl_xent_sizes", a, at, at + 8, at + 16)
+    return tuple(out)
+
+
+def _sizes(x, weight, reduction, train):
+    """Bytes of the kept buffer, the forward and the backward call's scratch: they depend on the sizes, the
+    type and on where the operands start within 16 bytes."""
+    return _sizes_of(x.shape[0], x.shape[1], weight.shape[0], N.DTYPES[x.dtype], reduction, train, x.data_ptr() & 15,
+                     weight.data_ptr() & 15)
 
 
 def _buffer(n, device):
@@ -48,18 +59,16 @@ def _forward(x, weight, targets, ignore_index, reduction, train):
         loss = torch.full((), 0.0 if reduction else float("nan"), device=dev)
     prep = None
     if T:
-        at = loss.data_ptr()
-        a = _args(x, weight, targets, None if reduction == 2 else at, at if reduction == 2 else None, None, None, None, None,
-                  None, ignore_index, reduction, train)
-        sizes = _sizes(a)
-        if sizes[1] <= 1 << 20:  # one buffer for both, where keeping the scratch too costs little
-            prep = _buffer(sizes[0] + sizes[1], dev)
-            a.prep = prep.data_ptr()
-            a.scratch = a.prep + sizes[0]
+        kept, scratch, _ = _sizes(x, weight, reduction, train)
+        if scratch <= 1 << 20:  # one buffer for both, where keeping the scratch too costs little
+            prep = _buffer(kept + scratch, dev)
+            at = prep.data_ptr() + kept
         else:
-            prep, scratch = _buffer(sizes[0], dev), _buffer(sizes[1], dev)
-            a.prep, a.scratch = prep.data_ptr(), scratch.data_ptr()
-        N.call_on(dev, "sl_xent_forward", N.byref(a))
+            prep, buf = _buffer(kept, dev), _buffer(scratch, dev)
+            at = buf.data_ptr()
+        to = loss.data_ptr()
+        N.call_on(dev, "sl_xent_forward", _args(x, weight, targets, 0 if reduction == 2 else to, to if reduction == 2 else 0,
+                                                prep.data_ptr(), at, 0, 0, 0, ignore_index, reduction, train))
     return loss, (x, weight, targets, prep)
 
 
@@ -73,11 +82,10 @@ def _backward(ctx, grad):
     if prep is None:
         return dx, None if dw is None else dw.zero_(), None, None, None
     grad = grad.contiguous()
-    a = _args(x, weight, targets, None, None, prep.data_ptr(), None, grad.data_ptr(), None if dx is None else dx.data_ptr(),
-              None if dw is None else dw.data_ptr(), ignore_index, reduction, 1)
-    scratch = _buffer(_sizes(a)[2], dev)
-    a.scratch = scratch.data_ptr()
-    N.call_on(dev, "sl_xent_backward", N.byref(a))
+    scratch = _buffer(_sizes(x, weight, reduction, 1)[2], dev)
+    N.call_on(dev, "sl_xent_backward", _args(x, weight, targets, 0, 0, prep.data_ptr(), scratch.data_ptr(), grad.data_ptr(),
+                                             0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
+                                             ignore_index, reduction, 1))
     return dx, dw, None, None, None
 
 

@@ -37,11 +37,11 @@ def _vector(t, name, D, y):
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _solid(t):
-    return t if t is None or t.is_contiguous() else t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 @functools.lru_cache(maxsize=256)
@@ -62,13 +62,14 @@ def _sizes(dtype, rdtype, weight, gate, T, D, opts):
 def _forward(y, residual, weight, bias, gate, scale_t, pw, pb, opts, keep_stats):
     D = weight.shape[0]
     T = y.numel() // D
-    y, residual, weight, bias, gate, pw, pb = map(_solid, (y, residual, weight, bias, gate, pw, pb))
+    y, residual, weight = _solid(y), _solid(residual), _solid(weight)
+    bias, gate, pw, pb = (t if t is None else _solid(t) for t in (bias, gate, pw, pb))
     out, h = torch.empty_like(residual), torch.empty_like(y)
     stats = torch.empty(4 * T, dtype=torch.float32, device=y.device) if keep_stats else None
-    a = N.SlNormArgs(y.data_ptr(), residual.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(gate), _ptr(pw), _ptr(pb),
-                     out.data_ptr(), h.data_ptr(), _ptr(stats), _ptr(scale_t), None, None, None, None, None, None, None,
-                     None, None, None, None, *_sizes(y.dtype, residual.dtype, weight, gate, T, D, opts))
-    N.call_on(y.device, "sl_norm_forward", N.byref(a))
+    a = N.NORM_ARGS.pack(y.data_ptr(), residual.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(gate), _ptr(pw), _ptr(pb),
+                         out.data_ptr(), h.data_ptr(), _ptr(stats), _ptr(scale_t), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                         *_sizes(y.dtype, residual.dtype, weight, gate, T, D, opts))
+    N.call_on(y.device, "sl_norm_forward", a)
     return out, h, (y, weight, bias, gate, pw, pb, stats)
 
 
@@ -101,11 +102,11 @@ def _backward(ctx, dout, dh):
         ws = torch.empty(_workspace_bytes(dev, T, D, sizes[2]), dtype=torch.uint8, device=dev)
         w = weight.data_ptr()
         # of the bias its presence is all that is asked for
-        a = N.SlNormArgs((out if y is None else y).data_ptr(), None, w, w if has_bias else None, _ptr(gate), _ptr(pw),
-                         _ptr(pb), out.data_ptr(), None, stats.data_ptr(), _ptr(scale_t), dout.data_ptr(), dh.data_ptr(),
-                         dr.data_ptr(), _ptr(dy), _ptr(dgate), _ptr(dw), _ptr(db), _ptr(dpw), _ptr(dpb), _ptr(ds),
-                         ws.data_ptr(), *sizes)
-        N.call_on(dev, "sl_norm_backward", N.byref(a))
+        a = N.NORM_ARGS.pack((out if y is None else y).data_ptr(), 0, w, w if has_bias else 0, _ptr(gate), _ptr(pw),
+                             _ptr(pb), out.data_ptr(), 0, stats.data_ptr(), _ptr(scale_t), dout.data_ptr(),
+                             dh.data_ptr(), dr.data_ptr(), _ptr(dy), _ptr(dgate), _ptr(dw), _ptr(db), _ptr(dpw),
+                             _ptr(dpb), _ptr(ds), ws.data_ptr(), *sizes)
+        N.call_on(dev, "sl_norm_backward", a)
     else:
         for t in (dw, db, dpw, dpb, dgate, ds):
             if t is not None:
@@ -218,8 +219,10 @@ def residual_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
             raise ValueError("residual_norm: a tensor scale must be one float32 element")
         scale, scale_t = 1.0, scale
     opts = (_KINDS[kind], eps, post_eps, float(scale))
-    if torch.is_grad_enabled() and (y.requires_grad or residual.requires_grad or weight.requires_grad
-                                    or any(t is not None and t.requires_grad
-                                           for t in (bias, gate, scale_t, post_weight, post_bias))):
+    if torch.is_grad_enabled() and (
+            y.requires_grad or residual.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+            or (gate is not None and gate.requires_grad) or (scale_t is not None and scale_t.requires_grad)
+            or (post_weight is not None and post_weight.requires_grad)
+            or (post_bias is not None and post_bias.requires_grad)):
         return _ResidualNormFunction.apply(y, residual, weight, bias, gate, scale_t, post_weight, post_bias, opts)
     return _forward(y, residual, weight, bias, gate, scale_t, post_weight, post_bias, opts, False)[:2]
