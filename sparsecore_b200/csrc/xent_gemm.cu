@@ -547,11 +547,17 @@ join_kernel(Problem p, Output o, int64_t M, int64_t N, int64_t stride, int64_t s
         const int64_t m = i / across;
         const float* q = o.slabs + m * stride + (i - m * across);
         float v[W] = {}, f[W];
-#pragma unroll 8
-        for (int s = 0; s < splits; ++s) {
-            load_f<float, W>(q + s * slab, f);
+        for (int s0 = 0; s0 < splits; s0 += 8) {  // eight loads under way
+            float g[8][W];
 #pragma unroll
-            for (int k = 0; k < W; ++k) v[k] += f[k];
+            for (int s = 0; s < 8; ++s)
+                if (s0 + s < splits) load_f<float, W>(q + (s0 + s) * slab, g[s]);
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+                if (s0 + s < splits) {
+#pragma unroll
+                    for (int k = 0; k < W; ++k) v[k] += g[s][k];
+                }
         }
         if (o.acc) {
             if (!o.first) {
@@ -607,7 +613,8 @@ int run(Args& a, const Operand& A, const Operand& B, cudaStream_t s) {
     if (int rc = a.p.f32 ? launch<2, MODE>(A, B, a, s) : launch<1, MODE>(A, B, a, s)) return rc;
     if (a.splits > 1) {
         const int64_t stride = static_cast<int64_t>(a.tiles_n) * kTile;
-        const int w = a.N % 4 == 0 ? 4 : 1;
+        // four columns a thread where that still fills the GPU
+        const int w = a.N % 4 == 0 && a.M * a.N >= num_sms() * 2048 ? 4 : 1;
         const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((a.M * a.N / w + 255) / 256, num_sms() * 16));
         if (w == 4) join_kernel<4><<<blocks, 256, 0, s>>>(a.p, a.o, a.M, a.N, stride, a.slab_stride, a.splits, a.p.f32);
         else join_kernel<1><<<blocks, 256, 0, s>>>(a.p, a.o, a.M, a.N, stride, a.slab_stride, a.splits, a.p.f32);
