@@ -146,7 +146,8 @@ __device__ __forceinline__ int64_t gate_offset(const A& a, int64_t t) {
 // lane, without a barrier; more warps a row beyond.  A CTA takes row after
 // row; as many CTAs as an SM holds.  TV: type of the vectors (asked for at run
 // time it cost 10 of 73 us on 8191 x 4096 bf16 rows with a norm on both sides,
-// 63 us of 41 for 268 MB, bound by instructions: 45 an element).  16384 x 768
+// 57 us now, of 41 for 268 MB: 34 instructions an element, issued in 61 % of the
+// clocks; one barrier a norm instead of two changed nothing).  16384 x 768
 // fp32: 33 us of 31 for 201 MB, bound by memory.
 template <typename TY, typename TR, typename TV, int VE, int NV, bool POST>
 __global__ void __launch_bounds__(kMaxThreads, VE * NV <= 16 ? 2 : 1)
@@ -420,9 +421,10 @@ struct Ring {
 // Between two barriers a warp has the sums of the next row and the results
 // of this one to work on, which hide each other's latencies.
 //
-// 8191 x 4096 bf16 with both norms and a gate a channel: 100 us of 62 for its
-// 403 MB; 220 us with two barriers a row and no ring, 121 us before the next
-// row's sums were taken beside this row's results.  Bound by the latency of
+// 8191 x 4096 bf16 with both norms and a gate a channel (which has a kernel of
+// its own below): 100 us of 62 for its 403 MB; 220 us with two barriers a row
+// and no ring, 121 us before the next row's sums were taken beside this row's
+// results.  Bound by the latency of
 // sixteen warps with one row under way (the scheduler issues in half of the
 // clocks).  L: LayerNorm, or a bias.
 template <typename TY, typename TR, int VE, int NV, bool POST, bool L, bool RING>

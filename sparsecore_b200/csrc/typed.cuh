@@ -71,7 +71,9 @@ __device__ __forceinline__ Pack<T, N> pack(const float (&in)[N]) {
 
 template <typename T, int N>
 __device__ __forceinline__ void load_f(const T* src, float (&out)[N]) {
-    unpack(*reinterpret_cast<const Pack<T, N>*>(src), out);
+    // a copy first: taken apart where they lie, 16-bit values come in words of 4 bytes
+    const Pack<T, N> q = *reinterpret_cast<const Pack<T, N>*>(src);
+    unpack(q, out);
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_f(T* dst, const float (&in)[N]) {

@@ -281,7 +281,7 @@ bool copies_x(const sl_xent_args& a) { return a.train || a.dtype == SL_F32 || a.
 // A vocabulary of one tile: the forward pass has a row's logits together and
 // leaves G (of all tokens: at most 256 columns) for the backward pass, which
 // then has no logits to make again.  Single losses' gradients are not known
-// in time.  16384 x 768 x 256 fp32: two launches less and 153 -> 120 us.
+// in time.  16384 x 768 x 256 fp32: two launches less and 153 -> 134 us.
 bool one_tile(const sl_xent_args& a) {
     return a.vocab <= kOneTile && copies_x(a) && !(a.train && a.reduction == SL_XENT_NONE);
 }
