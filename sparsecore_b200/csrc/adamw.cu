@@ -17,7 +17,7 @@
 // 32-bit moments are bound by memory: 12.2 M weights in padded arrays (32
 // bytes a slot, padding read too) take 67 us, 5.8 TB/s.  8-bit ones are bound
 // by instructions, about 65 an element, half of them integer and logic ones
-// for the dither: 335 M bf16 weights take 0.89 ms where their 10 bytes each
+// for the dither: 335 M bf16 weights take 0.88 ms where their 10 bytes each
 // would take 0.52.
 #include <cuda_fp8.h>
 

@@ -108,6 +108,8 @@ __device__ __forceinline__ unsigned finite_bits(float v) {
 __global__ void __launch_bounds__(kThreads)
 absmax_kernel(Source q, int x_blocks, unsigned* part, int vec) {
     __shared__ unsigned s[kThreads / 32];
+    let_follow();
+    follow();
     const bool is_w = blockIdx.x >= x_blocks;
     const int64_t rows = is_w ? q.V : q.T, first = is_w ? blockIdx.x - x_blocks : blockIdx.x;
     const int64_t step = (is_w ? gridDim.x - x_blocks : x_blocks) * static_cast<int64_t>(kThreads / 32);
@@ -137,6 +139,8 @@ __global__ void __launch_bounds__(kThreads)
 planes_kernel(Source q, int64_t dp, const unsigned* part, int x_blocks, int w_blocks, Header* head, void* xp,
               void* wp, int vec) {
     __shared__ unsigned s[kThreads / 32];
+    let_follow();
+    follow();
     float scale_x = 1.f, scale_w = 1.f;
     if (sizeof(T) == 4) {
         unsigned mx = 0, mw = 0;
@@ -188,6 +192,8 @@ planes_kernel(Source q, int64_t dp, const unsigned* part, int x_blocks, int w_bl
 __global__ void __launch_bounds__(1024)
 grad_max_kernel(Problem p) {
     __shared__ unsigned s[32];
+    let_follow();
+    follow();
     unsigned m = 0;
     for (int64_t t = threadIdx.x; t < p.T; t += 1024)
         if (p.targets[t] != p.ignore) m = max(m, finite_bits(p.g_rows[t]));
@@ -216,6 +222,8 @@ finish_kernel(Problem p, int parts, float* __restrict__ rows, float* loss, doubl
     __shared__ double total[32];
     __shared__ int found[32];
     __shared__ bool last;
+    let_follow();
+    follow();
     const int64_t t0 = blockIdx.x * static_cast<int64_t>(32);
     float2 q = make_float2(-INFINITY, 0.f);
     if (t0 + threadIdx.x < p.T) {
@@ -351,11 +359,12 @@ int forward(const sl_xent_args& a, cudaStream_t st) {
     void *xp = s.prep + s.l.x, *wp = cw ? s.prep + s.l.w : nullptr;
     const int blocks = blocks_for(src.T + (cw ? V : 0));
     if (s.p.f32) {
-        absmax_kernel<<<bx + bw, kThreads, 0, st>>>(src, bx, maxima, vec);
-        planes_kernel<float><<<blocks, kThreads, 0, st>>>(src, s.l.dp, maxima, bx, bw, s.p.head, xp, wp, vec);
+        launch_following(absmax_kernel, bx + bw, kThreads, 0, st, src, bx, maxima, vec);
+        launch_following(planes_kernel<float>, blocks, kThreads, 0, st, src, s.l.dp, maxima, bx, bw, s.p.head, xp, wp, vec);
     } else if (cx || cw) {
-        if (s.p.bf16) planes_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(src, s.l.dp, nullptr, 0, 0, s.p.head, xp, wp, vec);
-        else planes_kernel<__half><<<blocks, kThreads, 0, st>>>(src, s.l.dp, nullptr, 0, 0, s.p.head, xp, wp, vec);
+        const unsigned* none = nullptr;
+        launch_following(s.p.bf16 ? planes_kernel<__nv_bfloat16> : planes_kernel<__half>, blocks, kThreads, 0, st, src, s.l.dp,
+                         none, 0, 0, s.p.head, xp, wp, vec);
     }
     SL_RETURN_IF_LAUNCH_FAILED("sl_xent_forward");
     double* sums = reinterpret_cast<double*>(s.scratch + s.l.sums);
@@ -368,8 +377,8 @@ int forward(const sl_xent_args& a, cudaStream_t st) {
     const int parts = static_cast<int>((V + kPart - 1) / kPart);
     int groups = 1;
     while (groups < parts && groups < 32) groups *= 2;
-    finish_kernel<<<static_cast<unsigned>((T + 31) / 32), dim3(32, groups), 0, st>>>(
-        s.p, parts, a.loss_rows, a.loss, sums, counts);
+    launch_following(finish_kernel, static_cast<unsigned>((T + 31) / 32), dim3(32, groups), 0, st, s.p, parts, a.loss_rows,
+                     a.loss, sums, counts);
     SL_RETURN_IF_LAUNCH_FAILED("sl_xent_forward");
     return SL_OK;
 }
@@ -379,7 +388,7 @@ int backward(const sl_xent_args& a, cudaStream_t st) {
     const int64_t T = a.tokens, V = a.vocab;
     if (a.reduction == SL_XENT_NONE) {
         s.p.g_rows = a.grad;
-        grad_max_kernel<<<1, 1024, 0, st>>>(s.p);
+        launch_following(grad_max_kernel, 1, 1024, 0, st, s.p);
         SL_RETURN_IF_LAUNCH_FAILED("sl_xent_backward");
     } else {
         s.p.grad = a.grad;

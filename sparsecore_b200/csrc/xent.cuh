@@ -1,11 +1,37 @@
 // What the parts of the linear cross entropy share: the layout of its
-// buffers and of its operands as 16-bit planes.
+// buffers and of its operands as 16-bit planes, and how its kernels follow
+// one another.
 #pragma once
+
+#include <utility>
 
 #include "typed.cuh"
 
 namespace slb {
 namespace xent {
+
+// A pass is a chain of short kernels.  Each may start while the one before it
+// ends: it sets itself up, and then waits until all of that one's results are
+// there (and so those of all before).  Every thread calls follow() before its
+// first access to global memory.  33 x 1024 x 32003 fp16, losses only: 34 -> 31 us;
+// 16384 x 768 x 256 fp32 trained: 141 -> 134 (graph replay 129 -> 126).
+__device__ __forceinline__ void follow() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_follow() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... P, typename... A>
+void launch_following(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, A&&... a) {
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c{};
+    c.gridDim = grid;
+    c.blockDim = block;
+    c.dynamicSmemBytes = smem;
+    c.stream = s;
+    c.attrs = &early;
+    c.numAttrs = 1;
+    cudaLaunchKernelEx(&c, kernel, std::forward<A>(a)...);  // errors: cudaGetLastError, as of any launch
+}
 
 constexpr int kPart = 128;          // vocabulary columns of one partial (max, sum) of a row
 constexpr int64_t kMostSlabFloats = int64_t(16) << 20;  // sums that a split product may leave to be joined

@@ -379,7 +379,6 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     Shared& sh = *reinterpret_cast<Shared*>(ring + kRing * kBox);
     const int warp = threadIdx.x >> 5, lane = lane_id();
     const uint32_t rank = cluster_rank();
-    if (MODE == kStats && blockIdx.x == 0 && threadIdx.x == 0) a.p.head->done = 0;  // for the finish
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&sh.full[s], 1);
@@ -396,6 +395,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     __syncthreads();
     cluster_sync();
     tc_fence_after();
+    let_follow();
+    follow();
+    if (MODE == kStats && blockIdx.x == 0 && threadIdx.x == 0) a.p.head->done = 0;  // for the finish
     const uint32_t tmem = sh.tmem;
     const int tiles = a.tiles_m * a.tiles_n * a.splits, pairs = gridDim.x / 2, pair = blockIdx.x / 2;
     const int all = static_cast<int>((a.K + kSlice - 1) / kSlice);
@@ -540,6 +542,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 template <int W>
 __global__ void __launch_bounds__(256)
 join_kernel(Problem p, Output o, int64_t M, int64_t N, int64_t stride, int64_t slab, int splits, bool f32) {
+    let_follow();
+    follow();
     const float scale = out_scale(p, o.by_x, f32);
     const int64_t step = static_cast<int64_t>(gridDim.x) * 256 * W;
     const int across = static_cast<int>(N);
@@ -588,7 +592,7 @@ int launch(const Operand& A, const Operand& B, const Args& a, cudaStream_t s) {
     if (!map(&ma, A, a.a_mn) || !map(&mb, B, a.b_mn)) return fail(SL_ERR_CUDA, "sl_xent: tensor map could not be made");
     const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits;
     const int64_t pairs = std::min<int64_t>(tiles, std::min(kMostCtas / 2, std::max(1, num_sms() / 2)));
-    gemm_kernel<PL, MODE><<<static_cast<unsigned>(2 * pairs), kThreads, kSmem, s>>>(ma, mb, a);
+    launch_following(gemm_kernel<PL, MODE>, static_cast<unsigned>(2 * pairs), kThreads, kSmem, s, ma, mb, a);
     SL_RETURN_IF_LAUNCH_FAILED("sl_xent");
     return SL_OK;
 }
@@ -616,8 +620,8 @@ int run(Args& a, const Operand& A, const Operand& B, cudaStream_t s) {
         // four columns a thread where that still fills the GPU
         const int w = a.N % 4 == 0 && a.M * a.N >= num_sms() * 2048 ? 4 : 1;
         const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((a.M * a.N / w + 255) / 256, num_sms() * 16));
-        if (w == 4) join_kernel<4><<<blocks, 256, 0, s>>>(a.p, a.o, a.M, a.N, stride, a.slab_stride, a.splits, a.p.f32);
-        else join_kernel<1><<<blocks, 256, 0, s>>>(a.p, a.o, a.M, a.N, stride, a.slab_stride, a.splits, a.p.f32);
+        launch_following(w == 4 ? join_kernel<4> : join_kernel<1>, blocks, 256, 0, s, a.p, a.o, a.M, a.N, stride, a.slab_stride,
+                         a.splits, a.p.f32);
         SL_RETURN_IF_LAUNCH_FAILED("sl_xent");
     }
     return SL_OK;

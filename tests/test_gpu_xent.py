@@ -324,3 +324,51 @@ def test_refusals():
             sl.linear_cross_entropy(*bad)
     with pytest.raises(RuntimeError):
         sl.linear_cross_entropy(x, w.cpu(), t)
+
+
+@gpu
+@pytest.mark.parametrize("vocab", [70, 600])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_between_other_work(dtype, vocab):
+    """The kernels of a pass may start before the one ahead of them ends: what
+    lies before and behind them (a fill, a copy, another stream's work, the
+    reuse of their buffers) is ordered all the same, eager and captured."""
+    import sparsecore_b200 as sl
+
+    x, w, t = _case(300, 136, vocab, dtype, 23)
+    xl, wl = torch.zeros_like(x).requires_grad_(), torch.zeros_like(w).requires_grad_()
+    tl = torch.zeros_like(t)
+    side = torch.cuda.Stream()
+
+    def once():
+        with torch.no_grad():
+            wl.zero_()  # a fill, a copy and a kernel of another stream write the operands
+            xl.copy_(x)
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                wl.add_(w)
+                tl.copy_(t)
+            torch.cuda.current_stream().wait_stream(side)
+        loss = sl.linear_cross_entropy(xl, wl, tl)
+        grads = torch.autograd.grad(loss, (xl, wl))
+        with torch.no_grad():
+            xl.fill_(float("nan"))
+            wl.zero_()
+            tl.zero_()
+            return [loss.detach().clone(), *(g.clone() for g in grads)]
+
+    xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = sl.linear_cross_entropy(xr, wr, t)
+    want = [loss.detach(), *torch.autograd.grad(loss, (xr, wr))]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = once()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = once()
+    for _ in range(20):
+        for h in held:
+            h.zero_()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
