@@ -225,6 +225,12 @@ class AdamWPlan:
         return [g.contiguous() for g in grads]
 
 
+def _check_counter(step, device):
+    """Refuses a step count that the kernel on `device` must not write to."""
+    if not isinstance(step, torch.Tensor) or step.device != device or step.dtype != torch.int64 or step.numel() != 1:
+        raise ValueError(f"FusedAdamW: a step count on the device must be one int64 element on {device}, got {step!r}")
+
+
 def _no_overlap(tensors):
     """Refuses tensors that are written and share memory (the same one twice, or views that overlap)."""
     spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
@@ -337,6 +343,7 @@ class FusedAdamW(torch.optim.Optimizer):
         """Adds one to the group's step count on the device and makes the step's numbers there."""
         if not isinstance(group.get("step"), torch.Tensor):
             group["step"] = torch.full((), int(group.get("step", 0)), dtype=torch.int64, device=dev)
+        _check_counter(group["step"], dev)
         hyper = self._hypers.get(k)
         if hyper is None or hyper.device != dev:
             hyper = self._hypers[k] = torch.empty(int(N.lib().sl_adamw_hyper_bytes()), dtype=torch.uint8, device=dev)
@@ -359,6 +366,14 @@ class FusedAdamW(torch.optim.Optimizer):
         for i, p in zip(ids, [p for g in self.param_groups for p in g["params"]]):
             for name, v in state_dict["state"].get(i, {}).items():
                 self.state[p][name] = v.detach().to(p.device, copy=True)
+        # A group's numbers came as they were saved, on the host maybe; the kernels read them where its parameters are.
+        for group in self.param_groups:
+            dev = group["params"][0].device
+            if "step" in group:
+                at = int(group["step"])
+                group["step"] = torch.full((), at, dtype=torch.int64, device=dev) if self.capturable else at
+            if isinstance(group["lr"], torch.Tensor):
+                group["lr"] = group["lr"].to(dev) if self.capturable else float(group["lr"])
 
     def state_values(self, p) -> tuple[torch.Tensor, torch.Tensor]:
         """The first and second moment of ``p`` in 32 bits, in its shape."""

@@ -1,0 +1,61 @@
+"""The optimizer's bookkeeping that needs no GPU: where a loaded state's counts
+and learning rates end up, what copies keep, and what is refused before any
+address is read."""
+import copy
+import pickle
+
+import pytest
+import torch
+
+
+def _saved(capturable, counts=(5, 5, 2), torchs=False, lr=1e-3):
+    """A state dict of three parameters as it comes from a file, on the host."""
+    import sparsecore_b200 as sl
+
+    params = [torch.zeros(4, requires_grad=True) for _ in counts]
+    opt = torch.optim.AdamW(params, lr=lr) if torchs else sl.FusedAdamW(params, lr=lr, capturable=capturable)
+    count = (lambda c: torch.tensor(c, dtype=torch.int64)) if capturable else int
+    if torchs:
+        count = lambda c: torch.tensor(float(c))  # noqa: E731
+    for p, c in zip(params, counts):
+        if c is None:
+            continue
+        opt.state[p].update(exp_avg=torch.ones(4), exp_avg_sq=torch.ones(4))
+        if torchs or c != counts[0]:
+            opt.state[p]["step"] = count(c)
+    if not torchs:
+        opt.param_groups[0]["step"] = count(counts[0])
+    return opt.state_dict()
+
+
+def test_counts_and_rates_go_to_the_parameters_device():
+    import sparsecore_b200 as sl
+
+    state = _saved(True, counts=(5, 5, 5), lr=torch.tensor(0.25))
+    params = [torch.zeros(4, device="meta", requires_grad=True) for _ in range(3)]
+    opt = sl.FusedAdamW(params, capturable=True)
+    opt.load_state_dict(state)
+    group = opt.param_groups[0]
+    for v in (group["step"], group["lr"]):
+        assert v.device.type == "meta" and v.numel() == 1
+    assert group["step"].dtype == torch.int64
+
+
+def test_a_counter_elsewhere_is_refused_before_it_is_used():
+    from sparsecore_b200 import optim
+
+    gpu0, host, z = torch.device("cuda", 0), torch.device("cpu"), torch.zeros
+    for bad, dev in ((z((), dtype=torch.int64), gpu0), (z((), dtype=torch.int64, device="meta"), gpu0), (z(()), host),
+                     (z(2, dtype=torch.int64), host), (3, gpu0)):
+        with pytest.raises(ValueError, match="step"):
+            optim._check_counter(bad, dev)
+    optim._check_counter(z((), dtype=torch.int64), host)
+
+
+def test_a_state_before_the_first_step_has_no_count():
+    import sparsecore_b200 as sl
+
+    make = lambda: sl.FusedAdamW([torch.zeros(4, requires_grad=True)])  # noqa: E731
+    opt = make()
+    opt.load_state_dict(make().state_dict())
+    assert not opt.param_groups[0].get("step")
