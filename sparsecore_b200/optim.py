@@ -102,19 +102,21 @@ class AdamWPlan:
     its block's scale, and ``exp_avg_sqs`` hold the second moments' square
     roots (see ``sl_adamw_multi``).  ``live``: per parameter None, or the int32
     column indices of a padded CSR whose slots below 0 are left alone, value
-    and moments.
+    and moments.  ``numbers``: the parameters' numbers that the 8-bit moments'
+    dither depends on, where the list is part of a longer one (default: 0, 1, ...).
 
     The plan keeps the tensors and the table of their addresses; a tensor
     whose storage was replaced since is looked up again at the next step.
     """
 
-    def __init__(self, params, exp_avgs, exp_avg_sqs, *, live=None, scales=None):
+    def __init__(self, params, exp_avgs, exp_avg_sqs, *, live=None, scales=None, numbers=None):
         self.params, self.exp_avgs, self.exp_avg_sqs = list(params), list(exp_avgs), list(exp_avg_sqs)
         n = len(self.params)
         self.live = [None] * n if live is None else list(live)
         self.scales = None if scales is None else [tuple(s) for s in scales]
+        self.numbers = list(range(n) if numbers is None else numbers)
         for name, v in (("exp_avgs", self.exp_avgs), ("exp_avg_sqs", self.exp_avg_sqs), ("live", self.live),
-                        ("scales", self.scales)):
+                        ("scales", self.scales), ("numbers", self.numbers)):
             if v is not None and len(v) != n:
                 raise ValueError(f"AdamWPlan: {name} has {len(v)} entries for {n} params")
         self._flat = self.params + self.exp_avgs + self.exp_avg_sqs + [t for t in self.live if t is not None]
@@ -161,7 +163,7 @@ class AdamWPlan:
         for i, p in enumerate(self.params):
             sm, sv = (None, None) if self.scales is None else self.scales[i]
             table[i] = (p.data_ptr(), 0, ptr(self.exp_avgs[i]), ptr(self.exp_avg_sqs[i]), ptr(sm), ptr(sv),
-                        ptr(self.live[i]), p.numel(), i)
+                        ptr(self.live[i]), p.numel(), self.numbers[i])
         self._sizes = list(map(_get_numel, self.params))
         self._dtypes = list(map(_get_dtype, self.params))
         kinds = sorted(set(self._dtypes), key=lambda d: N.DTYPES[d])
@@ -258,6 +260,10 @@ class FusedAdamW(torch.optim.Optimizer):
     ``capturable``: the step count is kept on the device, and a learning rate
     given as a float32 CUDA tensor is read there, so that a captured step
     replays correctly.
+
+    Each parameter's moments are corrected by the steps that it has taken itself,
+    as in torch's AdamW: one that begins late, misses steps or is drawn again is
+    stepped by its own count (in a launch of its own for each different count).
     """
 
     def __init__(self, model_or_params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
@@ -296,8 +302,8 @@ class FusedAdamW(torch.optim.Optimizer):
                 st[k] = torch.zeros(p.numel(), dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)
                 st[k + "_scale"] = torch.zeros(-(-p.numel() // BLOCK), dtype=torch.float32, device=p.device)
 
-    def _plan(self, k, params, cols):
-        """The group's plan; made again where a tensor of it is another one."""
+    def _plan(self, k, group, params, cols):
+        """The plan of a group's parameters of one count; made again where a tensor of it is another one."""
         live = [cols.get(p) for p in params]
         st = [self.state[p] for p in params]
         if self.state_bits == 32:
@@ -309,7 +315,8 @@ class FusedAdamW(torch.optim.Optimizer):
         if (kept is None or len(kept.params) != len(params)
                 or any(a is not b for a, b in zip(kept.params + kept.exp_avgs + kept.exp_avg_sqs + kept.live,
                                                   params + ms + vs + live))):
-            kept = self._plans[k] = AdamWPlan(params, ms, vs, live=live, scales=scales)
+            number = {p: i for i, p in enumerate(group["params"])}
+            kept = self._plans[k] = AdamWPlan(params, ms, vs, live=live, scales=scales, numbers=[number[p] for p in params])
         return kept
 
     @torch.no_grad()
@@ -319,39 +326,87 @@ class FusedAdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         cols = self._columns()
+        used = set()
         for k, group in enumerate(self.param_groups):
             params = [p for p in group["params"] if p.grad is not None]
             if not params:
                 continue
-            for p in params:
-                st = self.state[p]
-                if not st or st["exp_avg"].numel() != p.numel():  # new, or a layer drawn again at another capacity
-                    self._init_state(p)
-            plan = self._plan(k, params, cols)
-            grads = [p.grad for p in params]
-            lr, kw = group["lr"], {}
-            if self.capturable:
-                kw["hyper"] = self._advance(k, group, plan.device)
-                lr = 0.0
-            else:
-                group["step"] = kw["step"] = int(group.get("step", 0)) + 1
-            plan.step(grads, lr=lr, betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
-                      seed=self.seed, **kw)
+            for j, (count, members, holders) in enumerate(self._counted(group, params)):
+                used.add((k, j))
+                plan = self._plan((k, j), group, members, cols)
+                grads = [p.grad for p in members]
+                if self.capturable:
+                    plan.step(grads, seed=self.seed, hyper=self._advance((k, j), count, group, plan.device))
+                    continue
+                plan.step(grads, step=count + 1, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                          weight_decay=group["weight_decay"], seed=self.seed)
+                for h in holders:
+                    h["step"] = count + 1
+        if len(self._plans) > len(used):  # of counts that are no more
+            self._plans = {key: plan for key, plan in self._plans.items() if key in used}
         return loss
 
-    def _advance(self, k, group, dev):
-        """Adds one to the group's step count on the device and makes the step's numbers there."""
-        if not isinstance(group.get("step"), torch.Tensor):
-            group["step"] = torch.full((), int(group.get("step", 0)), dtype=torch.int64, device=dev)
-        _check_counter(group["step"], dev)
-        hyper = self._hypers.get(k)
+    def _counted(self, group, params):
+        """[(step count, the parameters of ``params`` that have it, the dictionaries that hold it)].  AdamW corrects
+        a parameter's moments by its own steps: the group's "step" counts those of the parameters that have
+        taken every one, and a parameter that began later, missed one or was drawn again has a "step" in
+        its state.  On the device (capturable) parameters of one history share one tensor."""
+        state = self.state
+        at = group.get("step", 0)
+        begun = isinstance(at, torch.Tensor) or at > 0
+        if self.capturable and not isinstance(at, torch.Tensor):
+            at = group["step"] = torch.full((), at, dtype=torch.int64, device=params[0].device)
+        late, zero = False, None
+        for p in params:
+            st = state[p]
+            if not st or st["exp_avg"].numel() != p.numel():  # new, or a layer drawn again at another capacity
+                self._init_state(p)
+                st.pop("step", None)
+                if begun:
+                    zero = (torch.zeros_like(at) if self.capturable else 0) if zero is None else zero
+                    st["step"] = zero
+            late = late or "step" in st
+        if len(params) < len(group["params"]):
+            self._set_apart(group, params, at)
+            late = late or any("step" in state[p] for p in params)
+        if not late:
+            return [(at, params, [group])]
+        by: dict = {}
+        for p in params:
+            count = state[p].get("step")
+            key = None if count is None else id(count) if isinstance(count, torch.Tensor) else count
+            by.setdefault(key, (at if count is None else count, []))[1].append(p)
+        return [(count, ps, [group] if key is None else [state[p] for p in ps]) for key, (count, ps) in by.items()]
+
+    def _set_apart(self, group, params, at):
+        """Gives parameters that miss this step a count of their own where the one they share goes on without them."""
+        state, copies = self.state, {}
+        shared = {id(state[p].get("step", group)) for p in params}
+        for p in group["params"]:
+            st = state.get(p)
+            if p.grad is not None or not st:
+                continue
+            count = st.get("step")
+            if id(group if count is None else count) not in shared or isinstance(count, int):
+                continue
+            count = at if count is None else count
+            if isinstance(count, torch.Tensor):
+                if id(count) not in copies:
+                    copies[id(count)] = count.clone()
+                count = copies[id(count)]
+            st["step"] = count
+
+    def _advance(self, key, count, group, dev):
+        """Adds one to a step count on the device and makes the step's numbers there."""
+        _check_counter(count, dev)
+        hyper = self._hypers.get(key)
         if hyper is None or hyper.device != dev:
-            hyper = self._hypers[k] = torch.empty(int(N.lib().sl_adamw_hyper_bytes()), dtype=torch.uint8, device=dev)
+            hyper = self._hypers[key] = torch.empty(int(N.lib().sl_adamw_hyper_bytes()), dtype=torch.uint8, device=dev)
         lr = group["lr"]
         on_device = isinstance(lr, torch.Tensor)
         if on_device and (lr.device != dev or lr.dtype != torch.float32 or lr.numel() != 1):
             raise ValueError(f"FusedAdamW: a tensor lr must be one float32 element on {dev}")
-        N.call_on(dev, "sl_adamw_hyper", N.ptr(group["step"]), N.ptr(lr if on_device else None),
+        N.call_on(dev, "sl_adamw_hyper", N.ptr(count), N.ptr(lr if on_device else None),
                   0.0 if on_device else float(lr), float(group["betas"][0]), float(group["betas"][1]),
                   float(group["eps"]), float(group["weight_decay"]), self.seed & 0xFFFFFFFF, N.ptr(hyper))
         return hyper
@@ -365,15 +420,31 @@ class FusedAdamW(torch.optim.Optimizer):
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(ids, [p for g in self.param_groups for p in g["params"]]):
             for name, v in state_dict["state"].get(i, {}).items():
-                self.state[p][name] = v.detach().to(p.device, copy=True)
-        # A group's numbers came as they were saved, on the host maybe; the kernels read them where its parameters are.
+                keep = name == "step" or not isinstance(v, torch.Tensor)
+                self.state[p][name] = v if keep else v.detach().to(p.device, copy=True)
         for group in self.param_groups:
-            dev = group["params"][0].device
-            if "step" in group:
-                at = int(group["step"])
-                group["step"] = torch.full((), at, dtype=torch.int64, device=dev) if self.capturable else at
-            if isinstance(group["lr"], torch.Tensor):
-                group["lr"] = group["lr"].to(dev) if self.capturable else float(group["lr"])
+            self._place_numbers(group)
+
+    def _place_numbers(self, group):
+        """A loaded group's step counts and learning rate came as they were saved, on the host maybe: they go where its
+        parameters are, or become plain numbers where nothing is captured.  A state of ``torch.optim.AdamW`` has
+        every count in its parameter's state."""
+        if not group["params"]:
+            return
+        dev = group["params"][0].device
+        put = lambda n: torch.full((), n, dtype=torch.int64, device=dev) if self.capturable else n  # noqa: E731
+        held = [self.state[p] for p in group["params"] if self.state.get(p)]
+        own = [int(st["step"]) if "step" in st else None for st in held]
+        if "step" in group or any(n is not None for n in own):
+            at = int(group["step"]) if "step" in group else max(n for n in own if n is not None)
+            group["step"], counts = put(at), {}
+            for st, n in zip(held, own):
+                if n is None or n == at:
+                    st.pop("step", None)
+                else:
+                    st["step"] = counts[n] = counts[n] if n in counts else put(n)
+        if isinstance(group["lr"], torch.Tensor):
+            group["lr"] = group["lr"].to(dev) if self.capturable else float(group["lr"])
 
     def state_values(self, p) -> tuple[torch.Tensor, torch.Tensor]:
         """The first and second moment of ``p`` in 32 bits, in its shape."""

@@ -1,0 +1,187 @@
+"""FusedAdamW's step counts, states and rare values: each parameter's own count,
+pauses and late starts against torch's AdamW, captured steps, copies and
+checkpoints, 8-bit moments at the ends of the range."""
+import copy
+import math
+import pickle
+
+import pytest
+import torch
+
+from gpu_helpers import dev
+
+gpu = pytest.mark.gpu
+
+
+def _params(seed=1, sizes=(70, 300, 5)):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(n, generator=g).to(dev()).requires_grad_() for n in sizes]
+
+
+def _grads(params, step, on, seed=2):
+    g = torch.Generator().manual_seed(seed * 1000 + step)
+    for k, p in enumerate(params):
+        gr = torch.randn(p.shape, generator=g).to(dev())
+        p.grad = gr if k in on else None
+
+
+# which parameters have a gradient at each step: a late start, pauses, all at once
+PATTERNS = [[{0}] * 5 + [{0, 1, 2}] * 4,
+            [{0, 1, 2}, {0, 1, 2}, {1, 2}, {0, 1, 2}, {1}, {0, 2}, {0, 1, 2}],
+            [set(), {2}, {1}, {0}, {0, 1, 2}, {0, 1}, {0, 1, 2}],
+            [{0, 1, 2}, {0}, {0}, {0, 1, 2}, {1, 2}, {0, 1, 2}]]
+
+
+@gpu
+@pytest.mark.parametrize("pattern", PATTERNS)
+@pytest.mark.parametrize("capturable", [False, True])
+def test_each_parameter_counts_its_own_steps(pattern, capturable):
+    import sparsecore_b200 as sl
+
+    a, b = _params(), _params()
+    kw = dict(lr=1e-2, betas=(0.9, 0.99), weight_decay=0.05)
+    oa, ob = torch.optim.AdamW(a, **kw), sl.FusedAdamW(b, capturable=capturable, **kw)
+    for step, on in enumerate(pattern):
+        _grads(a, step, on)
+        _grads(b, step, on)
+        oa.step()
+        ob.step()
+        for p, q in zip(a, b):
+            torch.testing.assert_close(q, p, rtol=1e-5, atol=1e-6)
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_first_step_of_a_late_parameter_is_the_learning_rate(bits):
+    """m / root of a first step is 1 whatever the gradient is, to the rounding of
+    32-bit numbers (the 8-bit step takes its quotient to 2^-22)."""
+    import sparsecore_b200 as sl
+
+    params = _params()
+    opt = sl.FusedAdamW(params, lr=1e-2, weight_decay=0.0, state_bits=bits)
+    for step in range(300):
+        _grads(params, step, {0, 2})
+        opt.step()
+    before = params[1].detach().clone()
+    _grads(params, 300, {0, 1, 2})
+    opt.step()
+    moved = (params[1].detach() - before).abs().double()
+    big = params[1].grad.abs() > 1e-3  # eps is then below 1e-5 of the root
+    assert bool(((moved[big] - 1e-2).abs() <= 1e-2 * 2e-5 + 2.0 ** -23 * before[big].abs()).all())
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_layer_drawn_again_starts_its_count_again(bits, capturable):
+    import sparsecore_b200 as sl
+
+    torch.manual_seed(3)
+    model = torch.nn.Sequential(sl.SparseLinear(96, 64, sparsity=0.8, device=dev()), torch.nn.Linear(64, 8).to(dev()))
+    # after 50 steps the old count's corrections make a first step 0.5 / sqrt(0.001 / (1 - 0.999^51)) = 3.5 times lr
+    opt = sl.FusedAdamW(model, lr=1e-3, betas=(0.5, 0.999), weight_decay=0.0, state_bits=bits, capturable=capturable)
+    x = torch.randn(40, 96, device=dev())
+
+    def once():
+        opt.zero_grad()
+        model(x).square().mean().backward()
+        opt.step()
+
+    for _ in range(50):
+        once()
+    n = model[0]._values.numel()
+    while model[0]._values.numel() == n:  # until the number of slots is another one
+        model[0].reset_parameters()
+    before = model[0]._values.detach().clone()
+    once()
+    assert float((model[0]._values.detach() - before).abs().max()) <= 1e-3 * 1.0001 + 2.0 ** -23
+    once()
+    assert torch.isfinite(model[0]._values).all()
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_steps_with_a_late_parameter_equal_eager_ones(bits):
+    import sparsecore_b200 as sl
+
+    sets = [_params() for _ in range(2)]
+    opts = [sl.FusedAdamW(p, lr=1e-2, capturable=True, state_bits=bits) for p in sets]
+    fixed = _params(9)
+    for p in sets:
+        for q, f, k in zip(p, fixed, range(3)):
+            q.grad = f.detach().clone() if k != 1 else None
+    for _ in range(6):
+        for o in opts:
+            o.step()
+    for p in sets:
+        p[1].grad = fixed[1].detach().clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for o in opts:
+            o.step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opts[0].step()
+    for _ in range(3):
+        graph.replay()
+        opts[1].step()
+    torch.cuda.synchronize()
+    for p, q in zip(*sets):
+        assert torch.equal(p, q)
+    assert int(opts[0].param_groups[0]["step"]) == 10
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_state_that_was_on_the_host_goes_on_as_before(bits, capturable, tmp_path):
+    """Through a file and back to the host, as checkpoints go, with parameters at different counts."""
+    import sparsecore_b200 as sl
+
+    kw = dict(state_bits=bits, capturable=capturable)
+    lr = lambda: torch.tensor(1e-2, device=dev()) if capturable else 1e-2  # noqa: E731
+    a, b = _params(), _params()
+    oa, ob = sl.FusedAdamW(a, lr=lr(), **kw), sl.FusedAdamW(b, lr=lr(), **kw)
+    for step, on in enumerate(PATTERNS[1]):
+        _grads(a, step, on)
+        oa.step()
+    torch.save(oa.state_dict(), tmp_path / "opt.pt")
+    ob.load_state_dict(torch.load(tmp_path / "opt.pt", map_location="cpu"))
+    for group in ob.param_groups:
+        for v in (group["step"], group["lr"]):
+            assert isinstance(v, torch.Tensor) == capturable and (not capturable or v.device == dev())
+    with torch.no_grad():
+        for p, q in zip(a, b):
+            q.copy_(p)
+    for step, on in enumerate(PATTERNS[0], 50):
+        for params, o in ((a, oa), (b, ob)):
+            _grads(params, step, on)
+            o.step()
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)
+
+
+@gpu
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_state_of_torchs_optimizer_goes_on(capturable):
+    import sparsecore_b200 as sl
+
+    a, b = _params(), _params()
+    kw = dict(lr=1e-2, betas=(0.9, 0.99), weight_decay=0.05)
+    oa = torch.optim.AdamW(a, **kw)
+    for step, on in enumerate(PATTERNS[1]):
+        _grads(a, step, on)
+        oa.step()
+    ob = sl.FusedAdamW(b, capturable=capturable, **kw)
+    ob.load_state_dict(oa.state_dict())
+    with torch.no_grad():
+        for p, q in zip(a, b):
+            q.copy_(p)
+    for step, on in enumerate(PATTERNS[1], 50):
+        for params, o in ((a, oa), (b, ob)):
+            _grads(params, step, on)
+            o.step()
+        for p, q in zip(a, b):
+            torch.testing.assert_close(q, p, rtol=1e-5, atol=1e-6)

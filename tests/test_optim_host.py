@@ -59,3 +59,37 @@ def test_a_state_before_the_first_step_has_no_count():
     opt = make()
     opt.load_state_dict(make().state_dict())
     assert not opt.param_groups[0].get("step")
+
+
+def test_counts_of_late_parameters_go_there_too():
+    import sparsecore_b200 as sl
+
+    params = [torch.zeros(4, device="meta", requires_grad=True) for _ in range(3)]
+    opt = sl.FusedAdamW(params, capturable=True)
+    opt.load_state_dict(_saved(True))
+    own = opt.state[params[2]]["step"]
+    assert own.device.type == "meta" and own.numel() == 1 and own.dtype == torch.int64
+    assert "step" not in opt.state[params[0]] and "step" not in opt.state[params[1]]
+
+
+@pytest.mark.parametrize("torchs", [False, True])
+@pytest.mark.parametrize("was", [False, True])
+@pytest.mark.parametrize("now", [False, True])
+def test_counts_keep_their_values(was, now, torchs):
+    import sparsecore_b200 as sl
+
+    if torchs and was:
+        pytest.skip("one form of torch's state is enough")
+    for counts in ((5, 5, 2), (7, 7, 7), (3, None, 3), (4, 6, 6)):
+        params = [torch.zeros(4, requires_grad=True) for _ in counts]
+        opt = sl.FusedAdamW(params, capturable=now)
+        opt.load_state_dict(_saved(was, counts, torchs))
+        at = opt.param_groups[0]["step"]
+        assert isinstance(at, torch.Tensor) == now
+        for p, c in zip(params, counts):
+            st = opt.state.get(p)
+            if c is None:
+                assert not st
+                continue
+            own = st.get("step", at)
+            assert int(own) == c and isinstance(own, torch.Tensor) == now
