@@ -287,6 +287,16 @@ class FusedAdamW(torch.optim.Optimizer):
         self._hypers: dict = {}
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
+    # torch's optimizers keep only their defaults, states and groups; a copy makes its own tables.  (SparseLinears hold
+    # addresses and refuse to be copied, and so does an optimizer over them.)
+    def __getstate__(self):
+        return super().__getstate__() | {k: self.__dict__[k] for k in ("_sparse", "_live", "state_bits", "capturable", "seed")}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for k in ("_plans", "_hypers"):
+            self.__dict__.setdefault(k, {})
+
     def _columns(self):
         cols = {m._values: m._csr.col_indices for m in self._sparse}
         cols.update(self._live)

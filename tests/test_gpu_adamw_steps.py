@@ -185,3 +185,33 @@ def test_a_state_of_torchs_optimizer_goes_on(capturable):
             o.step()
         for p, q in zip(a, b):
             torch.testing.assert_close(q, p, rtol=1e-5, atol=1e-6)
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("way", ["copy", "pickle"])
+def test_copies_of_an_optimizer_go_on_by_themselves(bits, capturable, way, tmp_path):
+    """(torch's 8-bit floats go through its files but not through plain pickle.)"""
+    import sparsecore_b200 as sl
+
+    a = _params()
+    oa = sl.FusedAdamW(a, lr=1e-2, state_bits=bits, capturable=capturable, seed=3)
+    for step, on in enumerate(PATTERNS[1]):
+        _grads(a, step, on)
+        oa.step()
+    if way == "copy":
+        ob = copy.deepcopy(oa)
+    elif bits == 32:
+        ob = pickle.loads(pickle.dumps(oa))
+    else:
+        torch.save(oa, tmp_path / "opt.pt")
+        ob = torch.load(tmp_path / "opt.pt", weights_only=False)
+    b = ob.param_groups[0]["params"]
+    assert all(p is not q and p.data_ptr() != q.data_ptr() for p, q in zip(a, b))
+    for step, on in enumerate(PATTERNS[1], 50):
+        for params, o in ((a, oa), (b, ob)):
+            _grads(params, step, on)
+            o.step()
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)

@@ -93,3 +93,19 @@ def test_counts_keep_their_values(was, now, torchs):
                 continue
             own = st.get("step", at)
             assert int(own) == c and isinstance(own, torch.Tensor) == now
+
+
+@pytest.mark.parametrize("way", [copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))])
+def test_copies_keep_what_a_step_needs(way):
+    import sparsecore_b200 as sl
+
+    p, q = torch.zeros(4, requires_grad=True), torch.zeros(4, requires_grad=True)
+    opt = sl.FusedAdamW([p, q], lr=0.5, state_bits=8, capturable=True, seed=9, live={q: torch.zeros(4, dtype=torch.int32)})
+    got = way(opt)
+    assert (got.state_bits, got.capturable, got.seed) == (8, True, 9)
+    new_p, new_q = got.param_groups[0]["params"]
+    assert new_p is not p and list(got._columns()) == [new_q]
+    with pytest.raises(ValueError):  # their own plans, not the first one's
+        new_p.grad, new_q.grad = torch.ones(4), torch.ones(4)
+        got.load_state_dict(_saved(False))
+    assert got._plans == {} and got._plans is not opt._plans
