@@ -259,7 +259,9 @@ class FusedAdamW(torch.optim.Optimizer):
     256 elements (a quarter of the memory; ``state_values`` gives them back).
     ``capturable``: the step count is kept on the device, and a learning rate
     given as a float32 CUDA tensor is read there, so that a captured step
-    replays correctly.
+    replays correctly.  Before a capture, take one step with gradients on the
+    same parameters: moments and counts that would begin inside it are refused,
+    and so is a capture without ``capturable``.
 
     Each parameter's moments are corrected by the steps that it has taken itself,
     as in torch's AdamW: one that begins late, misses steps or is drawn again is
@@ -341,6 +343,8 @@ class FusedAdamW(torch.optim.Optimizer):
             params = [p for p in group["params"] if p.grad is not None]
             if not params:
                 continue
+            if not self.capturable and params[0].is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("FusedAdamW: a captured step needs capturable=True (its replays would repeat one step's numbers)")
             for j, (count, members, holders) in enumerate(self._counted(group, params)):
                 used.add((k, j))
                 plan = self._plan((k, j), group, members, cols)
@@ -365,11 +369,13 @@ class FusedAdamW(torch.optim.Optimizer):
         at = group.get("step", 0)
         begun = isinstance(at, torch.Tensor) or at > 0
         if self.capturable and not isinstance(at, torch.Tensor):
+            self._not_captured(params[0])
             at = group["step"] = torch.full((), at, dtype=torch.int64, device=params[0].device)
         late, zero = False, None
         for p in params:
             st = state[p]
             if not st or st["exp_avg"].numel() != p.numel():  # new, or a layer drawn again at another capacity
+                self._not_captured(p)
                 self._init_state(p)
                 st.pop("step", None)
                 if begun:
@@ -401,10 +407,17 @@ class FusedAdamW(torch.optim.Optimizer):
                 continue
             count = at if count is None else count
             if isinstance(count, torch.Tensor):
+                self._not_captured(p)
                 if id(count) not in copies:
                     copies[id(count)] = count.clone()
                 count = copies[id(count)]
             st["step"] = count
+
+    @staticmethod
+    def _not_captured(p):
+        if p.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedAdamW: moments or step counts would begin inside a graph capture, and every replay would begin "
+                               "them again; take one step with gradients on the same parameters before the capture")
 
     def _advance(self, key, count, group, dev):
         """Adds one to a step count on the device and makes the step's numbers there."""

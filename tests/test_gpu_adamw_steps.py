@@ -215,3 +215,39 @@ def test_copies_of_an_optimizer_go_on_by_themselves(bits, capturable, way, tmp_p
             o.step()
         for p, q in zip(a, b):
             assert torch.equal(p, q)
+
+
+@gpu
+def test_what_a_capture_would_freeze_is_refused():
+    """A count on the host, and moments or counts that begin inside the capture (every replay would begin them again)."""
+    import sparsecore_b200 as sl
+
+    params = _params()
+    _grads(params, 0, {0, 1, 2})
+    opt = sl.FusedAdamW(params, lr=1e-2)
+    opt.step()
+    keep = [p.detach().clone() for p in params]
+    late = _params(5)
+    _grads(late, 0, {0, 2})
+    opt2 = sl.FusedAdamW(late, lr=1e-2, capturable=True)
+    for o, on in ((opt, None), (opt2, None)):
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="captur"):
+            with torch.cuda.graph(graph):
+                torch.zeros(8, device=dev())
+                o.step()
+    opt2.step()
+    _grads(late, 1, {0, 1, 2})  # a parameter that begins inside the capture
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captur"):
+        with torch.cuda.graph(graph):
+            torch.zeros(8, device=dev())
+            opt2.step()
+    _grads(late, 1, {0})  # one that pauses inside it
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captur"):
+        with torch.cuda.graph(graph):
+            torch.zeros(8, device=dev())
+            opt2.step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, k) for p, k in zip(params, keep))
