@@ -171,6 +171,8 @@ class AdamWPlan:
         self._groups = [(N.DTYPES[d], np.array([i for i, e in enumerate(self._dtypes) if e == d]), None) for d in kinds]
         self._groups = [(d, rows, np.ascontiguousarray(table[rows])) for d, rows, _ in self._groups]
         self._ptrs = list(map(_get_ptr, self._flat))
+        # While the table has an address its memory is kept: no other tensor's can be taken for it.
+        self._kept = [t.untyped_storage() for t in self._flat]
 
     def step(self, grads, *, step: int | None = None, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
              weight_decay: float = 1e-2, seed: int = 0, hyper: torch.Tensor | None = None) -> None:
@@ -199,6 +201,10 @@ class AdamWPlan:
             sizes, dtypes = [self._sizes[i] for i in on], [self._dtypes[i] for i in on]
         else:
             on, sizes, dtypes = None, self._sizes, self._dtypes
+        if list(map(_get_numel, given)) != sizes or list(map(_get_dtype, given)) != dtypes:
+            self._build()  # maybe a parameter was cut or given another type where it lies
+            every = range(len(grads)) if on is None else on
+            sizes, dtypes = [self._sizes[i] for i in every], [self._dtypes[i] for i in every]
         if (list(map(_get_dtype, given)) != dtypes or list(map(_get_numel, given)) != sizes
                 or set(map(_get_device, given)) != {self.device.index} or not all(map(_is_contiguous, given))):
             given = self._fit(given, sizes, dtypes)

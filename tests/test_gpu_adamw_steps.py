@@ -251,3 +251,31 @@ def test_what_a_capture_would_freeze_is_refused():
             opt2.step()
     torch.cuda.synchronize()
     assert all(torch.equal(p, k) for p, k in zip(params, keep))
+
+
+@gpu
+def test_a_plan_sees_tensors_that_changed_under_it():
+    """Its parameter is cut short where it lies, or replaced; an address in its table is nobody else's."""
+    import sparsecore_b200 as sl
+
+    base, m, v = (torch.zeros(64, device=dev()) for _ in range(3))
+    p = base.view(64)
+    plan = sl.AdamWPlan([p], [m], [v])
+    plan.step([torch.ones(64, device=dev())], step=1)
+    after = base.clone()
+    p.data = p.data[:10]
+    with pytest.raises(ValueError, match="elements"):  # its moments are still 64 long
+        plan.step([torch.ones(10, device=dev())], step=2)
+    m.data, v.data = m.data[:10], v.data[:10]
+    plan.step([torch.ones(10, device=dev())], step=2)
+    assert not (base[:10] == after[:10]).any() and torch.equal(base[10:], after[10:])
+    p, m, v = (torch.zeros(100000, device=dev()) for _ in range(3))
+    plan = sl.AdamWPlan([p], [m], [v])
+    plan.step([torch.ones(100000, device=dev())], step=1)
+    at = p.data_ptr()
+    p.data = torch.zeros(10, device=dev())
+    m.data, v.data = torch.zeros(10, device=dev()), torch.zeros(10, device=dev())
+    others = [torch.zeros(100000, device=dev()) for _ in range(3)]
+    assert all(t.data_ptr() != at for t in others)
+    plan.step([torch.ones(10, device=dev())], step=1)
+    assert p.all() and not any(t.any() for t in others)
