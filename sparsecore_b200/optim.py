@@ -20,6 +20,7 @@ bits; ``AdamWPlan`` is the same step over a caller's own lists.
 """
 from __future__ import annotations
 
+import functools
 from operator import attrgetter
 
 import numpy as np
@@ -190,6 +191,8 @@ class AdamWPlan:
                 raise ValueError(f"AdamWPlan: step must be at least 1, got {step}")
         if not grads:
             return
+        if hyper is not None:
+            _check_numbers(hyper, self.device)
         if list(map(_get_ptr, self._flat)) != self._ptrs:
             self._build()
         given = grads
@@ -231,6 +234,20 @@ class AdamWPlan:
             if g.numel() != n or g.dtype != d:
                 raise ValueError(f"AdamWPlan: a grad has {g.numel()} elements of {g.dtype}; its param {n} of {d}")
         return [g.contiguous() for g in grads]
+
+
+@functools.lru_cache(maxsize=None)
+def _hyper_bytes():
+    return int(N.lib().sl_adamw_hyper_bytes())
+
+
+def _check_numbers(hyper, device):
+    """Refuses what the kernel on `device` cannot read a step's numbers from."""
+    if not isinstance(hyper, torch.Tensor):
+        raise TypeError(f"AdamWPlan: hyper must be a torch.Tensor, got {type(hyper).__name__}")
+    if (hyper.device != device or not hyper.is_contiguous() or hyper.numel() * hyper.element_size() < _hyper_bytes()
+            or hyper.data_ptr() % 16):
+        raise ValueError(f"AdamWPlan: hyper must be {_hyper_bytes()} contiguous bytes on {device}, 16-byte aligned")
 
 
 def _check_counter(step, device):
@@ -430,7 +447,7 @@ class FusedAdamW(torch.optim.Optimizer):
         _check_counter(count, dev)
         hyper = self._hypers.get(key)
         if hyper is None or hyper.device != dev:
-            hyper = self._hypers[key] = torch.empty(int(N.lib().sl_adamw_hyper_bytes()), dtype=torch.uint8, device=dev)
+            hyper = self._hypers[key] = torch.empty(_hyper_bytes(), dtype=torch.uint8, device=dev)
         lr = group["lr"]
         on_device = isinstance(lr, torch.Tensor)
         if on_device and (lr.device != dev or lr.dtype != torch.float32 or lr.numel() != 1):

@@ -279,3 +279,22 @@ def test_a_plan_sees_tensors_that_changed_under_it():
     assert all(t.data_ptr() != at for t in others)
     plan.step([torch.ones(10, device=dev())], step=1)
     assert p.all() and not any(t.any() for t in others)
+
+
+@gpu
+def test_numbers_made_on_the_device_are_checked():
+    import sparsecore_b200 as sl
+
+    p, m, v, g = (torch.zeros(8, device=dev()) for _ in range(4))
+    plan = sl.AdamWPlan([p], [m], [v])
+    for bad in (torch.zeros(64, dtype=torch.uint8), torch.zeros(4, dtype=torch.uint8, device=dev()), 7,
+                torch.zeros(64, dtype=torch.uint8, device=dev())[::2], torch.zeros(65, dtype=torch.uint8, device=dev())[1:]):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            plan.step([g], hyper=bad)
+    opt = sl.FusedAdamW([p.requires_grad_()], capturable=True)
+    p.grad = g
+    opt.step()
+    for bad in (torch.zeros((), dtype=torch.int64), torch.zeros((), device=dev()), torch.zeros(2, dtype=torch.int64, device=dev())):
+        opt.param_groups[0]["step"] = bad
+        with pytest.raises(ValueError):
+            opt.step()

@@ -109,3 +109,18 @@ def test_copies_keep_what_a_step_needs(way):
         new_p.grad, new_q.grad = torch.ones(4), torch.ones(4)
         got.load_state_dict(_saved(False))
     assert got._plans == {} and got._plans is not opt._plans
+
+
+def test_numbers_made_elsewhere_are_refused_before_they_are_read():
+    from sparsecore_b200 import _native as N
+    from sparsecore_b200 import optim
+
+    n = int(N.load_library().sl_adamw_hyper_bytes())
+    host, gpu0 = torch.device("cpu"), torch.device("cuda", 0)
+    z = lambda k: torch.zeros(k, dtype=torch.uint8)  # noqa: E731
+    optim._check_numbers(z(n), host)
+    for bad, dev in ((z(n), gpu0), (z(n - 1), host), (z(2 * n)[::2], host), (z(n + 1)[1:], host)):
+        with pytest.raises(ValueError, match="hyper"):
+            optim._check_numbers(bad, dev)
+    with pytest.raises(TypeError):
+        optim._check_numbers(7, host)
