@@ -1084,9 +1084,12 @@ int backward(const sl_norm_args& n, cudaStream_t s) {
             int stages = 1;
             // Gates of whole runs of rows: one run a CTA (always so where its gradient is asked for).
             const bool shared = !n.gate || (a.gate_rows > 1 && (a.gate_rows == a.T || sp.seg > 0));
-            if constexpr (ring) {  // this row, the next, and one or two on their way
+            if constexpr (ring) {
+                // This row, the next, and one or two on their way.  Three fit at every width and type; the tightest is a
+                // 16-bit gate a row over a 32-bit stream at 4096 columns, 7 granules x 8 KB a row beside 3 vectors of 16 KB.
                 const size_t lap = 16 * block.x, stage = G::granules(!shared && G::kGates && a.gate_rows == 1 && !a.gate_f32) * lap;
-                bytes = (shared ? 2 : G::kVectors ? 4 : 0) * G::kVec * lap;
+                // (vectors; the last of four is a gate that rows share)
+                bytes = (shared ? 2 : G::kVectors ? (a.gate_rows == 1 ? 3 : 4) : 0) * G::kVec * lap;
                 stages = static_cast<int>(std::min<size_t>(4, (kFullSmem - bytes) / stage));
                 if (stages < 3) return fail(SL_ERR_UNSUPPORTED, "sl_norm_backward: rows do not fit");
                 bytes += stages * stage;
