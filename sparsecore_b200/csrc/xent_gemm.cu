@@ -195,8 +195,9 @@ __device__ __forceinline__ void epilogue_grad(const Args& a, float (&z)[128], in
     const int tg = target_of(a.p, t);
     float one = a.p.bf16 ? 1.f : kGradScale;
     if (a.p.g_rows) {  // single losses' gradients, over the largest
-        const float top = __uint_as_float(a.p.head->max_g);
-        one = top > 0.f ? one * (a.p.g_rows[t] / top) : 0.f;
+        const float top = __uint_as_float(a.p.head->max_g), g = a.p.g_rows[t];
+        // without a finite one above zero: zeros, and what is not finite, which stays so
+        one = top > 0.f ? one * (g / top) : g == 0.f ? 0.f : __int_as_float(0x7fffffff);
     }
     if (tg == kIgnored) one = 0.f;  // its logits are zeros
     const float m = a.p.row_max[t];
