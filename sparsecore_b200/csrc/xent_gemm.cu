@@ -120,9 +120,12 @@ __device__ __forceinline__ void load32(const void* src, uint32_t (&v)[8]) {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// What brings a sum of 32-bit operands' planes back to the logit.
+// What brings a sum of 32-bit operands' planes back to the logit.  Never 0,
+// which would make NaN of the columns behind the last: logits that would need a
+// smaller one are below 2^-76 either way, the planes' sums below 2^50.
 __device__ __forceinline__ float logit_scale(const Problem& p) {
-    return exp2f(static_cast<float>(min(127, -plane_exponent(p.head->max_x) - plane_exponent(p.head->max_w))));
+    const int e = -plane_exponent(p.head->max_x) - plane_exponent(p.head->max_w);
+    return exp2f(static_cast<float>(max(-126, min(127, e))));
 }
 
 // Maximum and sum of exponentials of this thread's row t over 128 columns

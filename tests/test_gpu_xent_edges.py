@@ -34,3 +34,11 @@ def test_gradients_of_single_losses_that_are_not_finite(dtype, V):
         if rest == 0.0:
             assert not dx[20:].any()
         assert not torch.isfinite(dw).any()
+
+
+@gpu
+@pytest.mark.parametrize("V", [200, 300, 384])
+def test_operands_that_are_both_tiny(V):
+    x, w, t = _case(90, 128, V, torch.float32, 2)
+    _check(x * 1e-20, w * 1e-20, t)
+    _check(x * 1e-30, w * 1e-5, t)
