@@ -15,8 +15,8 @@
 // 16-bit inputs are multiplied as they are.  32-bit ones are split into two
 // fp16 planes, a = 2^-k (a_hi + a_lo) with 22 bits between them (2^-k from
 // the operand's largest value), and three products hi.hi, hi.lo, lo.hi are
-// summed in 32 bits: the result is as exact as a 32-bit product's, on the
-// 16-bit matrix units.
+// summed in 32 bits: the result is as exact as a 32-bit product's where the
+// operands' rows are of one order of size, on the 16-bit matrix units.
 #include <algorithm>
 
 #include "xent.cuh"
@@ -141,15 +141,15 @@ planes_kernel(Source q, int64_t dp, const unsigned* part, int x_blocks, int w_bl
     __shared__ unsigned s[kThreads / 32];
     let_follow();
     follow();
-    float scale_x = 1.f, scale_w = 1.f;
+    Factor scale_x{1.f, 1.f}, scale_w{1.f, 1.f};
     if (sizeof(T) == 4) {
         unsigned mx = 0, mw = 0;
         for (int k = threadIdx.x; k < x_blocks; k += kThreads) mx = max(mx, part[k]);
         for (int k = threadIdx.x; k < w_blocks; k += kThreads) mw = max(mw, part[x_blocks + k]);
         mx = block_max(mx, s);
         mw = block_max(mw, s);
-        scale_x = exp2f(static_cast<float>(plane_exponent(mx)));
-        scale_w = exp2f(static_cast<float>(plane_exponent(mw)));
+        scale_x = power_of_two(plane_exponent(mx));
+        scale_w = power_of_two(plane_exponent(mw));
         if (blockIdx.x == 0 && threadIdx.x == 0) head->max_x = mx, head->max_w = mw;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) head->done = 0;
@@ -159,7 +159,7 @@ planes_kernel(Source q, int64_t dp, const unsigned* part, int x_blocks, int w_bl
         const int64_t row = is_w ? r - q.T : r;
         const bool on = is_w || q.targets[row] != q.ignore;
         const T* src = static_cast<const T*>(is_w ? q.w : q.x) + row * q.D;
-        const float scale = is_w ? scale_w : scale_x;
+        const Factor scale = is_w ? scale_w : scale_x;
         const int64_t plane = (is_w ? q.V : q.T) * dp;
         uint16_t* dst = static_cast<uint16_t*>(is_w ? wp : xp) + row * dp;
         for (int64_t c = lane_id() * 8; c < dp; c += 256) {
@@ -176,7 +176,7 @@ planes_kernel(Source q, int64_t dp, const unsigned* part, int x_blocks, int w_bl
                 float lo[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    v[k] *= scale;
+                    v[k] = v[k] * scale.a * scale.b;
                     lo[k] = v[k] - __half2float(__float2half_rn(v[k]));
                 }
                 store_f<__half, 8>(reinterpret_cast<__half*>(dst) + c, v);

@@ -46,13 +46,24 @@ struct Header {
 
 enum : int { kIgnored = -1, kInvalid = -2 };  // in place of a target
 
-// Power of two that brings values of up to `bits` (a float's bits) below
-// 2^15, where fp16 holds what is down to 2^-29 of it at full precision.
+// Exponent of the power of two that brings values of up to `bits` (a float's
+// bits, subnormal ones too) into [2^14, 2^15): -113 to 163.  Two fp16 planes
+// then hold 22 bits of what is down to 2^-17 of the largest, and 2^-39 of the
+// largest of what is smaller: an operand is as exact as its largest values ask
+// for, not element by element.
 __device__ __forceinline__ int plane_exponent(unsigned bits) {
-    const int e = static_cast<int>(bits >> 23);
-    if (e == 0) return 0;
-    const int k = 14 - (e - 127);
-    return k > 100 ? 100 : k < -100 ? -100 : k;
+    if (bits == 0) return 0;
+    return 14 - (bits >= 0x800000u ? static_cast<int>(bits >> 23) - 127 : -118 - __clz(bits));
+}
+
+// a * b, the second 1 but where the product is beyond a float's exponents.
+struct Factor {
+    float a, b;
+};
+__device__ __forceinline__ float pow2(int k) { return __int_as_float((k + 127) << 23); }  // -126 <= k <= 127
+__device__ __forceinline__ Factor power_of_two(int k) {  // -252 <= k <= 254
+    const int h = max(-126, min(127, k));
+    return {pow2(h), pow2(k - h)};
 }
 
 // One operand: planes of [rows, stride] 16-bit values whose sum is it.

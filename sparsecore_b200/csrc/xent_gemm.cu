@@ -123,9 +123,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // What brings a sum of 32-bit operands' planes back to the logit.  Never 0,
 // which would make NaN of the columns behind the last: logits that would need a
 // smaller one are below 2^-76 either way, the planes' sums below 2^50.
-__device__ __forceinline__ float logit_scale(const Problem& p) {
-    const int e = -plane_exponent(p.head->max_x) - plane_exponent(p.head->max_w);
-    return exp2f(static_cast<float>(max(-126, min(127, e))));
+__device__ __forceinline__ Factor logit_scale(const Problem& p) {
+    return power_of_two(max(-126, -plane_exponent(p.head->max_x) - plane_exponent(p.head->max_w)));
 }
 
 // Maximum and sum of exponentials of this thread's row t over 128 columns
@@ -287,12 +286,16 @@ __device__ __forceinline__ void finish_losses(const Args& a, Shared& sh, double 
 }
 
 // What is multiplied into a finished sum.
-__device__ __forceinline__ float out_scale(const Problem& p, bool by_x, bool f32) {
+__device__ __forceinline__ Factor out_scale(const Problem& p, bool by_x, bool f32) {
     float g = p.g_rows ? __uint_as_float(p.head->max_g) : *p.grad;
     if (p.mean) g = p.head->count ? g / static_cast<float>(p.head->count) : 0.f;
-    if (!p.bf16) g *= 1.f / kGradScale;
-    return f32 ? g * exp2f(-static_cast<float>(plane_exponent(by_x ? p.head->max_x : p.head->max_w))) : g;
+    if (!f32) return {p.bf16 ? g : g * (1.f / kGradScale), 1.f};
+    const double s = scalbn(static_cast<double>(g), -15 - plane_exponent(by_x ? p.head->max_x : p.head->max_w));
+    if (s != 0.0 && fabs(s) < 0x1p-126) return {static_cast<float>(s * 0x1p100), 0x1p-100f};
+    if (fabs(s) >= 0x1p128 && isfinite(g)) return {static_cast<float>(s * 0x1p-100), 0x1p100f};
+    return {static_cast<float>(s), 1.f};
 }
+static_assert(kGradScale == 32768.f, "2^15 in out_scale");
 
 __device__ __forceinline__ void store_out(const Output& o, int64_t i, float v) {
     if (o.dtype == SL_F32) static_cast<float*>(o.dst)[i] = v;
@@ -300,7 +303,7 @@ __device__ __forceinline__ void store_out(const Output& o, int64_t i, float v) {
     else static_cast<__half*>(o.dst)[i] = __float2half_rn(v);
 }
 
-__device__ __forceinline__ void epilogue_out(const Args& a, float (&z)[128], int64_t m, int64_t n0, int split, float scale) {
+__device__ __forceinline__ void epilogue_out(const Args& a, float (&z)[128], int64_t m, int64_t n0, int split, Factor by) {
     if (m >= a.M) return;
     if (a.splits > 1) {
         float* dst = a.o.slabs + split * a.slab_stride + m * (static_cast<int64_t>(a.tiles_n) * kTile) + n0;
@@ -341,6 +344,12 @@ __device__ __forceinline__ void epilogue_out(const Args& a, float (&z)[128], int
                 }
         }
         if (!a.o.last) return;
+    }
+    float scale = by.a;
+    if (by.b != 1.f) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j) z[j] = z[j] * by.a * by.b;
+        scale = 1.f;
     }
     const int64_t bytes = a.o.dtype == SL_F32 ? 4 : 2;
     char* dst = static_cast<char*>(a.o.dst) + row * bytes;
@@ -496,7 +505,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-        const float u = MODE == kOut ? out_scale(a.p, a.o.by_x, PL == 2) : PL == 2 ? logit_scale(a.p) : 1.f;
+        const Factor u = MODE == kOut ? out_scale(a.p, a.o.by_x, PL == 2) : PL == 2 ? logit_scale(a.p) : Factor{1.f, 1.f};
         uint32_t done = 0;
         bool ok = true;
         double loss = 0.0;
@@ -527,9 +536,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             if (!ok) break;
             const int64_t t = static_cast<int64_t>(tm) * kTile + rank * 128 + quarter * 32 + lane;
             const int64_t n0 = static_cast<int64_t>(tn) * kTile + half * 128;
-            if (MODE == kStats) epilogue_stats(a, z, t, n0, u);
-            else if (MODE == kGrad) epilogue_grad<PL>(a, z, t, n0, u);
-            else if (MODE == kLosses) epilogue_losses<PL>(a, sh, z, t, quarter * 32 + lane, half, u, loss, count);
+            if (MODE != kOut && PL == 2 && u.b != 1.f) {
+#pragma unroll
+                for (int j = 0; j < 128; ++j) z[j] *= u.b;
+            }
+            if (MODE == kStats) epilogue_stats(a, z, t, n0, u.a);
+            else if (MODE == kGrad) epilogue_grad<PL>(a, z, t, n0, u.a);
+            else if (MODE == kLosses) epilogue_losses<PL>(a, sh, z, t, quarter * 32 + lane, half, u.a, loss, count);
             else epilogue_out(a, z, t, n0, split, u);
         }
         if (MODE == kLosses && ok) finish_losses(a, sh, loss, count);
@@ -548,7 +561,7 @@ __global__ void __launch_bounds__(256)
 join_kernel(Problem p, Output o, int64_t M, int64_t N, int64_t stride, int64_t slab, int splits, bool f32) {
     let_follow();
     follow();
-    const float scale = out_scale(p, o.by_x, f32);
+    const Factor scale = out_scale(p, o.by_x, f32);
     const int64_t step = static_cast<int64_t>(gridDim.x) * 256 * W;
     const int across = static_cast<int>(N);
     for (int64_t i = (blockIdx.x * static_cast<int64_t>(256) + threadIdx.x) * W; i < M * N; i += step) {
@@ -577,7 +590,7 @@ join_kernel(Problem p, Output o, int64_t M, int64_t N, int64_t stride, int64_t s
         }
         if (o.last) {
 #pragma unroll
-            for (int k = 0; k < W; ++k) store_out(o, i + k, v[k] * scale);
+            for (int k = 0; k < W; ++k) store_out(o, i + k, v[k] * scale.a * scale.b);
         }
     }
 }

@@ -42,3 +42,37 @@ def test_operands_that_are_both_tiny(V):
     x, w, t = _case(90, 128, V, torch.float32, 2)
     _check(x * 1e-20, w * 1e-20, t)
     _check(x * 1e-30, w * 1e-5, t)
+
+
+@gpu
+@pytest.mark.parametrize("V", [200, 700])
+def test_operands_near_the_ends_of_the_range(V):
+    x, w, t = _case(90, 128, V, torch.float32, 3)
+    for size in (1e33, 1e35):
+        _check(x * size, w / size, t)
+        _check(x / size, w * size, t)
+    for size in (1e37, 1e40):  # subnormal on one side: the losses
+        small = w.double() / size
+        _check(x * 1e37, small.float(), t, need=(False, False))
+        _check((x.double() / size).float(), w * 1e37, t, need=(False, False))
+    _check(x * 1e-35, w * 1e-35, t, need=(False, False))
+    _check(x * 1e-43, w, t, need=(False, False))
+
+
+@gpu
+@pytest.mark.parametrize("V", [200, 700])
+def test_gradients_that_need_both_ends(V):
+    """The weight is subnormal and the gradient that comes in large, or the other way round: what goes out is in
+    the middle of the range.  dx = grad * (softmax - onehot) . w; at a constant x every softmax is 1 / V."""
+    import sparsecore_b200 as sl
+
+    g = torch.Generator().manual_seed(4)
+    w = (torch.randn(V, 64, generator=g).double() * 1e-38).float().to(dev())
+    x = torch.zeros(50, 64, device=dev(), requires_grad=True)
+    t = torch.randint(0, V, (50,), generator=g).to(dev())
+    for grad, weight in ((1e30, w), (1e-30, w * 1e30 * 1e38)):
+        (dx,) = torch.autograd.grad(sl.linear_cross_entropy(x, weight, t, reduction="sum"), (x,), torch.tensor(grad, device=dev()))
+        ref = grad * (weight.double().mean(0) - weight.double()[t])
+        # 2^-22 an operand, and sums of V
+        lim = (16 + V / 8) * 2.0 ** -24 * grad * (weight.double().abs().mean(0) + weight.double()[t].abs()) + 2.0 ** -39 * grad * float(weight.abs().max()) * V
+        assert bool(((dx.double() - ref).abs() <= lim).all())
