@@ -148,8 +148,9 @@ __device__ __forceinline__ void epilogue_stats(const Args& a, float (&z)[128], i
 #pragma unroll
     for (int j = 0; j < 128; ++j) m = fmaxf(m, z[j]);
     m *= u;
+    const float from = m == -INFINITY ? 0.f : m;  // of logits that are all -inf the sum is 0
 #pragma unroll
-    for (int j = 0; j < 128; ++j) s[j & 3] += exp2_fast(fmaf(z[j], u, -m) * kLog2e);
+    for (int j = 0; j < 128; ++j) s[j & 3] += exp2_fast(fmaf(z[j], u, -from) * kLog2e);
     a.p.part[n0 / kPart * a.M + t] = make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
 }
 

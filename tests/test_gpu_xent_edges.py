@@ -76,3 +76,17 @@ def test_gradients_that_need_both_ends(V):
         # 2^-22 an operand, and sums of V
         lim = (16 + V / 8) * 2.0 ** -24 * grad * (weight.double().abs().mean(0) + weight.double()[t].abs()) + 2.0 ** -39 * grad * float(weight.abs().max()) * V
         assert bool(((dx.double() - ref).abs() <= lim).all())
+
+
+@gpu
+def test_columns_whose_logits_are_minus_infinity():
+    """A stretch of the vocabulary that cannot be chosen adds nothing to the sum."""
+    import sparsecore_b200 as sl
+
+    x, w, t = _case(60, 64, 1000, torch.bfloat16, 5, ignored=0)
+    x = x.abs() + 0.01
+    w[300:] = -math.inf
+    t = t % 300
+    got = sl.linear_cross_entropy(x, w, t, reduction="none")
+    want = sl.linear_cross_entropy(x, w[:300].contiguous(), t, reduction="none")
+    assert bool(((got - want).abs() <= 16 * 2.0 ** -24 * (1 + want.abs())).all())
