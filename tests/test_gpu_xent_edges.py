@@ -90,3 +90,26 @@ def test_columns_whose_logits_are_minus_infinity():
     got = sl.linear_cross_entropy(x, w, t, reduction="none")
     want = sl.linear_cross_entropy(x, w[:300].contiguous(), t, reduction="none")
     assert bool(((got - want).abs() <= 16 * 2.0 ** -24 * (1 + want.abs())).all())
+
+
+@gpu
+def test_long_sums_of_one_sign_do_not_drift():
+    """2^18 tokens with one target: dW is a sum of terms of one sign, and cutting
+    at each addition would show as a drift of n / 4 steps of 2^-23 (n sums of 16).
+    softmax is 1 / 1024 everywhere, so the target's gradient -1023/1024 is held
+    exactly; what is left is the output's rounding, which has no sign: over 4096
+    columns its mean is below 2^-12 / 64 * 4."""
+    import sparsecore_b200 as sl
+
+    T, D, V = 1 << 18, 4096, 1024
+    g = torch.Generator(device=dev()).manual_seed(6)
+    x = torch.rand(T, D, generator=g, device=dev(), dtype=torch.float16).add_(0.5).requires_grad_(False)
+    w = torch.zeros(V, D, device=dev(), dtype=torch.float16, requires_grad=True)
+    t = torch.full((T,), 7, dtype=torch.int64, device=dev())
+    (dw,) = torch.autograd.grad(sl.linear_cross_entropy(x, w, t), (w,))
+    total = torch.zeros(D, dtype=torch.float64, device=dev())
+    for a in range(0, T, 8192):
+        total += x[a:a + 8192].double().sum(0)
+    ref = -1023 / 1024 * total / T
+    drift = float(((dw[7].double() - ref) / ref).mean())
+    assert abs(drift) <= 2.0 ** -16, drift
