@@ -43,6 +43,15 @@ def _sizes(x, weight, reduction, train):
                      weight.data_ptr() & 15)
 
 
+def _laid_like(weight, off):
+    """The weight at an address that is on 16 bytes, or is not, as it was in the forward call: that call's kept buffer is laid
+    out by it.  (Hooks on saved tensors may bring it back elsewhere.)"""
+    if (weight.data_ptr() & 15 != 0) == off:
+        return weight
+    n = weight.numel()
+    return torch.empty(n + off, dtype=weight.dtype, device=weight.device)[int(off):].view(weight.shape).copy_(weight)
+
+
 def _buffer(n, device):
     return torch.empty(n, dtype=torch.uint8, device=device)
 
@@ -74,7 +83,8 @@ def _forward(x, weight, targets, ignore_index, reduction, train):
 
 def _backward(ctx, grad):
     x, weight, targets, prep = ctx.saved_tensors
-    ignore_index, reduction, shape = ctx.opts
+    ignore_index, reduction, shape, off = ctx.opts
+    weight = _laid_like(weight, off)
     need = ctx.needs_input_grad
     dev = x.device
     dx = torch.empty(shape, dtype=x.dtype, device=dev) if need[0] else None
@@ -102,7 +112,7 @@ class _LinearCrossEntropyFunction(torch.autograd.Function):
     def forward(ctx, x, weight, targets, ignore_index, reduction):
         loss, saved = _forward(x, weight, targets, ignore_index, reduction, 1)
         ctx.save_for_backward(*saved)
-        ctx.opts = (ignore_index, reduction, x.shape)
+        ctx.opts = (ignore_index, reduction, x.shape, saved[1].data_ptr() & 15 != 0)
         return loss
 
     @staticmethod

@@ -113,3 +113,29 @@ def test_long_sums_of_one_sign_do_not_drift():
     ref = -1023 / 1024 * total / T
     drift = float(((dw[7].double() - ref) / ref).mean())
     assert abs(drift) <= 2.0 ** -16, drift
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [70, 600])
+@pytest.mark.parametrize("was,now", [(0, 1), (1, 0), (0, 0), (1, 1)])
+def test_saved_tensors_that_come_back_elsewhere(dtype, V, was, now):
+    """Hooks may put what is kept for the backward pass away and bring it back at another address."""
+    import sparsecore_b200 as sl
+
+    def at(v, off):
+        n = v.numel()
+        return torch.empty(n + 8, dtype=v.dtype, device=dev())[off:off + n].view(v.shape).copy_(v)
+
+    x, w, t = _case(130, 64, V, dtype, 8)
+    xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+    want = torch.autograd.grad(sl.linear_cross_entropy(xr, wr, t), (xr, wr))
+    xl, wl = at(x, was).requires_grad_(), at(w, was).requires_grad_()
+
+    def back(v):
+        return at(v.to(dev()), now) if v.dim() == 2 else v.to(dev())
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: v.cpu(), back):
+        loss = sl.linear_cross_entropy(xl, wl, t)
+    got = torch.autograd.grad(loss, (xl, wl))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
