@@ -38,7 +38,7 @@ struct Layout {
 
 int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
-Layout layout(int64_t T, int64_t D, int64_t V, int dtype, bool copy_x, bool copy_w, bool one_tile) {
+Layout layout(int64_t T, int64_t D, int64_t V, int dtype, bool copy_x, bool copy_w, bool keep_g) {
     Layout l{};
     const int64_t planes = dtype == SL_F32 ? 2 : 1;
     l.dp = up(D, 64);
@@ -48,7 +48,7 @@ Layout layout(int64_t T, int64_t D, int64_t V, int dtype, bool copy_x, bool copy
     l.row_inv = take(4 * T);
     l.x = take(copy_x ? planes * T * l.dp * 2 : 0);
     l.w = take(copy_w ? planes * V * l.dp * 2 : 0);
-    if (one_tile) l.g = take(planes * T * up(V, 64) * 2);
+    if (keep_g) l.g = take(planes * T * up(V, 64) * 2);
     l.prep = o;
     o = 0;
     l.zt = take(4 * T);
@@ -66,7 +66,7 @@ Layout layout(int64_t T, int64_t D, int64_t V, int dtype, bool copy_x, bool copy
     const int64_t pieces = std::max<int64_t>(1, (V + most - 1) / most);
     l.piece = up((V + pieces - 1) / pieces, 256);
     l.gp = up(std::min(l.piece, V), 64);
-    if (!one_tile) l.g = take(planes * T * l.gp * 2);
+    if (!keep_g) l.g = take(planes * T * l.gp * 2);
     l.acc = take(V > l.piece ? 4 * T * D : 0);
     const bool two = dtype == SL_F32;
     const int64_t rest = V - (V - 1) / l.piece * l.piece;  // of the last piece
@@ -294,7 +294,7 @@ bool one_tile(const sl_xent_args& a) {
     return a.vocab <= kOneTile && copies_x(a) && !(a.train && a.reduction == SL_XENT_NONE);
 }
 Layout layout(const sl_xent_args& a) {
-    return layout(std::max<int64_t>(a.tokens, 1), a.dim, a.vocab, a.dtype, copies_x(a), copies_w(a), one_tile(a));
+    return layout(std::max<int64_t>(a.tokens, 1), a.dim, a.vocab, a.dtype, copies_x(a), copies_w(a), a.train && one_tile(a));
 }
 
 int check(const sl_xent_args* a, const char* fn) {

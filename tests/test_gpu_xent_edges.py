@@ -139,3 +139,13 @@ def test_saved_tensors_that_come_back_elsewhere(dtype, V, was, now):
         loss = sl.linear_cross_entropy(xl, wl, t)
     got = torch.autograd.grad(loss, (xl, wl))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+def test_a_call_without_gradients_keeps_no_room_for_them():
+    """Of a vocabulary of one tile only a training call keeps the logits' gradient."""
+    from sparsecore_b200 import loss as L
+
+    x, w = torch.zeros(20000, 64, device=dev()), torch.zeros(200, 64, device=dev())
+    kept = {train: L._sizes(x, w, 0, train)[0] for train in (0, 1)}
+    assert kept[1] - kept[0] >= 20000 * 200 * 2 * 2
