@@ -297,12 +297,16 @@ Layout layout(const sl_xent_args& a) {
     return layout(std::max<int64_t>(a.tokens, 1), a.dim, a.vocab, a.dtype, copies_x(a), copies_w(a), a.train && one_tile(a));
 }
 
-int check(const sl_xent_args* a, const char* fn) {
+int check_shape(const sl_xent_args* a, const char* fn) {
     SL_REQUIRE(a != nullptr, fn, "NULL arguments");
     SL_REQUIRE(known_dtype(a->dtype), fn, "unknown dtype");
     SL_REQUIRE(a->tokens >= 0 && a->dim >= 1 && a->vocab >= 1, fn, "negative or empty shape");
     SL_REQUIRE(a->tokens <= INT_MAX / 2 && a->dim <= (1 << 20) && a->vocab <= INT_MAX / 2, fn, "shape beyond 2^30 rows or 2^20 columns");
     SL_REQUIRE(a->reduction >= SL_XENT_MEAN && a->reduction <= SL_XENT_NONE, fn, "unknown reduction");
+    return SL_OK;
+}
+int check(const sl_xent_args* a, const char* fn) {
+    if (int rc = check_shape(a, fn)) return rc;
     if (a->tokens == 0) return SL_OK;
     SL_REQUIRE(a->x && a->weight && a->targets && a->prep && a->scratch, fn, "NULL operand");
     SL_REQUIRE(!off_by(a->x, dtype_bytes(a->dtype)) && !off_by(a->weight, dtype_bytes(a->dtype)) && !off_by(a->targets, 8) &&
@@ -422,8 +426,8 @@ using namespace slb;
 
 extern "C" int sl_xent_sizes(const sl_xent_args* a, int64_t* prep, int64_t* forward, int64_t* backward) {
     const char* fn = "sl_xent_sizes";
-    SL_REQUIRE(a && prep && forward && backward, fn, "NULL argument");
-    SL_REQUIRE(known_dtype(a->dtype) && a->tokens >= 0 && a->dim >= 1 && a->vocab >= 1, fn, "bad shape or type");
+    SL_REQUIRE(prep && forward && backward, fn, "NULL argument");
+    if (int rc = xent::check_shape(a, fn)) return rc;
     const xent::Layout l = xent::layout(*a);
     *prep = l.prep;
     *forward = l.fwd;
