@@ -12,6 +12,7 @@ import struct
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "libsparsecore_b200.so")
@@ -149,6 +150,13 @@ def require_cuda(device: torch.device | None = None) -> torch.device:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def refuse_tangents(fn: str, *tensors) -> None:
+    """Raises where one of the tensors carries a forward-mode tangent: the kernels read values alone, and a result
+    without its tangent would be wrong in silence."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{fn}: forward-mode derivatives are not implemented")
 
 
 def stream_ptr(device: torch.device) -> P:

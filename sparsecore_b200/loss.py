@@ -133,8 +133,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     where none does, with gradients of zero), "sum", or "none" (a loss for each
     token, 0 for ignored ones).  The loss is float32.
 
-    Raises TypeError (not tensors), RuntimeError (not on one CUDA device) and
-    ValueError (shapes, types, reduction).
+    Raises TypeError (not tensors), RuntimeError (not on one CUDA device,
+    forward-mode derivatives) and ValueError (shapes, types, reduction).
     """
     for t, name in ((x, "x"), (weight, "weight"), (targets, "targets")):
         if not isinstance(t, torch.Tensor):
@@ -160,6 +160,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
         raise ValueError(f"linear_cross_entropy: targets must have shape {tuple(x.shape[:-1])}, got {tuple(targets.shape)}")
     if weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"linear_cross_entropy: weight must not be empty, got {tuple(weight.shape)}")
+    N.refuse_tangents("linear_cross_entropy", x, weight)
     code = _REDUCTIONS[reduction]
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         loss = _LinearCrossEntropyFunction.apply(x, weight, targets, int(ignore_index), code)

@@ -159,8 +159,8 @@ def residual_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
     per sequence).  ``scale``: a number, or a float32 CUDA tensor of one element
     (a learned scale).
 
-    Raises TypeError (not tensors), RuntimeError (not on one CUDA device) and
-    ValueError (shapes, types, kind).
+    Raises TypeError (not tensors), RuntimeError (not on one CUDA device,
+    forward-mode derivatives) and ValueError (shapes, types, kind).
     """
     for t, name in ((y, "y"), (residual, "residual"), (weight, "weight")):
         if not isinstance(t, torch.Tensor):
@@ -218,6 +218,7 @@ def residual_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
         if scale.numel() != 1 or scale.dtype != torch.float32:
             raise ValueError("residual_norm: a tensor scale must be one float32 element")
         scale, scale_t = 1.0, scale
+    N.refuse_tangents("residual_norm", y, residual, weight, bias, gate, scale_t, post_weight, post_bias)
     opts = (_KINDS[kind], eps, post_eps, float(scale))
     if torch.is_grad_enabled() and (
             y.requires_grad or residual.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)

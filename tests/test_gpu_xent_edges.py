@@ -149,3 +149,23 @@ def test_a_call_without_gradients_keeps_no_room_for_them():
     x, w = torch.zeros(20000, 64, device=dev()), torch.zeros(200, 64, device=dev())
     kept = {train: L._sizes(x, w, 0, train)[0] for train in (0, 1)}
     assert kept[1] - kept[0] >= 20000 * 200 * 2 * 2
+
+
+@gpu
+def test_forward_mode_is_refused():
+    """Tangents have no way through; a result without one would be wrong in silence."""
+    import torch.autograd.forward_ad as fw
+
+    import sparsecore_b200 as sl
+
+    x, w, t = _case(8, 16, 20, torch.float32, 9)
+    n = torch.ones(16, device=dev())
+    with fw.dual_level():
+        d, dw, dn = (fw.make_dual(v, torch.ones_like(v)) for v in (x, w, n))
+        for call in (lambda: sl.linear_cross_entropy(d, w, t), lambda: sl.linear_cross_entropy(x, dw, t),
+                     lambda: sl.residual_norm(d, x, n), lambda: sl.residual_norm(x, x, n, gate=dn),
+                     lambda: sl.residual_norm(x, x, n, scale=fw.make_dual(torch.ones(1, device=dev()), torch.ones(1, device=dev())))):
+            with pytest.raises(RuntimeError, match="forward"):
+                call()
+        sl.linear_cross_entropy(x, w, t)  # what has no tangent goes through
+        sl.residual_norm(x, x, n)
