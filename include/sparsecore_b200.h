@@ -374,8 +374,8 @@ enum { SL_F32 = 0, SL_BF16 = 1, SL_F16 = 2 };
 
 /* One tensor of an AdamW step.  m and v are float[n] (state_bits 32) or
  * e4m3 bytes [n] with one fp32 scale per SL_ADAMW_BLOCK elements in scale_m
- * and scale_v, v then holding the second moment's square root (state_bits
- * 8).  live: int32[n] column indices of a padded CSR (slots below 0 are left
+ * and scale_v, v then holding the second moment's square root, the byte 0xFF
+ * an infinite one (state_bits 8).  live: int32[n] column indices of a padded CSR (slots below 0 are left
  * alone), or NULL.  number: the tensor's number in the caller's list, which
  * its dither bits depend on. */
 enum { SL_ADAMW_BLOCK = 256 };

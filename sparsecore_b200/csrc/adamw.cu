@@ -12,7 +12,9 @@
 // rounded up or down by 16 dither bits instead (a hash of the element's
 // number, the tensor's number, the step and the caller's seed), which keeps
 // every moment right on average.  A root above zero is never held as zero:
-// its element's next update would be divided by eps alone.
+// its element's next update would be divided by eps alone.  What is not finite
+// is held as NaN, an infinite root (of a gradient whose square passes 32 bits)
+// as the byte 0xFF: m / root is 0 then, as with 32-bit moments.
 //
 // 32-bit moments are bound by memory: 12.2 M weights in padded arrays (32
 // bytes a slot, padding read too) take 67 us, 5.8 TB/s.  8-bit ones are bound
@@ -91,7 +93,8 @@ __device__ __forceinline__ void store(T* dst, int64_t i, int left, bool vec, con
 
 // Square roots to half a step but for rare cases (one Newton step on an
 // approximate 1 / root, so that what the 8-bit values are cut from is as exact
-// as a 32-bit number can be); of a subnormal number 0.
+// as a 32-bit number can be).  Of infinity NaN; of a subnormal number, which the
+// approximation takes for 0, up to 0x1p-62 (see kExactBelow).
 __device__ __forceinline__ void roots(float (&v)[kPer]) {
     float y[kPer], r[kPer], e[kPer];
 #pragma unroll
@@ -217,13 +220,22 @@ __device__ __forceinline__ void step32(const Item& d, const Hyper& h, int64_t i,
     store(V, i, left, vv, v);
 }
 
+// Blocks with second moments that are subnormal or infinite take a path of
+// their own with each root rounded: a call with nothing kept over it, since what
+// it needs would be taken from every other block's registers (335 M bf16
+// weights: 874 us without it, 881 so, 931 inlined).  A block takes it where it
+// has something that is not finite, where its largest root is below 0x1p-44, or
+// where eps would not hide a root below 0x1p-62 from the update.  Beside a root of
+// 0x1p-44 such a one is held as the smallest 8-bit value, whatever its digits are.
+constexpr float kExactBelow = 0x1p-44f, kExactEps = 1e-12f;
+
 // Eight elements of a block with 8-bit moments; a warp has the whole block.
 // The kernel is bound by its instructions as much as by its bytes (10 of a
 // 16-bit weight), so the quotient is an approximate one (2^-22 of p's update),
 // and padding, ends and odd addresses are kept out of the
 // ordinary path.
-template <typename T, bool PLAIN>
-__device__ __forceinline__ void step8(const Item& d, const Hyper& h, uint32_t key, int64_t i, int64_t block, int left) {
+template <typename T, bool PLAIN, bool EXACT = false>
+__device__ __forceinline__ bool step8(const Item& d, const Hyper& h, uint32_t key, int64_t i, int64_t block, int left) {
     T* P = static_cast<T*>(d.p);
     const T* G = static_cast<const T*>(d.g);
     uint8_t* M = static_cast<uint8_t*>(d.m) + i;
@@ -239,6 +251,11 @@ __device__ __forceinline__ void step8(const Item& d, const Hyper& h, uint32_t ke
     const uint32_t on = PLAIN ? 0xFFu : taking_part(d.live, i, left);
     from_e4m3(cm, m);
     from_e4m3(cu, u);
+    if constexpr (EXACT) {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+            if (((k < 4 ? cu.x : cu.y) >> (8 * (k & 3)) & 0xFF) == 0xFF) u[k] = INFINITY;
+    }
     // Each step is rounded by itself, in the formula's order: the 8-bit values
     // are then those of the formula in 32-bit operations, and not now and then
     // their neighbours.  (The additions one by one: in pairs they would be made
@@ -257,7 +274,12 @@ __device__ __forceinline__ void step8(const Item& d, const Hyper& h, uint32_t ke
         m1[k] = __fadd_rn(m[k], m1[k]);
         root[k] = __fadd_rn(root[k], g[k]);
     }
-    roots(root);
+    if constexpr (EXACT) {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) root[k] = sqrtf(root[k]);
+    } else {
+        roots(root);
+    }
     vfma(q, root, h.inv_root, h.eps);
 #pragma unroll
     for (int k = 0; k < kPer; ++k) q[k] = rcp_fast(q[k]);
@@ -283,21 +305,25 @@ __device__ __forceinline__ void step8(const Item& d, const Hyper& h, uint32_t ke
         tm = max_nan(tm, fabsf(m[k]));
         tu = max_nan(tu, u[k]);
     }
-    store(P, i, left, pv, p);
     // the largest magnitudes' bits: what is not finite is above all that is
     uint32_t bm = __reduce_max_sync(0xffffffffu, __float_as_uint(tm)), bu = __reduce_max_sync(0xffffffffu, __float_as_uint(tu));
-    uint32_t bad = 0;  // elements that are not finite: held as NaN, and no part of the scales
-    if (bm >= 0x7F800000u || bu >= 0x7F800000u) {
+    uint32_t bad = 0;
+    if constexpr (EXACT) {  // elements that are not finite are no part of the scales: held as NaN, an infinite root as 0xFF
         bm = bu = 0;
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
             const uint32_t a = __float_as_uint(m[k]) & 0x7FFFFFFFu, b = __float_as_uint(u[k]) & 0x7FFFFFFFu;
             if (a >= 0x7F800000u) bad |= 1u << k, m[k] = 0.f; else bm = max(bm, a);
-            if (b >= 0x7F800000u) bad |= 256u << k, u[k] = 0.f; else bu = max(bu, b);
+            if (b >= 0x7F800000u) bad |= (b == 0x7F800000u ? 0x10000u : 0x100u) << k, u[k] = 0.f; else bu = max(bu, b);
         }
         bm = __reduce_max_sync(0xffffffffu, bm);
         bu = __reduce_max_sync(0xffffffffu, bu);
+    } else {
+        const uint32_t low = h.eps < kExactEps ? 0x7F800000u : __float_as_uint(kExactBelow);
+        if (bm >= 0x7F800000u || bu - low >= 0x7F800000u - low)
+            if (bu != 0 || bm >= 0x7F800000u) return false;
     }
+    store(P, i, left, pv, p);
     const float fm = fmaxf(__uint_as_float(bm), 0x1p-100f), fu = fmaxf(__uint_as_float(bu), 0x1p-100f);
     const float im = __frcp_rn(fm) * 448.f, iu = __frcp_rn(fu) * 448.f;
     const uint32_t first = static_cast<uint32_t>(i) * 0x9E3779B1u + key;
@@ -323,24 +349,42 @@ __device__ __forceinline__ void step8(const Item& d, const Hyper& h, uint32_t ke
         m[k] = copysignf(am[k], m[k]);
         u[k] = fmaxf(u[k], floor[k]);
     }
-    if (bad) {
+    if (EXACT && bad) {
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
             if (bad >> k & 1) m[k] = __int_as_float(0x7fffffff);
             if (bad >> (8 + k) & 1) u[k] = __int_as_float(0x7fffffff);
         }
     }
+    uint2 held = to_e4m3(u);
+    if constexpr (EXACT) {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+            if (bad >> (16 + k) & 1) (k < 4 ? held.x : held.y) |= 0xFFu << (8 * (k & 3));
+    }
     store8(M, left, mv, to_e4m3(m));
-    store8(U, left, uv, to_e4m3(u));
+    store8(U, left, uv, held);
     if (lane_id() == 0) {
         d.sm[block] = fm * (1.f / 448.f);
         d.su[block] = fu * (1.f / 448.f);
     }
+    return true;
+}
+
+// Key of a tensor's dither.
+__device__ __forceinline__ uint32_t dither_key(const Hyper& h, const Item& d) { return mix32(h.key + 0x85EBCA77u * d.number); }
+
+template <typename T>
+__device__ __noinline__ void step8_exact(const Item& d, Hyper h, int64_t tile) {
+    const int64_t block = (tile - d.first) * (kTile / kBlock) + (threadIdx.x >> 5), i = (tile - d.first) * kTile + threadIdx.x * kPer;
+    const int64_t rest = d.n - i;
+    step8<T, false, true>(d, h, dither_key(h, d), i, block, rest >= kPer ? kPer : rest > 0 ? static_cast<int>(rest) : 0);
 }
 
 template <typename T, bool EIGHT, int MAX>
 __global__ void __launch_bounds__(kThreads, 4)
-adamw_multi_kernel(const __grid_constant__ Table<MAX> t, Hyper h, const Hyper* dev) {
+adamw_multi_kernel(const __grid_constant__ Table<MAX> t, const Hyper host, const Hyper* dev) {
+    Hyper h = host;
     if (dev) h = *dev;
     int at = 0;
     int64_t end = 0;
@@ -353,7 +397,7 @@ adamw_multi_kernel(const __grid_constant__ Table<MAX> t, Hyper h, const Hyper* d
                 if (t.item[mid].first <= tile) at = mid; else hi = mid;
             }
             end = at + 1 < t.count ? t.item[at + 1].first : t.tiles;
-            key = mix32(h.key + 0x85EBCA77u * t.item[at].number);
+            key = dither_key(h, t.item[at]);
         }
         const Item& d = t.item[at];
         const int64_t i = (tile - d.first) * kTile + threadIdx.x * kPer;
@@ -362,8 +406,15 @@ adamw_multi_kernel(const __grid_constant__ Table<MAX> t, Hyper h, const Hyper* d
         const int left = rest >= kPer ? kPer : rest > 0 ? static_cast<int>(rest) : 0;
         if constexpr (EIGHT) {
             const int64_t block = (tile - d.first) * (kTile / kBlock) + (threadIdx.x >> 5);
-            if (full && d.plain) step8<T, true>(d, h, key, i, block, kPer);
-            else if (block * kBlock < d.n) step8<T, false>(d, h, key, i, block, left);
+            bool done = true;
+            if (full && d.plain) done = step8<T, true>(d, h, key, i, block, kPer);
+            else if (block * kBlock < d.n) done = step8<T, false>(d, h, key, i, block, left);
+            if (!done) {
+                step8_exact<T>(d, h, tile);
+                h = host;  // made again, as the tensor is, so that nothing is kept over the call
+                if (dev) h = *dev;
+                at = 0, end = 0;
+            }
         } else {
             if (full && d.plain) step32<T, true>(d, h, i, kPer);
             else if (left) step32<T, false>(d, h, i, left);

@@ -101,7 +101,7 @@ class AdamWPlan:
     all float8_e4m3fn with ``scales``: a pair of float32 tensors per parameter,
     one value per 256 elements.  In 8 bits an element is its e4m3 value times
     its block's scale, and ``exp_avg_sqs`` hold the second moments' square
-    roots (see ``sl_adamw_multi``).  ``live``: per parameter None, or the int32
+    roots, the byte 0xFF for an infinite one (see ``sl_adamw_multi``).  ``live``: per parameter None, or the int32
     column indices of a padded CSR whose slots below 0 are left alone, value
     and moments.  ``numbers``: the parameters' numbers that the 8-bit moments'
     dither depends on, where the list is part of a longer one (default: 0, 1, ...).
@@ -499,5 +499,7 @@ class FusedAdamW(torch.optim.Optimizer):
             return st["exp_avg"].clone(), st["exp_avg_sq"].clone()
         spread = lambda s: s.repeat_interleave(BLOCK)[:p.numel()]  # noqa: E731
         m = st["exp_avg"].float() * spread(st["exp_avg_scale"])
-        r = st["exp_avg_sq_root"].float() * spread(st["exp_avg_sq_root_scale"])
+        root = st["exp_avg_sq_root"]
+        r = root.float() * spread(st["exp_avg_sq_root_scale"])
+        r.masked_fill_(root.view(torch.uint8) == 0xFF, float("inf"))
         return m.view(p.shape), r.square().view(p.shape)

@@ -298,3 +298,60 @@ def test_numbers_made_on_the_device_are_checked():
         opt.param_groups[0]["step"] = bad
         with pytest.raises(ValueError):
             opt.step()
+
+
+def _state8(n):
+    z = lambda: torch.zeros(n, dtype=torch.uint8, device=dev()).view(torch.float8_e4m3fn)  # noqa: E731
+    return z(), z(), (torch.zeros(-(-n // 256), device=dev()), torch.zeros(-(-n // 256), device=dev()))
+
+
+@gpu
+@pytest.mark.parametrize("n", [256, 300, 2048])
+def test_a_second_moment_beyond_32_bits(n):
+    """A finite gradient whose square is not: m / sqrt(v) is 0 then and stays it, as with 32-bit moments."""
+    import sparsecore_b200 as sl
+
+    kw = dict(lr=1e-3, betas=(0.9, 0.99), weight_decay=0.1)
+    g = torch.Generator().manual_seed(n)
+    p0 = torch.randn(n, generator=g).to(dev())
+    gr = torch.randn(n, generator=g).to(dev())
+    p8, p32 = p0.clone(), p0.clone()
+    m8, v8, s = _state8(n)
+    m32, v32 = torch.zeros(n, device=dev()), torch.zeros(n, device=dev())
+    big = torch.zeros(n, dtype=torch.bool, device=dev())
+    big[7] = big[n - 1] = True
+    for step in (1, 2, 3, 4):
+        now = torch.where(big, 3e19 if step == 1 else 0.5, gr)
+        sl.adamw_step([p8], [now], [m8], [v8], step=step, scales=[s], **kw)
+        sl.adamw_step([p32], [now], [m32], [v32], step=step, **kw)
+        assert torch.isfinite(p8).all() and torch.isfinite(s[0]).all() and torch.isfinite(s[1]).all()
+        assert torch.equal(p8[big], p32[big])
+        assert torch.isinf(v32[big]).all()
+    opt = sl.FusedAdamW([p8.requires_grad_()], state_bits=8)
+    opt.state[p8].update(exp_avg=m8, exp_avg_sq_root=v8, exp_avg_scale=s[0], exp_avg_sq_root_scale=s[1])
+    m, v = opt.state_values(p8)
+    assert torch.equal(torch.isinf(v), big) and torch.isfinite(m).all()
+
+
+@gpu
+@pytest.mark.parametrize("n", [512, 4096])
+@pytest.mark.parametrize("eps", [0.0, 1e-8])
+def test_second_moments_below_the_normal_range(n, eps):
+    """Gradients of 1e-20: v is subnormal, its root is not.  One step from nothing, in 32-bit operations: 16 roundings
+    (the root of a subnormal v is taken of the rounded v)."""
+    import sparsecore_b200 as sl
+
+    g = torch.Generator().manual_seed(8)
+    gr = (torch.rand(n, generator=g).double() * 4e-20 + 1e-21).float().to(dev())
+    gr[256:300] = 0.3  # a block with ordinary ones beside them
+    p = torch.zeros(n, device=dev())
+    m, v, s = _state8(n)
+    sl.adamw_step([p], [gr], [m], [v], step=1, scales=[s], lr=1.0, betas=(0.9, 0.99), eps=eps, weight_decay=0.0)
+    root = (gr * gr * torch.tensor(1 - 0.99, device=dev())).sqrt()
+    m1 = gr * torch.tensor(1 - 0.9, device=dev())
+    want = -(m1.double() / (1 - 0.9)) / (root.double() / math.sqrt(1 - 0.99) + eps)
+    assert bool(((p.double() - want).abs() <= 16 * 2.0 ** -24 * want.abs()).all())
+    top = root.view(-1, 256).amax(1).clamp_min(2.0 ** -100)
+    torch.testing.assert_close(s[1], top / 448, rtol=1e-6, atol=0)
+    held, step = v.float() * s[1].repeat_interleave(256), s[1].repeat_interleave(256) * 2.0 ** -9
+    assert bool(((held - root).abs() <= root / 8 * 1.001 + step).all()) and bool((held > 0).all())
