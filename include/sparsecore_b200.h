@@ -492,6 +492,11 @@ SL_API int sl_xent_sizes(const sl_xent_args* args, int64_t* prep, int64_t* forwa
 SL_API int sl_xent_forward(const sl_xent_args* args, void* stream);
 SL_API int sl_xent_backward(const sl_xent_args* args, void* stream);
 
+/* Kernels that this thread's last sl_xent_forward / backward,
+ * sl_norm_backward or sl_adamw_multi call launched (their number depends on the
+ * arguments). */
+SL_API int64_t sl_last_launches(void);
+
 #ifdef __cplusplus
 }
 #endif

@@ -104,6 +104,7 @@ SIGNATURES: dict[str, tuple] = {
     "sl_xent_sizes": (I32, [P, P, P, P]),
     "sl_xent_forward": (I32, [P, P]),
     "sl_xent_backward": (I32, [P, P]),
+    "sl_last_launches": (I64, []),
     "sl_set_regrow_draws": (I32, [P, P, P, I64, P, P, I64, P, P, I64, P]),
 }
 
@@ -172,7 +173,8 @@ def ptr(t: torch.Tensor | None) -> P:
     return P(t.data_ptr()) if t is not None else P(0)
 
 
-# Kernels each entry point launches (for launch accounting).
+# Kernels each entry point launches (for launch accounting); None where their number depends on the arguments and the
+# library counts them (sl_last_launches).
 KERNELS_PER_CALL = {
     "sl_spmm_fwd": 1, "sl_spmm_fwd_gelu": 1, "sl_spmm_fwd_act": 1, "sl_transpose_bias_f32": 1, "sl_sddmm_dw": 1, "sl_transpose_count": 3, "sl_transpose_fill": 2,
     "sl_transpose_with_perm_noalloc": 5,
@@ -183,8 +185,8 @@ KERNELS_PER_CALL = {
     "sl_unpack_live_batch": 1, "sl_exclusive_scan": 1,
     "sl_set_regrow_draws": 0,  # host only
     "sl_probe_ffma": 1, "sl_probe_smem": 1,
-    "sl_adamw_multi": 1, "sl_adamw_hyper": 1, "sl_norm_forward": 1, "sl_norm_backward": 2,
-    "sl_xent_sizes": 0, "sl_xent_forward": 3, "sl_xent_backward": 3,
+    "sl_adamw_multi": None, "sl_adamw_hyper": 1, "sl_norm_forward": 1, "sl_norm_backward": None,
+    "sl_xent_sizes": 0, "sl_xent_forward": None, "sl_xent_backward": None,
 }
 launches = {"count": 0}
 
@@ -199,7 +201,7 @@ def call(name: str, *args) -> None:
     if got is None or got[0] is not lb:
         got = _fns[name] = (lb, getattr(lb, name), KERNELS_PER_CALL.get(name, 1))
     rc = got[1](*args)
-    launches["count"] += got[2]
+    launches["count"] += lb.sl_last_launches() if got[2] is None else got[2]
     if rc:
         check(rc, name)
 

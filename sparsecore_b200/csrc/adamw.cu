@@ -470,6 +470,7 @@ int launch(const sl_adamw_item* items, int64_t count, const Hyper& h, const Hype
         if (t.count == 0) continue;
         const int64_t cap = static_cast<int64_t>(num_sms()) * 8;
         const int64_t grid = t.tiles < cap ? t.tiles : cap;
+        ++g_launched;
         adamw_multi_kernel<T, EIGHT, MAX><<<static_cast<unsigned>(grid), kThreads, 0, s>>>(t, h, dev);
         SL_RETURN_IF_LAUNCH_FAILED("sl_adamw_multi");
     }
@@ -503,6 +504,7 @@ extern "C" int sl_adamw_multi(const sl_adamw_item* items, int64_t count, int dty
                               double beta1, double beta2, double eps, double weight_decay, int64_t step, uint32_t seed,
                               const void* hyper_dev, void* stream) {
     const char* fn = "sl_adamw_multi";
+    g_launched = 0;
     SL_REQUIRE(count >= 0, fn, "negative count");
     SL_REQUIRE(known_dtype(dtype), fn, "unknown dtype");
     SL_REQUIRE(state_bits == 8 || state_bits == 32, fn, "state_bits must be 8 or 32");

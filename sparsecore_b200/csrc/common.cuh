@@ -19,6 +19,8 @@ void note_kernel(const char* name);
 int fail(int code, const std::string& msg);
 // SL_OK, or SL_ERR_CUDA with the runtime's message prefixed by `what`.
 int cuda_status(cudaError_t e, const char* what);
+// Kernels launched by this thread's last call of those that count them.
+extern thread_local int64_t g_launched;
 // SM count of the current device (cached per device).
 int num_sms();
 

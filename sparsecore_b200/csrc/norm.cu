@@ -58,6 +58,7 @@ extern "C" int sl_norm_forward(const sl_norm_args* n, void* stream) {
 }
 
 extern "C" int sl_norm_backward(const sl_norm_args* n, void* stream) {
+    g_launched = 0;
     if (int rc = check(n, "sl_norm_backward", true)) return rc;
     if (n->rows == 0) return SL_OK;
     if (n->dtype == SL_F32) return norm_backward<float>(*n, as_stream(stream));

@@ -1098,6 +1098,7 @@ int backward(const sl_norm_args& n, cudaStream_t s) {
                 if (bytes > 40 * 1024)  // with what the kernel has besides, beyond the default
                     if (int e = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)), "sl_norm_backward"))
                         return e;
+                ++g_launched;
                 kernel<<<grid, block, bytes, s>>>(a, stages);
                 SL_RETURN_IF_LAUNCH_FAILED("sl_norm_backward");
                 return static_cast<int>(SL_OK);
@@ -1113,6 +1114,7 @@ int backward(const sl_norm_args& n, cudaStream_t s) {
     } else {
         const size_t join = block.y > 1 ? 2 * sizeof(float) * n.cols : 0;
         rc = with_plan<TY>(p, [&](auto ve, auto nv) {
+            ++g_launched;
             norm_bwd_kernel<TY, TR, ve, nv><<<grid, block, join, s>>>(a);
             SL_RETURN_IF_LAUNCH_FAILED("sl_norm_backward");
             return static_cast<int>(SL_OK);
@@ -1130,6 +1132,7 @@ int backward(const sl_norm_args& n, cudaStream_t s) {
     if (!any) return SL_OK;
     const int64_t groups = std::max<int64_t>(1, l.r[4].groups);
     const dim3 grid2(static_cast<unsigned>((a.D + 31) / 32), static_cast<unsigned>(std::min<int64_t>(groups, 4096)), 6);
+    ++g_launched;
     norm_reduce_kernel<TY><<<grid2, dim3(32, 32), 0, s>>>(l);
     SL_RETURN_IF_LAUNCH_FAILED("sl_norm_backward");
     return SL_OK;

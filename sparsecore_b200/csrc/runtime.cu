@@ -12,6 +12,7 @@ namespace slb {
 
 thread_local std::string g_last_error;
 thread_local const char* g_last_kernel = "";
+thread_local int64_t g_launched = 0;
 
 void set_error(const std::string& msg) { g_last_error = msg; }
 void note_kernel(const char* name) { g_last_kernel = name; }
@@ -238,6 +239,8 @@ extern "C" {
 const char* sl_last_error(void) { return slb::g_last_error.c_str(); }
 
 const char* sl_last_kernel(void) { return slb::g_last_kernel; }
+
+int64_t sl_last_launches(void) { return slb::g_launched; }
 
 const char* sl_version(void) { return "sparsecore_b200 0.1.0 (sm_100a)"; }
 

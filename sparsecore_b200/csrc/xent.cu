@@ -436,6 +436,7 @@ extern "C" int sl_xent_sizes(const sl_xent_args* a, int64_t* prep, int64_t* forw
 }
 
 extern "C" int sl_xent_forward(const sl_xent_args* a, void* stream) {
+    g_launched = 0;
     if (int rc = xent::check(a, "sl_xent_forward")) return rc;
     if (a->tokens == 0) return SL_OK;
     SL_REQUIRE(a->reduction == SL_XENT_NONE ? a->loss_rows != nullptr : a->loss != nullptr, "sl_xent_forward", "NULL loss");
@@ -443,6 +444,7 @@ extern "C" int sl_xent_forward(const sl_xent_args* a, void* stream) {
 }
 
 extern "C" int sl_xent_backward(const sl_xent_args* a, void* stream) {
+    g_launched = 0;
     if (int rc = xent::check(a, "sl_xent_backward")) return rc;
     if (a->tokens == 0) return SL_OK;
     SL_REQUIRE(a->grad != nullptr && a->train, "sl_xent_backward", "NULL gradient, or a forward call without train");

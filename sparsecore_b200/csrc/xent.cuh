@@ -30,6 +30,7 @@ void launch_following(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, 
     c.stream = s;
     c.attrs = &early;
     c.numAttrs = 1;
+    ++g_launched;
     cudaLaunchKernelEx(&c, kernel, std::forward<A>(a)...);  // errors: cudaGetLastError, as of any launch
 }
 
