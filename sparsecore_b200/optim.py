@@ -193,14 +193,16 @@ class AdamWPlan:
             return
         if hyper is not None:
             _check_numbers(hyper, self.device)
+        self._launch(*self._take(grads), lr, betas, eps, weight_decay, step, seed, hyper)
+
+    def _take(self, grads):
+        """(which parameters take the step, None for all; their gradients as the kernel reads them), checked."""
         if list(map(_get_ptr, self._flat)) != self._ptrs:
             self._build()
         given = grads
         if any(g is None for g in grads):
             on = [i for i, g in enumerate(grads) if g is not None]
             given = [grads[i] for i in on]
-            if not given:
-                return
             sizes, dtypes = [self._sizes[i] for i in on], [self._dtypes[i] for i in on]
         else:
             on, sizes, dtypes = None, self._sizes, self._dtypes
@@ -209,9 +211,12 @@ class AdamWPlan:
             every = range(len(grads)) if on is None else on
             sizes, dtypes = [self._sizes[i] for i in every], [self._dtypes[i] for i in every]
         if (list(map(_get_dtype, given)) != dtypes or list(map(_get_numel, given)) != sizes
-                or set(map(_get_device, given)) != {self.device.index} or not all(map(_is_contiguous, given))):
+                or not set(map(_get_device, given)) <= {self.device.index} or not all(map(_is_contiguous, given))):
             given = self._fit(given, sizes, dtypes)
-        ptrs = np.zeros(len(grads), np.uint64)
+        return on, given
+
+    def _launch(self, on, given, lr, betas, eps, weight_decay, step, seed, hyper):
+        ptrs = np.zeros(len(self.params), np.uint64)
         ptrs[slice(None) if on is None else on] = list(map(_get_ptr, given))
         bits = 32 if self.scales is None else 8
         with_step = (float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
@@ -361,26 +366,28 @@ class FusedAdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         cols = self._columns()
-        used = set()
+        used, stepped = set(), set()
         for k, group in enumerate(self.param_groups):
             params = [p for p in group["params"] if p.grad is not None]
             if not params:
                 continue
             if not self.capturable and params[0].is_cuda and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("FusedAdamW: a captured step needs capturable=True (its replays would repeat one step's numbers)")
+            stepped.add(k)
             for j, (count, members, holders) in enumerate(self._counted(group, params)):
                 used.add((k, j))
                 plan = self._plan((k, j), group, members, cols)
                 grads = [p.grad for p in members]
                 if self.capturable:
-                    plan.step(grads, seed=self.seed, hyper=self._advance((k, j), count, group, plan.device))
+                    taken = plan._take(grads)  # what is refused is refused before it is counted
+                    plan._launch(*taken, 0.0, group["betas"], 0.0, 0.0, None, self.seed, self._advance((k, j), count, group, plan.device))
                     continue
                 plan.step(grads, step=count + 1, lr=group["lr"], betas=group["betas"], eps=group["eps"],
                           weight_decay=group["weight_decay"], seed=self.seed)
                 for h in holders:
                     h["step"] = count + 1
         if len(self._plans) > len(used):  # of counts that are no more
-            self._plans = {key: plan for key, plan in self._plans.items() if key in used}
+            self._plans = {key: plan for key, plan in self._plans.items() if key in used or key[0] not in stepped}
         return loss
 
     def _counted(self, group, params):

@@ -355,3 +355,31 @@ def test_second_moments_below_the_normal_range(n, eps):
     torch.testing.assert_close(s[1], top / 448, rtol=1e-6, atol=0)
     held, step = v.float() * s[1].repeat_interleave(256), s[1].repeat_interleave(256) * 2.0 ** -9
     assert bool(((held - root).abs() <= root / 8 * 1.001 + step).all()) and bool((held > 0).all())
+
+
+@gpu
+def test_groups_that_take_turns_keep_their_tables():
+    """And a step that is refused counts for nothing."""
+    import sparsecore_b200 as sl
+
+    for capturable in (False, True):
+        a, b = _params(1), _params(2)
+        opt = sl.FusedAdamW([{"params": a}, {"params": b}], lr=1e-2, capturable=capturable)
+        seen = []
+        for step in range(6):
+            now, rest = (a, b) if step % 2 == 0 else (b, a)
+            _grads(now, step, {0, 1, 2})
+            _grads(rest, step, set())
+            opt.step()
+            seen.append(dict(opt._plans))
+        assert seen[1] == seen[5]
+        _grads(a, 7, {0, 1, 2})
+        _grads(b, 7, set())
+        a[1].grad = None
+        a[1].data = a[1].data[:5]  # its moments are longer
+        count, keep = int(opt.param_groups[0]["step"]), a[0].detach().clone()
+        a[1].grad = torch.ones(5, device=dev())
+        opt.state[a[1]]["exp_avg"].data = torch.zeros(5, device=dev())
+        with pytest.raises(ValueError):
+            opt.step()
+        assert int(opt.param_groups[0]["step"]) == count and torch.equal(a[0], keep)
