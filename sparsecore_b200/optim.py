@@ -209,9 +209,8 @@ class AdamWPlan:
         if list(map(_get_numel, given)) != sizes or list(map(_get_dtype, given)) != dtypes:
             self._build()  # maybe a parameter was cut or given another type where it lies
             every = range(len(grads)) if on is None else on
-            sizes, dtypes = [self._sizes[i] for i in every], [self._dtypes[i] for i in every]
-        if (list(map(_get_dtype, given)) != dtypes or list(map(_get_numel, given)) != sizes
-                or not set(map(_get_device, given)) <= {self.device.index} or not all(map(_is_contiguous, given))):
+            given = self._fit(given, [self._sizes[i] for i in every], [self._dtypes[i] for i in every])
+        elif not set(map(_get_device, given)) <= {self.device.index} or not all(map(_is_contiguous, given)):
             given = self._fit(given, sizes, dtypes)
         return on, given
 
