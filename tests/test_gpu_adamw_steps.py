@@ -383,3 +383,28 @@ def test_groups_that_take_turns_keep_their_tables():
         with pytest.raises(ValueError):
             opt.step()
         assert int(opt.param_groups[0]["step"]) == count and torch.equal(a[0], keep)
+
+
+@gpu
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("n", [300, 2048])
+def test_neighbours_of_what_is_not_finite_are_what_they_would_be(n, bad):
+    """Bit for bit: the largest of the block, which its scale is of, is another element."""
+    import sparsecore_b200 as sl
+
+    g = torch.Generator().manual_seed(12)
+    p0, gr = torch.randn(n, generator=g).to(dev()), torch.randn(n, generator=g).to(dev())
+    gr[9] = 20.0
+    runs = []
+    for value in (0.5, bad):
+        p, (m, v, s) = p0.clone(), _state8(n)
+        now = gr.clone()
+        now[7] = value
+        for step in (1, 2, 3):
+            sl.adamw_step([p], [now], [m], [v], step=step, scales=[s], lr=1e-2)
+            now[7] = 0.5
+        runs.append((p, m.view(torch.uint8), v.view(torch.uint8), *s))
+    rest = torch.arange(n, device=dev()) != 7
+    assert all(torch.equal(a[rest], b[rest]) for a, b in zip(runs[0][:3], runs[1][:3]))
+    assert torch.equal(runs[0][3], runs[1][3]) and torch.equal(runs[0][4], runs[1][4])
+    assert torch.isnan(runs[1][0][7]) and torch.isfinite(runs[0][0]).all()
