@@ -251,9 +251,9 @@ def check_device_status(device: torch.device | int | None = None, sync: bool = T
     """Read and clear the library's device status word; raise if a bounded
     device-side wait gave up since the last check.
 
-    The TMA-fed kernels (X-stationary forward, tiled SDDMM) bound every
-    mbarrier wait.  A wait that runs out raises bit 0 of a per-device status
-    word and the kernel returns early, so its output (Y or dW) is incomplete;
+    The TMA-fed kernels (X-stationary forward, tiled SDDMM, the products of
+    the linear cross entropy) bound every mbarrier wait.  A wait that runs out raises bit 0 of a per-device status
+    word and the kernel returns early, so its output is incomplete;
     the C call itself has already returned SL_OK by then.  This check turns
     that bit into ``RuntimeError`` (the C-ABI's SL_ERR_TIMEOUT).  It costs a
     device synchronisation (``sync=True``) plus a 4-byte read, so callers run

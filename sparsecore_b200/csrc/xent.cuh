@@ -36,7 +36,9 @@ void launch_following(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, 
 
 constexpr int kPart = 128;          // vocabulary columns of one partial (max, sum) of a row
 constexpr int64_t kMostSlabFloats = int64_t(16) << 20;  // sums that a split product may leave to be joined
-constexpr float kGradScale = 32768.f;  // softmax - onehot is held in fp16 times 2^15
+// softmax - onehot is held in fp16 times 2^15: in two planes 22 bits of what is
+// above 2^-17, and what is below to within 2^-40.
+constexpr float kGradScale = 32768.f;
 
 // First bytes of the `prep` buffer.
 struct Header {
@@ -49,9 +51,9 @@ enum : int { kIgnored = -1, kInvalid = -2 };  // in place of a target
 
 // Exponent of the power of two that brings values of up to `bits` (a float's
 // bits, subnormal ones too) into [2^14, 2^15): -113 to 163.  Two fp16 planes
-// then hold 22 bits of what is down to 2^-17 of the largest, and 2^-39 of the
-// largest of what is smaller: an operand is as exact as its largest values ask
-// for, not element by element.
+// then hold 22 bits of what is above 2^-17 of the largest, and what is smaller
+// to within 2^-39 of the largest: an operand is as exact as a sum with its
+// largest values in it can be, not element by element.
 __device__ __forceinline__ int plane_exponent(unsigned bits) {
     if (bits == 0) return 0;
     return 14 - (bits >= 0x800000u ? static_cast<int>(bits >> 23) - 127 : -118 - __clz(bits));

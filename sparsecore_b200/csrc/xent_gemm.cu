@@ -102,6 +102,7 @@ __device__ __forceinline__ void locate(const Args& a, int id, int& m, int& n, in
     n = id / rows;
 }
 
+// Off by 2^-22 at most, as much as the logits' own last bits make it.
 __device__ __forceinline__ float exp2_fast(float v) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -158,7 +159,9 @@ __device__ __forceinline__ void epilogue_stats(const Args& a, float (&z)[128], i
 }
 
 // 128 columns of G (less the `one` of the target column `at`), as planes:
-// v = e * c, from e in z.
+// v = e * c, from e in z.  An MMA has both operands of one type, so G of 16-bit
+// operands is rounded to theirs (half a step, 2^-9 or 2^-12 of an element and without
+// a sign; the gradients are rounded to the same type in the end).
 template <int PL>
 __device__ __forceinline__ void store_grad(const Args& a, const float (&z)[128], int64_t t, int64_t n0, float c, int at, float one) {
     const int64_t room = min(static_cast<int64_t>(128), a.g_stride - n0);

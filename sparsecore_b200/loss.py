@@ -133,6 +133,12 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     where none does, with gradients of zero), "sum", or "none" (a loss for each
     token, 0 for ignored ones).  The loss is float32.
 
+    Digits: a float32 operand is held as two fp16 planes under one power of two,
+    22 bits of each element above 2^-17 of the operand's largest, smaller ones to
+    within 2^-39 of the largest; softmax - onehot has 22 bits above 2^-17, and is
+    held to within 2^-40 below.  For 16-bit operands it is rounded to their type
+    before it is multiplied.  Sums are float32.
+
     Raises TypeError (not tensors), RuntimeError (not on one CUDA device,
     forward-mode derivatives) and ValueError (shapes, types, reduction).
     """

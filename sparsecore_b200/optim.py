@@ -293,6 +293,7 @@ class FusedAdamW(torch.optim.Optimizer):
     Each parameter's moments are corrected by the steps that it has taken itself,
     as in torch's AdamW: one that begins late, misses steps or is drawn again is
     stepped by its own count (in a launch of its own for each different count).
+    Parameters are contiguous, and those of a group on one device.
     """
 
     def __init__(self, model_or_params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
